@@ -350,6 +350,52 @@ const char* qw4_st_last_error(void);
 int qw4_load_ct_fused(qw4_weights* w, const qw4_st* st, const char* const* prefixes,
                       int nparts, int in_f, int group_size, void* stream);
 
+/* ------------------------------------------------------- layers of experts
+ * A token's feed-forward spread over experts (no reference counterpart: its
+ * model is dense). Four calls make the layer:
+ *   qw4_route         top_k experts of each token, and the plan
+ *   qw4_gemm_grouped  gate|up of every chosen expert, with QW4_ACT_SWIGLU
+ *   qw4_gemm_grouped  down
+ *   qw4_combine       the weighted sum of each token's rows
+ * A "pair" is (token t, slot j), numbered t top_k + j. The plan groups the pairs
+ * by expert, in pair order, so that expert e owns the positions [offsets[e],
+ * offsets[e + 1]); the products read and write rows in that order. All of it
+ * stays on the device: no call synchronizes. */
+typedef struct qw4_plan {
+  int32_t* offsets;        /* [experts + 1]                                        */
+  int32_t* tokens;         /* [max_pairs] token at each position, -1 behind the last */
+  int32_t* pos;            /* [max_pairs] position of each pair, -1: no expert     */
+  int32_t experts, max_pairs;
+} qw4_plan;
+
+/* Device arrays for `experts` (1..1024) and at most max_pairs pairs. A caller may
+ * also fill the struct with arrays of its own. */
+int qw4_plan_alloc(qw4_plan* plan, int experts, int max_pairs);
+int qw4_plan_free(qw4_plan* plan);
+
+/* The router: ids [T][top_k] and weights [T][top_k] of the top_k (1..16, at most
+ * experts) largest of each token's logits [T][experts], largest first, the lower
+ * expert among equals. -Inf (a masked expert) and NaN are never chosen: a token
+ * with fewer experts left gets id -1 and weight 0 in its last slots. Weights are
+ * the softmax in fp32 over the chosen experts (renorm != 0) or over all of them;
+ * experts at +Inf share the whole weight. plan (may be NULL) receives the
+ * grouping of the T top_k pairs; plan->experts must equal experts. T = 0 gives
+ * an empty plan. */
+int qw4_route(int32_t* ids, float* weights, const qw4_plan* plan, const uint16_t* logits, int T,
+              int experts, int top_k, int renorm, void* stream);
+int qw4_route_f32(int32_t* ids, float* weights, const qw4_plan* plan, const float* logits, int T,
+                  int experts, int top_k, int renorm, void* stream);
+/* The plan alone, for ids [T][top_k] from another rule; an id outside [0,
+ * plan->experts) has no expert here (on this GPU). */
+int qw4_route_ids(const qw4_plan* plan, const int32_t* ids, int T, int top_k, void* stream);
+
+/* out [T][dim] = bf16(residual + sum_j weights[t][j] y[plan->pos[t top_k + j]]), in
+ * fp32, slots in order; y [T top_k][dim] bf16 in plan order, pairs without an
+ * expert add nothing. residual [T][dim] (may be NULL, may be out). dim % 8 == 0;
+ * out, y and residual 16-byte aligned. */
+int qw4_combine(uint16_t* out, const uint16_t* y, const qw4_plan* plan, const float* weights, int T,
+                int top_k, int dim, const uint16_t* residual, void* stream);
+
 /* ------------------------------------------------- synthetic inputs
  * Device-side generator for the benchmark (no reference counterpart). The
  * counter-based spec is documented with the generator kernel:

@@ -162,4 +162,17 @@ void gemv_w4a16_rmsnorm(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bf
 void linear_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int T,
                   GemvScratch& s, GemmWorkspace& ws, hipStream_t stream = 0);
 
+// Layers of experts (no reference counterpart; qwen_w4a16.h describes the plan).
+void expert_plan_alloc(qw4_plan& plan, int experts, int max_pairs);
+void expert_plan_free(qw4_plan& plan);
+void route_experts(int32_t* ids, float* weights, const qw4_plan* plan, const __hip_bfloat16* logits,
+                   int T, int experts, int top_k, bool renorm, hipStream_t stream = 0);
+void route_experts_f32(int32_t* ids, float* weights, const qw4_plan* plan, const float* logits, int T,
+                       int experts, int top_k, bool renorm, hipStream_t stream = 0);
+void route_expert_ids(const qw4_plan& plan, const int32_t* ids, int T, int top_k,
+                      hipStream_t stream = 0);
+void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_plan& plan,
+                     const float* weights, int T, int top_k, int dim, const __hip_bfloat16* residual,
+                     hipStream_t stream = 0);
+
 }  // namespace qwen

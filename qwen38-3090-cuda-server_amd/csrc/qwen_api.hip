@@ -283,4 +283,32 @@ void linear_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16
   check(qw4_linear(u16(y), &v, u16(x), T, &s.impl, &q, stream), "linear_w4a16");
 }
 
+void expert_plan_alloc(qw4_plan& plan, int experts, int max_pairs) {
+  check(qw4_plan_alloc(&plan, experts, max_pairs), "expert_plan_alloc");
+}
+
+void expert_plan_free(qw4_plan& plan) { check(qw4_plan_free(&plan), "expert_plan_free"); }
+
+void route_experts(int32_t* ids, float* weights, const qw4_plan* plan, const __hip_bfloat16* logits,
+                   int T, int experts, int top_k, bool renorm, hipStream_t stream) {
+  check(qw4_route(ids, weights, plan, u16(logits), T, experts, top_k, renorm, stream), "route_experts");
+}
+
+void route_experts_f32(int32_t* ids, float* weights, const qw4_plan* plan, const float* logits, int T,
+                       int experts, int top_k, bool renorm, hipStream_t stream) {
+  check(qw4_route_f32(ids, weights, plan, logits, T, experts, top_k, renorm, stream),
+        "route_experts_f32");
+}
+
+void route_expert_ids(const qw4_plan& plan, const int32_t* ids, int T, int top_k, hipStream_t stream) {
+  check(qw4_route_ids(&plan, ids, T, top_k, stream), "route_expert_ids");
+}
+
+void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_plan& plan,
+                     const float* weights, int T, int top_k, int dim, const __hip_bfloat16* residual,
+                     hipStream_t stream) {
+  check(qw4_combine(u16(out), u16(y), &plan, weights, T, top_k, dim, u16(residual), stream),
+        "combine_experts");
+}
+
 }  // namespace qwen

@@ -47,7 +47,8 @@ EXPORTS = (
     "qw4_rmsnorm", "qw4_residual_add", "qw4_swiglu", "qw4_gemv_residual", "qw4_gemv_swiglu",
     "qw4_gemv_rmsnorm", "qw4_linear", "qw4_linear_max_t", "qw4_mfma_peak", "qw4_tune_decode",
     "qw4_tune_gemm", "qw4_tune_linear", "qw4_gemv_argmax_noalloc",
-    "qw4_quantize_w4a16",
+    "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
+    "qw4_route_ids", "qw4_combine",
 )
 
 # safetensors dtype order (qw4_st_tensor.dtype)
@@ -101,6 +102,12 @@ class GemmWorkspace(C.Structure):
     _fields_ = [("buf", C.c_void_p), ("bytes", C.c_size_t)]
 
 
+class ExpertPlan(C.Structure):
+    """qw4_plan: pairs (token, slot) grouped by expert."""
+    _fields_ = [("offsets", C.c_void_p), ("tokens", C.c_void_p), ("pos", C.c_void_p),
+                ("experts", C.c_int32), ("max_pairs", C.c_int32)]
+
+
 class StTensor(C.Structure):
     """qw4_st_tensor: one tensor of an open safetensors set (host view)."""
     _fields_ = [("dtype", C.c_int32), ("ndim", C.c_int32), ("shape", C.c_int64 * 8),
@@ -121,6 +128,7 @@ def lib():
     vp, i, sz, u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
     W, S, WS = C.POINTER(W4A16Weights), C.POINTER(GemvScratch), C.POINTER(GemmWorkspace)
     W8 = C.POINTER(W8A16Weights)
+    PL = C.POINTER(ExpertPlan)
     sig = {
         "qw4_status_string": ([i], C.c_char_p),
         "qw4_last_hip_error": ([], i),
@@ -177,6 +185,12 @@ def lib():
         "qw4_gemv_argmax_noalloc": ([vp, W, vp, i, vp], i),
         "qw4_quantize_w4a16": ([W, vp, i, i, i, vp], i),
         "qw4_tune_linear": ([i], i),
+        "qw4_plan_alloc": ([PL, i, i], i),
+        "qw4_plan_free": ([PL], i),
+        "qw4_route": ([vp, vp, PL, vp, i, i, i, i, vp], i),
+        "qw4_route_f32": ([vp, vp, PL, vp, i, i, i, i, vp], i),
+        "qw4_route_ids": ([PL, vp, i, i, vp], i),
+        "qw4_combine": ([vp, vp, PL, vp, i, i, i, vp, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -534,6 +548,69 @@ def argmax_rows(out, x, rows: int, n: int, stream=None) -> None:
     _need(out, rows * 4, "argmax_rows out")
     _need(x, rows * n * 2, "argmax_rows x")
     _chk(lib().qw4_argmax_rows(_ptr(out), _ptr(x), rows, n, _stream(stream)), "argmax_rows")
+
+
+# ------------------------------------------------------ layers of experts
+def expert_plan_alloc(experts: int, max_pairs: int) -> ExpertPlan:
+    """qw4_plan_alloc: device arrays of the library."""
+    p = ExpertPlan()
+    _chk(lib().qw4_plan_alloc(C.byref(p), experts, max_pairs), "expert_plan_alloc")
+    return p
+
+
+def expert_plan_over(offsets, tokens, pos) -> ExpertPlan:
+    """A plan over int32 device tensors of the caller, which keeps them alive:
+    offsets [experts + 1], tokens and pos [max_pairs]."""
+    pairs = tokens.numel()
+    _need(pos, pairs * 4, "expert_plan_over pos")
+    for t in (offsets, tokens, pos):
+        if t.element_size() != 4 or not t.is_contiguous():
+            raise ValueError("expert_plan_over: contiguous int32 tensors needed")
+    return ExpertPlan(_ptr(offsets), _ptr(tokens), _ptr(pos), offsets.numel() - 1, pairs)
+
+
+def expert_plan_free(p: ExpertPlan) -> None:
+    """qw4_plan_free: for plans of expert_plan_alloc only."""
+    _chk(lib().qw4_plan_free(C.byref(p)), "expert_plan_free")
+
+
+def route_experts(ids, weights, logits, T: int, experts: int, top_k: int, renorm: bool,
+                  plan: ExpertPlan | None = None, stream=None) -> None:
+    """qw4_route: top_k experts of each token from bf16 logits, softmax weights, plan."""
+    _route(lib().qw4_route, 2, "route_experts", ids, weights, logits, T, experts, top_k, renorm, plan,
+           stream)
+
+
+def route_experts_f32(ids, weights, logits, T: int, experts: int, top_k: int, renorm: bool,
+                      plan: ExpertPlan | None = None, stream=None) -> None:
+    """qw4_route_f32: the same from fp32 logits."""
+    _route(lib().qw4_route_f32, 4, "route_experts_f32", ids, weights, logits, T, experts, top_k, renorm,
+           plan, stream)
+
+
+def _route(call, size, where, ids, weights, logits, T, experts, top_k, renorm, plan, stream):
+    _need(ids, T * top_k * 4, where)
+    _need(weights, T * top_k * 4, where)
+    _need(logits, T * experts * size, where)
+    _chk(call(_ptr(ids), _ptr(weights), C.byref(plan) if plan is not None else None, _ptr(logits), T,
+              experts, top_k, int(renorm), _stream(stream)), where)
+
+
+def route_expert_ids(plan: ExpertPlan, ids, T: int, top_k: int, stream=None) -> None:
+    """qw4_route_ids: the plan of ids [T][top_k] chosen elsewhere."""
+    _need(ids, T * top_k * 4, "route_expert_ids ids")
+    _chk(lib().qw4_route_ids(C.byref(plan), _ptr(ids), T, top_k, _stream(stream)), "route_expert_ids")
+
+
+def combine_experts(out, y, weights, T: int, top_k: int, dim: int, plan: ExpertPlan, residual=None,
+                    stream=None) -> None:
+    """qw4_combine: out = bf16(residual + sum_j weights[t][j] * y[pos of (t, j)])."""
+    _need(out, T * dim * 2, "combine_experts out")
+    _need(y, T * top_k * dim * 2, "combine_experts y")
+    _need(weights, T * top_k * 4, "combine_experts weights")
+    _need(residual, T * dim * 2, "combine_experts residual")
+    _chk(lib().qw4_combine(_ptr(out), _ptr(y), C.byref(plan), _ptr(weights), T, top_k, dim,
+                           _ptr(residual), _stream(stream)), "combine_experts")
 
 
 # ------------------------------------------------------ synthetic inputs
