@@ -39,7 +39,8 @@ enum {
   QW4_ERR_NOMEM = 8,       /* device allocation failed                           */
   QW4_ERR_LAYOUT = 9,      /* unknown source layout id                           */
   QW4_ERR_IO = 10,         /* file cannot be opened, mapped or parsed            */
-  QW4_ERR_NOTFOUND = 11    /* tensor absent from a safetensors file              */
+  QW4_ERR_NOTFOUND = 11,   /* tensor absent from a safetensors file              */
+  QW4_ERR_ACT = 12         /* unknown activation                                 */
 };
 
 const char* qw4_status_string(int status);
@@ -349,6 +350,26 @@ const char* qw4_st_last_error(void);
  * stream (the uploaded sources are freed before returning). */
 int qw4_load_ct_fused(qw4_weights* w, const qw4_st* st, const char* const* prefixes,
                       int nparts, int in_f, int group_size, void* stream);
+
+/* ------------------------------------------------- products with an epilogue
+ * No reference counterpart as one call. act is one of */
+enum {
+  QW4_ACT_NONE = 0,
+  QW4_ACT_SILU = 1,        /* v / (1 + exp(-v))                                    */
+  QW4_ACT_GELU = 2,        /* v (1 + erf(v / sqrt 2)) / 2                          */
+  QW4_ACT_GELU_TANH = 3,   /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2    */
+  QW4_ACT_SWIGLU = 4       /* a fused [gate | up] weight: silu(v_gate) v_up        */
+};
+/* y [T][width] = bf16(act(x [T][in_f] @ W^T + bias) + residual), fp32 up to the one
+ * rounding (the separate steps, and qw4_gemv_residual / _swiglu, round the
+ * projection to bf16 first). width = out_f; QW4_ACT_SWIGLU: out_f / 2, out_f % 128
+ * == 0. bias [out_f] and residual [T][width] bf16, each may be NULL; residual may be
+ * y. Any T >= 1, on qw4_linear's paths: whole weights in up to qw4_linear_max_t(w)
+ * rows with a scratch, weights rounded to bf16 (qw4_gemm) beyond or without one. s
+ * and ws may be NULL. All pointers 16-byte aligned. */
+int qw4_linear_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T,
+                        const uint16_t* bias, int act, const uint16_t* residual, qw4_scratch* s,
+                        qw4_workspace* ws, void* stream);
 
 /* ------------------------------------------------------- layers of experts
  * A token's feed-forward spread over experts (no reference counterpart: its

@@ -162,6 +162,12 @@ void gemv_w4a16_rmsnorm(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bf
 void linear_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int T,
                   GemvScratch& s, GemmWorkspace& ws, hipStream_t stream = 0);
 
+// y = bf16(act(x @ W^T + bias) + residual) for any T (act: QW4_ACT_*; bias and
+// residual may be null; no reference counterpart as one call).
+void linear_epilogue_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int T,
+                           const __hip_bfloat16* bias, int act, const __hip_bfloat16* residual,
+                           GemvScratch& s, GemmWorkspace& ws, hipStream_t stream = 0);
+
 // Layers of experts (no reference counterpart; qwen_w4a16.h describes the plan).
 void expert_plan_alloc(qw4_plan& plan, int experts, int max_pairs);
 void expert_plan_free(qw4_plan& plan);

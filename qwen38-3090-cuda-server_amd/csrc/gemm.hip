@@ -19,6 +19,7 @@
 #include <cstring>
 
 #include "../../include/qwen_w4a16.h"
+#include "gemm_tile.h"
 #include "w4a16_common.h"
 
 namespace qw4 {
@@ -26,35 +27,9 @@ int check_weights_public(const qw4_weights* w);
 
 namespace {
 
-// ---------------------------------------------------------------------------
-// k_gemm: 256 (M) x 256 (N) workgroup tile -- 32 MB (M) for MB = 2..7 m-blocks
-// where the rows do not fill 256 (gemm_plan) -- v_mfma_f32_32x32x16_bf16 (the
-// full-rate bf16 shape on gfx950). The default: 4 waves, one per SIMD, each a
-// whole 64-row weight tile against all the tile's activation rows (its 32 MB
-// accumulator registers in AGPRs); G2Split below lists the 8-wave forms.
-//
-//  * Weights are the MFMA A operand (rows = output columns n). Each wave loads
-//    its packed rows straight into registers -- 32 B per lane per group, one
-//    group ahead -- and dequantizes them in registers to exactly
-//    RNE((q - z) * s): every weight element is converted once per workgroup
-//    and never touches LDS.
-//  * Activations are the B operand. A group's 256 x 128 activation tile goes
-//    global -> LDS directly (global_load_lds_dwordx4), double-buffered, one
-//    instruction per 4 full rows (1 KiB, fully coalesced). LDS row m holds
-//    16-byte chunk c of the row at slot c ^ (m % 16): lane i of a load
-//    instruction writes slot i % 16 and so fetches chunk (i % 16) ^ (m % 16)
-//    (the XOR keeps each 4-lane group inside one 64-byte sector). The MFMA
-//    operand reads (32 rows x 16 B per half-wave) then hit distinct banks.
-//  * k permutation: lane l (row r = l % 32, half h = l / 32) of k-step (s, t)
-//    holds k = 64 s + 32 h + 8 t + e -- word t of chunk 2 s + h of its weight
-//    row -- and reads the activation chunk 8 s + 4 h + t, the same k.
-//  * Row permutation: MFMA row r of tile half b reads tile position
-//    p = 16 (r % 4) + 8 b + 2 (r / 8) + (r / 4) % 2, so the four D rows a lane
-//    holds for each r / 8 are four consecutive output columns (an 8-byte
-//    piece of a staged row, see g2_store_staged).
-constexpr int G2_BM = 256, G2_BN = 256;   // rows at most (32 MB of them, see G2Split), columns
-
-typedef float f32x16v __attribute__((ext_vector_type(16)));
+// Outputs of k_gemm: the product in bf16; with an epilogue; with an epilogue that
+// joins gate and up (C, residual and ld of half the weight's rows).
+enum { GEMM_PLAIN = 0, GEMM_EPI = 1, GEMM_GLU = 2 };
 
 struct GemmArgs {
   const uint32_t* qw;
@@ -70,123 +45,9 @@ struct GemmArgs {
   // XCD-contiguous runs over (k-slice, tile row-major), P / tiles slices
   int full;             // tiles [0, full) are done whole, P at a time
   int U;                // (tile, group) units of tiles [full, tiles), split over P
+  Epilogue epi;
+  int ld;               // row stride of C and the residual
 };
-
-// Work split of a workgroup's 4 weight tiles x 8 m-blocks over its NW waves:
-//  * NH = 1, NW = 8: a wave owns one 32-row tile half against all 8 m-blocks;
-//  * NH = 2, NW = 8: a wave owns a whole 64-row tile against 4 m-blocks (half
-//    the LDS reads per MFMA, every weight dequantized by two waves);
-//  * NH = 2, NW = 4: one wave per SIMD owns a whole tile against all 8
-//    m-blocks (half the LDS reads, every weight dequantized once; its 256
-//    accumulator registers take the AGPR half of the register file).
-// MB: 32-row m-blocks of the workgroup's tile, 8 unless fewer rows need it.
-template <int NH, int NW, int MB>
-struct G2Split {
-  static constexpr int MBW = 8 * MB / (NW * NH);     // m-blocks per wave
-  static constexpr int UNITS = NH * MBW;             // (half, m-block) pairs per wave
-  static constexpr int ACT = 8 * MB / NW;            // 1 KiB (4-row) activation loads per wave and group
-  static constexpr int FIXP = (UNITS + 1) / 2;       // fixup blocks per wave region
-  // groups buffered: as many 8 MB KiB activation buffers as LDS holds, 4 at most
-  // (MB = 5: three buffers spill 14 VGPRs, 60 bytes a lane, and are still faster
-  // than two without a spill: whole tiles 3%, split-K 1%, the others equal)
-  static constexpr int DEPTH = MB <= 4 ? 4 : MB == 5 ? 3 : 2;
-  // k-step schedule (measured on MI355X at the config-4 shapes): VALU slots
-  // after each MFMA, LDS operand reads after each of the first MFMAs, and the
-  // k-steps that carry the next group's activation loads.
-  static constexpr int VALU = NW == 8 ? 4 * NH : 2;
-  static constexpr int DS = 2;
-  static constexpr int ACTSTEPS = NW == 8 ? 4 : 8;
-  static_assert(MBW * NH * NW == 8 * MB && ACT * NW == 8 * MB, "unsupported split");
-  __device__ static void coords(int wave, int& wt, int& b0, int& mw) {
-    wt = NH == 1 ? (wave >> 1) : (wave & 3);   // tile of the 4 this wave owns
-    b0 = NH == 1 ? (wave & 1) : 0;             // first tile half
-    mw = NH == 1 ? 0 : (wave >> 2) * MBW;      // first m-block
-  }
-};
-
-template <int NH>
-struct WeightGroup {
-  u32x4 q[NH][2];    // [half][s]: chunk 2 s + h of this lane's weight row
-  uint32_t s[NH];    // scale bits
-  uint32_t z[NH];    // zero-point word (4 rows, 4 bits each)
-};
-
-// Buffer-resource addressing: a 32-bit per-lane offset (loop-invariant) plus
-// a scalar offset, instead of a 64-bit address per lane and load. Loads are
-// unconditional (an out-of-range wave reads the last tile and stores nothing),
-// and the zero-point word is kept raw: arithmetic on a loaded value here
-// would make the compiler wait for every earlier load, including the
-// activation loads just issued.
-struct G2Rsrc {
-  __amdgpu_buffer_rsrc_t qw, sc, zr;
-};
-
-// part j < NH: the packed words of tile half j; part NH: the scales and zero
-// points; part -1: everything.
-template <int NH>
-__device__ __forceinline__ void g2_load_weights(WeightGroup<NH>& wg, const G2Rsrc& rs, int G,
-                                                int tile, int b0, int g, int lane, int part = -1) {
-  const int r = lane & 31, h = lane >> 5;
-  const uint32_t blk = (uint32_t)tile * (uint32_t)G + (uint32_t)g;   // < 2^26
-#pragma unroll
-  for (int j = 0; j < NH; ++j) {
-    const int a16 = 8 * (b0 + j) + 2 * (r >> 3) + ((r >> 2) & 1);   // position % 16
-    const int p = 16 * (r & 3) + a16;
-    if (part < 0 || part == j) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        wg.q[j][s] = __builtin_amdgcn_raw_buffer_load_b128(rs.qw, ((2 * s + h) * 64 + p) * 16,
-                                                           blk * 4096u, 0);
-    }
-    if (part < 0 || part == NH) {
-      wg.s[j] = __builtin_amdgcn_raw_buffer_load_b16(rs.sc, (4 * a16 + (r & 3)) * 2, blk * (uint32_t)kMetaBytes, 0);
-      wg.z[j] = __builtin_amdgcn_raw_buffer_load_b16(rs.zr, a16 * 2, blk * 32u, 0);
-    }
-  }
-}
-
-// Issue activation load i of this wave (4 rows, 1 KiB) of group g into buf: row
-// block i NW + wave. `act` covers rows [m0, M); rows past M lie outside it and
-// read as zeros. voff is the lane's byte offset relative to a block's first
-// row: the swizzle repeats every 4 blocks, so it is the same for all of a
-// wave's.
-template <int NW>
-__device__ __forceinline__ void g2_load_act1(__amdgpu_buffer_rsrc_t act, uint32_t voff,
-                                             uint32_t row_bytes, u32x4* buf, int g, int wave,
-                                             int i) {
-  const int rb = i * NW + wave;
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(act, buf + rb * 64, 16,
-                                           voff + (uint32_t)(4 * rb) * row_bytes,
-                                           (uint32_t)g * (kGroup * 2), 0, 0);
-}
-
-// One packed word -> 8 bf16 weights RNE((q - z) s), c = -z s, in the order
-// of nib8_bits (register i: elements i and i + 4). The even nibbles are the
-// low nibbles of the bytes of w & 0x0F0F0F0F, the odd ones of (w >> 4): each
-// converts to fp32 in one v_cvt_f32_ubyteN, and fma(q, s, -z s) is exact
-// (both products have at most 12 significant bits) -- 23 VALU per word.
-__device__ __forceinline__ bf16x8 g2_deq(uint32_t w, float s, float c) {
-  const uint32_t ev = w & 0x0F0F0F0Fu, od = (w >> 4) & 0x0F0F0F0Fu;
-  float q[8];   // q[2 b] = byte b of ev, q[2 b + 1] = byte b of od
-  asm("v_cvt_f32_ubyte0 %0, %1" : "=v"(q[0]) : "v"(ev));
-  asm("v_cvt_f32_ubyte1 %0, %1" : "=v"(q[2]) : "v"(ev));
-  asm("v_cvt_f32_ubyte2 %0, %1" : "=v"(q[4]) : "v"(ev));
-  asm("v_cvt_f32_ubyte3 %0, %1" : "=v"(q[6]) : "v"(ev));
-  asm("v_cvt_f32_ubyte0 %0, %1" : "=v"(q[1]) : "v"(od));
-  asm("v_cvt_f32_ubyte1 %0, %1" : "=v"(q[3]) : "v"(od));
-  asm("v_cvt_f32_ubyte2 %0, %1" : "=v"(q[5]) : "v"(od));
-  asm("v_cvt_f32_ubyte3 %0, %1" : "=v"(q[7]) : "v"(od));
-  auto f = [&](int e) { return __builtin_fmaf(q[e], s, c); };
-  u32x4 o;
-  o[0] = pack_bf16x2(f(0), f(4));   // elements 0, 4 (bytes 0 and 2 of ev)
-  o[1] = pack_bf16x2(f(1), f(5));   // 1, 5
-  o[2] = pack_bf16x2(f(2), f(6));   // 2, 6
-  o[3] = pack_bf16x2(f(3), f(7));   // 3, 7
-  return __builtin_bit_cast(bf16x8, o);
-}
-
-// s_waitcnt vmcnt(0) (expcnt and lgkmcnt left at their maxima).
-__device__ __forceinline__ void g2_wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 // Linear tile index -> (tn, tm), in bands of 4 M-tiles: consecutive tiles
 // share an activation tile (and, 4 apart, a weight tile), so the ~32
@@ -204,91 +65,22 @@ __device__ __forceinline__ void g2_tile_coords(const GemmArgs& a, int t, int& tn
   tn = w / rows;
 }
 
-// Workgroups are dealt round-robin to the 8 XCDs (each with its own L2): XCD x
-// runs blocks x, x + 8, ... Renumber so that each XCD owns a contiguous run of
-// work. Needs count % 8 == 0 (then it is a bijection).
-__device__ __forceinline__ int g2_xcd_order(int blk, int count) {
-  return (blk & 7) * (count >> 3) + (blk >> 3);
-}
-
-// One group of a segment: the MFMAs of group g (its activation rows in buf, its
-// weights in cur) while the loads of a later group gn go out, activations into
-// nbuf and weights into nxt (actn, rsn: zero-length resources where there is no
-// such group -- they fetch nothing and need no branch, which would split the
-// k-step schedule).
-template <int NH, int NW, int MB>
-__device__ __forceinline__ void g2_group(const GemmArgs& a, f32x16v (&acc)[NH][G2Split<NH, NW, MB>::MBW],
-                                         const WeightGroup<NH>& cur, WeightGroup<NH>& nxt,
-                                         const u32x4* buf, u32x4* nbuf,
-                                         __amdgpu_buffer_rsrc_t actn, const G2Rsrc& rsn,
-                                         uint32_t voff, uint32_t row_bytes, int ltile, int b0, int gn,
-                                         int wave, int lane) {
-  using Sp = G2Split<NH, NW, MB>;
-  constexpr int MBW = Sp::MBW;
-  const int r = lane & 31, h = lane >> 5;
-  const int zsh = 4 * (r & 3);
-  // Group gn's activation rows spread evenly over the first Sp::ACTSTEPS
-  // k-steps below, so that what the workgroup writes into LDS per group does
-  // not arrive in one burst on top of the first steps' operand reads (8
-  // waves: steps 0-3, 4% faster than one burst and 1.5% than one load per
-  // step; 4 waves: all 8 steps, equal to steps 0-3); its weights in k-steps
-  // kWStep.. kWStep + NH (0.5-0.8% faster than all at the group's start, where
-  // they delay its first MFMA).
-  float sf[NH], cf[NH];
-#pragma unroll
-  for (int j = 0; j < NH; ++j) {
-    sf[j] = bf16_bits_to_f32(cur.s[j]);
-    cf[j] = -(float)((cur.z[j] >> zsh) & 0xFu) * sf[j];
+// What a wave of column tile tn computes: weight tile and first half, and the first
+// column of its output. Gated: a workgroup's 128 output columns are two gate tiles and
+// the up tiles `up` rows on; a wave takes one half of a gate tile and the same half of
+// its up tile, so that gate and up of a column meet in one lane.
+struct WaveTile {
+  int tile, b0, col;
+  bool valid;
+};
+template <int OUT>
+__device__ __forceinline__ WaveTile g2_wave_tile(const GemmArgs& a, int tn, int wt, int b0) {
+  if (OUT == GEMM_GLU) {
+    const int t = tn * 2 + (wt >> 1);
+    return {t, wt & 1, t * kTileN + 32 * (wt & 1), t * kTileN < a.ld};
   }
-  // Software pipeline over the group's 8 k-steps: the activation operands
-  // and the dequantized weight operands of step u + 1 are produced while
-  // step u's MFMAs run.
-  u32x4 xo[2][MBW];
-  bf16x8 wd[2][NH];
-#pragma unroll
-  for (int mb = 0; mb < MBW; ++mb) xo[0][mb] = buf[mb * 512 + ((4 * h) ^ (r & 15))];
-#pragma unroll
-  for (int j = 0; j < NH; ++j) wd[0][j] = g2_deq(cur.q[j][0][0], sf[j], cf[j]);
-  // Fence: the prologue's reads must not fill the DS slots of the pattern below.
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int cu = u & 1, nu = cu ^ 1;
-    constexpr int kWStep = 4;
-    if (u >= kWStep && u <= kWStep + NH)
-      g2_load_weights(nxt, rsn, a.G, ltile, b0, gn, lane, u - kWStep);
-    if (u < Sp::ACTSTEPS) {
-#pragma unroll
-      for (int i = Sp::ACT * u / Sp::ACTSTEPS; i < Sp::ACT * (u + 1) / Sp::ACTSTEPS; ++i)
-        g2_load_act1<NW>(actn, voff, row_bytes, nbuf, gn, wave, i);
-    }
-    if (u + 1 < 8) {
-      const int s1 = (u + 1) >> 2, t1 = (u + 1) & 3;
-      const int slot = (8 * s1 + 4 * h + t1) ^ (r & 15);
-#pragma unroll
-      for (int mb = 0; mb < MBW; ++mb) xo[nu][mb] = buf[mb * 512 + slot];
-#pragma unroll
-      for (int j = 0; j < NH; ++j) wd[nu][j] = g2_deq(cur.q[j][s1][t1], sf[j], cf[j]);
-    }
-#pragma unroll
-    for (int mb = 0; mb < MBW; ++mb)
-#pragma unroll
-      for (int j = 0; j < NH; ++j)
-        acc[j][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            wd[cu][j], __builtin_bit_cast(bf16x8, xo[cu][mb]), acc[j][mb], 0, 0, 0);
-    if (u + 1 < 8) {
-#pragma unroll
-      for (int i = 0; i < MBW * NH; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-        if (i < (MBW + Sp::DS - 1) / Sp::DS) __builtin_amdgcn_sched_group_barrier(0x100, Sp::DS, 0);  // DS read
-        __builtin_amdgcn_sched_group_barrier(0x002, Sp::VALU, 0);  // VALU
-      }
-    }
-    // NW = 4: one scheduling region per k-step, so that the next step's
-    // operand reads stay under this step's MFMAs instead of sinking to their
-    // first use (with one wave per SIMD nothing else hides their latency).
-    if (NW == 4) __builtin_amdgcn_sched_barrier(0);
-  }
+  const int t = tn * 4 + wt;
+  return {t, b0, t * kTileN + 32 * b0, t * kTileN < a.N};
 }
 
 // Rows of a tile. The 8-wave variants exist for MB = 8 only and run the plan's
@@ -302,84 +94,6 @@ __device__ __forceinline__ int g2_tile_rows(const GemmArgs& a) {
 template <int NW>
 __device__ __forceinline__ int g2_row_end(const GemmArgs& a, int m0) {
   return NW == 8 ? min(a.M, m0 + a.bm) : a.M;
-}
-
-// One wave's share of one (tile, group range) segment: acc = sum over groups
-// [g0, g1) of this wave's weight rows x the tile's activation rows.
-template <int NH, int NW, int MB>
-__device__ __forceinline__ void g2_segment(const GemmArgs& a, const G2Rsrc& rs,
-                                           u32x4 (*lds)[32 * MB * 16],
-                                           f32x16v (&acc)[NH][G2Split<NH, NW, MB>::MBW], int m0,
-                                           int ltile, int b0, int mw, int g0, int g1, int wave,
-                                           int lane) {
-  using Sp = G2Split<NH, NW, MB>;
-  constexpr int MBW = Sp::MBW, D = Sp::DEPTH;
-  const int r = lane & 31;
-#pragma unroll
-  for (int j = 0; j < NH; ++j)
-#pragma unroll
-    for (int mb = 0; mb < MBW; ++mb) acc[j][mb] = f32x16v{};
-  // Activation rows [m0, row end): the buffer's end turns rows past it into zeros.
-  const uint32_t row_bytes = (uint32_t)a.K * 2u;
-  const __amdgpu_buffer_rsrc_t act = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.A) + (size_t)m0 * a.K, 0, (int)((uint32_t)(g2_row_end<NW>(a, m0) - m0) * row_bytes),
-      0x00020000);
-  const __amdgpu_buffer_rsrc_t act_none =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.A), 0, 0, 0x00020000);
-  const G2Rsrc rs_none = {
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(a.qw), 0, 0, 0x00020000),
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.sc), 0, 0, 0x00020000),
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.zr), 0, 0, 0x00020000)};
-  const int srow = 4 * (wave & 3) + (lane >> 4);   // row within the 16-row swizzle period
-  const uint32_t voff = (uint32_t)(lane >> 4) * row_bytes + (uint32_t)((lane & 15) ^ srow) * 16u;
-  __syncthreads();   // the previous segment's last LDS reads are done
-  if constexpr (D == 2) {
-    WeightGroup<NH> cur, nxt;
-#pragma unroll
-    for (int i = 0; i < Sp::ACT; ++i) g2_load_act1<NW>(act, voff, row_bytes, lds[0], g0, wave, i);
-    g2_load_weights(cur, rs, a.G, ltile, b0, g0, lane);
-    for (int g = g0; g < g1; ++g) {
-      g2_wait_vm0();
-      __syncthreads();
-      const int sb = (g - g0) & 1;
-      const bool more = g + 1 < g1;
-      g2_group<NH, NW, MB>(a, acc, cur, nxt, lds[sb] + (32 * mw + r) * 16, lds[sb ^ 1],
-                           more ? act : act_none, more ? rs : rs_none, voff, row_bytes, ltile, b0,
-                           g + 1, wave, lane);
-      cur = nxt;
-    }
-  } else {
-    // D buffers, the loads D - 1 groups ahead: a group of few m-blocks computes
-    // in less than a memory latency. Unrolled by D, so that every buffer --
-    // LDS and weight registers -- is named statically and no register is
-    // copied (a copy would wait for its load). Waits are counted: loads
-    // complete in order, and every group issues the same number.
-    constexpr int kLoads = Sp::ACT + 4 * NH;
-    WeightGroup<NH> wg[D];
-#pragma unroll
-    for (int d = 0; d < D - 1; ++d) {
-      const bool in = g0 + d < g1;
-#pragma unroll
-      for (int i = 0; i < Sp::ACT; ++i)
-        g2_load_act1<NW>(in ? act : act_none, voff, row_bytes, lds[d], g0 + d, wave, i);
-      g2_load_weights(wg[d], in ? rs : rs_none, a.G, ltile, b0, g0 + d, lane);
-    }
-    for (int gb = g0; gb < g1; gb += D) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        const int g = gb + d;
-        if (g >= g1) break;
-        // group g has landed (the D - 2 groups behind it may be in flight) for
-        // every wave, and every wave is done with group g - 1's buffer
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 2) * kLoads) : "memory");
-        constexpr int kBack = D - 1;
-        const bool more = g + kBack < g1;
-        g2_group<NH, NW, MB>(a, acc, wg[d], wg[(d + kBack) % D], lds[d] + (32 * mw + r) * 16,
-                             lds[(d + kBack) % D], more ? act : act_none, more ? rs : rs_none, voff,
-                             row_bytes, ltile, b0, g + kBack, wave, lane);
-      }
-    }
-  }
 }
 
 // Tile store. Accumulator layout: lane holds column m = 32 mb + r and rows
@@ -490,7 +204,9 @@ __device__ __forceinline__ int g2_owner_of(const GemmArgs& a, int u) {
 // stored by the main kernel.
 constexpr int kFixAhead = 4;
 
-template <int NH, int NW, int MB>
+//
+// In a gated product a block owns the two pairs of one m-block: gate and up.
+template <int NH, int NW, int MB, int OUT>
 __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   using Sp = G2Split<NH, NW, MB>;
   constexpr int MBW = Sp::MBW;
@@ -509,8 +225,9 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   Sp::coords(wave, wt, b0, mw);
   int tn, tm;
   g2_tile_coords(a, t, tn, tm);
-  const int tile = tn * 4 + wt;
-  if (tile * kTileN >= a.N) return;
+  const WaveTile w = g2_wave_tile<OUT>(a, tn, wt, b0);
+  if (!w.valid) return;
+  auto pair = [&](int e) { return OUT == GEMM_GLU ? e * MBW + part : part * kPer + e; };
   const __amdgpu_buffer_rsrc_t rs =
       __builtin_amdgcn_make_buffer_rsrc(a.slots, 0, (int)(2u * a.P * kSlotBytes), 0x00020000);
   f32x16v acc[kPer];
@@ -528,7 +245,7 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const uint32_t off =
-            live ? g2_slot_off(q, which, wave, Sp::UNITS, part * kPer + e, lane) : 0x80000000u;
+            live ? g2_slot_off(q, which, wave, Sp::UNITS, pair(e), lane) : 0x80000000u;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           v[k][e][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 1024 * i, 0, 0);
@@ -547,12 +264,47 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   }
   // pair index j * MBW + mb (g2_slot_store's order)
   const int m0 = tm * g2_tile_rows<NW, MB>(a);
+  if constexpr (OUT != GEMM_PLAIN) {
+    // straight from the accumulators' layout: 4 columns of a row at a time
+    constexpr int kOuts = OUT == GEMM_GLU ? 1 : kPer;
+#pragma unroll
+    for (int e = 0; e < kOuts; ++e) {
+      const int idx = pair(e), mb = idx % MBW;
+      const int m = m0 + 32 * (mw + mb) + r;
+      const bool in = m < g2_row_end<NW>(a, m0);
+      const int col = w.col + (OUT == GEMM_GLU ? 0 : 32 * (idx / MBW)) + 4 * h;
+      float v[OUT == GEMM_GLU ? 2 : 1][16];
+#pragma unroll
+      for (int j = 0; j < (OUT == GEMM_GLU ? 2 : 1); ++j)
+#pragma unroll
+        for (int jq = 0; jq < 4; ++jq) {
+          u32x2 b = {0u, 0u};
+          if (a.epi.bias) b = *reinterpret_cast<const u32x2*>(a.epi.bias + j * a.epi.up + col + 8 * jq);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[j][4 * jq + i] = acc[e + j][4 * jq + i] + bf16_bits_to_f32((b[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+        }
+      epilogue_act<OUT == GEMM_GLU>(v, a.epi.act);
+      if (!in) continue;
+#pragma unroll
+      for (int jq = 0; jq < 4; ++jq) {
+        const size_t at = (size_t)m * a.ld + col + 8 * jq;
+        u32x2 q = {0u, 0u};
+        if (a.epi.res) q = *reinterpret_cast<const u32x2*>(a.epi.res + at);
+        const float* f = &v[0][4 * jq];
+        *reinterpret_cast<u32x2*>(a.C + at) =
+            u32x2{pack_bf16x2(f[0] + bf16_bits_to_f32(q[0] & 0xffffu), f[1] + bf16_bits_to_f32(q[0] >> 16)),
+                  pack_bf16x2(f[2] + bf16_bits_to_f32(q[1] & 0xffffu), f[3] + bf16_bits_to_f32(q[1] >> 16))};
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     const int idx = part * kPer + e, j = idx / MBW, mb = idx % MBW;
     const int m = m0 + 32 * (mw + mb) + r;
     if (m >= g2_row_end<NW>(a, m0)) continue;
-    uint16_t* crow = a.C + (size_t)m * a.N + tile * kTileN;
+    uint16_t* crow = a.C + (size_t)m * a.N + w.tile * kTileN;
 #pragma unroll
     for (int jq = 0; jq < 4; ++jq) {
       const u32x2 o = {pack_bf16x2(acc[e][4 * jq], acc[e][4 * jq + 1]),
@@ -562,8 +314,9 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   }
 }
 
-template <int NH, int NW, int MB>
+template <int NH, int NW, int MB, int OUT>
 __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
+  static_assert(OUT == GEMM_PLAIN || (NH == 2 && NW == 4), "epilogues: the default kernel");
   using Sp = G2Split<NH, NW, MB>;
   constexpr int MBW = Sp::MBW;              // m-blocks per wave
   const int bm = g2_tile_rows<NW, MB>(a);   // rows of a tile
@@ -592,37 +345,40 @@ __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
   const int u0 = g2_range_start(a, vp), u1 = g2_range_start(a, vp + 1);
   const __amdgpu_buffer_rsrc_t rs =
       __builtin_amdgcn_make_buffer_rsrc(a.slots, 0, (int)(2u * a.P * kSlotBytes), 0x00020000);
-  G2Rsrc wr;
-  wr.qw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(a.qw), 0,
-                                            (int)((uint32_t)a.N * (uint32_t)a.K / 2u), 0x00020000);
-  wr.sc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.sc), 0,
-      (int)((uint32_t)a.N / kTileN * (uint32_t)a.G * (uint32_t)kMetaBytes), 0x00020000);
-  wr.zr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.zr), 0,
-                                            (int)((uint32_t)a.N * (uint32_t)a.G / 2u), 0x00020000);
-  for (int t = vp; t < a.full; t += a.P) {
+  const G2Rsrc wr = g2_weights(a.qw, a.sc, a.zr, a.N, a.G), none = g2_weights(a.qw, a.sc, a.zr, a.N, a.G, false);
+  const uint32_t row_bytes = (uint32_t)a.K * 2u;
+  const int srow = 4 * (wave & 3) + (lane >> 4);   // row within the 16-row swizzle period
+  const G2Rows rows{(uint32_t)(lane >> 4) * row_bytes + (uint32_t)((lane & 15) ^ srow) * 16u, row_bytes};
+  constexpr bool kGlu = OUT == GEMM_GLU;
+  const int up = a.epi.up / kTileN;
+  // groups [g0, g1) of tile t; stored if they are the whole tile
+  auto segment = [&](int t, int g0, int g1) __attribute__((always_inline)) {
     int tn, tm;
     g2_tile_coords(a, t, tn, tm);
-    const int tile = tn * 4 + wt;
-    const bool valid = tile * kTileN < a.N;
-    const int ltile = valid ? tile : (a.N / kTileN - 1);
-    g2_segment<NH, NW, MB>(a, wr, lds, acc, tm * bm, ltile, b0, mw, 0, a.G, wave, lane);
-    g2_store_staged<NH, NW, MB>(a, acc, &lds[0][0], tm * bm, tile, b0, mw, valid, wave, lane);
-  }
+    const int m0 = tm * bm;
+    const WaveTile w = g2_wave_tile<OUT>(a, tn, wt, b0);
+    const int ltile = w.valid ? w.tile : (kGlu ? a.ld : a.N) / kTileN - 1;
+    // Activation rows [m0, row end): the buffer's end turns rows past it into zeros.
+    const uint16_t* A0 = a.A + (size_t)m0 * a.K;
+    g2_segment<NH, NW, MB, kGlu>(a.G, wr, none, g2_rsrc(A0, (uint32_t)(g2_row_end<NW>(a, m0) - m0) * row_bytes),
+                                 g2_rsrc(A0, 0), rows, lds, acc, ltile, up, w.b0, mw, g0, g1, wave, lane);
+    if (g0 != 0 || g1 != a.G) return false;
+    if constexpr (OUT == GEMM_PLAIN) {
+      g2_store_staged<NH, NW, MB>(a, acc, &lds[0][0], m0, w.tile, b0, mw, w.valid, wave, lane);
+    } else {
+      const size_t at = (size_t)m0 * a.ld + w.col;
+      Epilogue e = a.epi;
+      if (e.bias) e.bias += w.col;
+      if (e.res) e.res += at;
+      g2_store_epilogue<MB, kGlu>(acc, &lds[0][0], a.C + at, e, a.ld, a.M - m0, w.valid, wave, lane);
+    }
+    return true;
+  };
+  for (int t = vp; t < a.full; t += a.P) segment(t, 0, a.G);
   for (int u = u0; u < u1;) {
     const int ts = u / a.G, g0 = u - ts * a.G;
     const int g1 = min(a.G, u1 - ts * a.G);
-    int tn, tm;
-    g2_tile_coords(a, a.full + ts, tn, tm);
-    const int tile = tn * 4 + wt;
-    const bool valid = tile * kTileN < a.N;
-    const int ltile = valid ? tile : (a.N / kTileN - 1);
-    g2_segment<NH, NW, MB>(a, wr, lds, acc, tm * bm, ltile, b0, mw, g0, g1, wave, lane);
-    if (g0 == 0 && g1 == a.G) {
-      g2_store_staged<NH, NW, MB>(a, acc, &lds[0][0], tm * bm, tile, b0, mw, valid, wave, lane);
-    } else {
-      g2_slot_store<NH, NW, MB>(rs, acc, vp, u == u0 ? 0 : 1, wave, lane);
-    }
+    if (!segment(a.full + ts, g0, g1)) g2_slot_store<NH, NW, MB>(rs, acc, vp, u == u0 ? 0 : 1, wave, lane);
     u = ts * a.G + g1;
   }
 }
@@ -653,11 +409,24 @@ std::atomic<int> g_gemm_schedule{-1};
 // sum every output in the same order, so their results are bitwise equal.
 std::atomic<int> g_gemm_variant{0};
 
-template <int NH, int NW, int MB>
+template <int NH, int NW, int MB, int OUT = GEMM_PLAIN>
 void launch_gemm(const GemmArgs& a, int grid, int nt, hipStream_t s) {
-  k_gemm<NH, NW, MB><<<grid, 64 * NW, 0, s>>>(a);
+  k_gemm<NH, NW, MB, OUT><<<grid, 64 * NW, 0, s>>>(a);
   if (a.full != nt)   // the split tiles
-    k_gemm_fixup<NH, NW, MB><<<(nt - a.full) * NW * G2Split<NH, NW, MB>::FIXP, 64, 0, s>>>(a);
+    k_gemm_fixup<NH, NW, MB, OUT><<<(nt - a.full) * NW * G2Split<NH, NW, MB>::FIXP, 64, 0, s>>>(a);
+}
+
+template <int OUT>
+void launch_gemm_rows(const GemmArgs& a, int mb, int grid, int nt, hipStream_t s) {
+  switch (mb) {
+    case 2: return launch_gemm<2, 4, 2, OUT>(a, grid, nt, s);
+    case 3: return launch_gemm<2, 4, 3, OUT>(a, grid, nt, s);
+    case 4: return launch_gemm<2, 4, 4, OUT>(a, grid, nt, s);
+    case 5: return launch_gemm<2, 4, 5, OUT>(a, grid, nt, s);
+    case 6: return launch_gemm<2, 4, 6, OUT>(a, grid, nt, s);
+    case 7: return launch_gemm<2, 4, 7, OUT>(a, grid, nt, s);
+    default: return launch_gemm<2, 4, 8, OUT>(a, grid, nt, s);
+  }
 }
 
 // How a call is cut: tiles of 32 mb rows, schedule (0 per tile, 1 stream-K, 2
@@ -723,6 +492,70 @@ GemmPlan gemm_plan(int M, int N, long long G, int mb, int cus, bool ws_ok, int s
   return p;
 }
 
+// Checked arguments; the epilogue of GEMM_PLAIN is empty.
+template <int OUT>
+int run_gemm(uint16_t* C, const qw4_weights* w, const uint16_t* A, int M, qw4_workspace* ws,
+             const Epilogue& epi, void* stream) {
+  // Loads address A and the weights through 32-bit buffer offsets.
+  if ((size_t)M * w->in_f * 2 >= (1ull << 32) || (size_t)w->out_f * w->in_f / 2 >= (1ull << 32))
+    return QW4_ERR_SHAPE;
+  const int schedule = g_gemm_schedule.load(std::memory_order_relaxed);
+  const int variant = OUT == GEMM_PLAIN ? g_gemm_variant.load(std::memory_order_relaxed) : 0;
+  const int cus = device_cus();
+  const bool ws_ok = ws && ws->buf && ws->bytes >= gemm_workspace_need(cus) && cus % 8 == 0;
+  GemmPlan p = gemm_plan(M, w->out_f, w->num_groups, 8, cus, ws_ok, schedule);
+  // Tiles of fewer rows where that costs less: rows that do not fill 256-row
+  // tiles (us, 256-row tiles against the plan's: gate|up 34816x5120 at 64 / 128 /
+  // 300 rows 98 / 98 / 150 -> 55 / 70 / 126, down 5120x17408 53 / 55 / 87 -> 30 / 39 /
+  // 66, o 5120x4096 36 / 36 / 40 -> 19 / 23 / 31), and few tiles, cut in fewer
+  // slices (o at 256 rows 37 -> 28). By 3% at least, what the model resolves:
+  // down at 2000 rows costs 100.9 in 224-row tiles against 101.3 and is 3% slower.
+  // Stream-K and hybrid of lower tiles by 7% against 256 rows: the cost of a
+  // workgroup's second segment does not shrink with the tile (9472x8448 at 500 / 1000
+  // rows, 128-row tiles costed at 0.93 / 0.95 of 256-row ones: 96.7 / 164 us against
+  // 94.0 / 155).
+  if (schedule == -1) {
+    const double cost8 = p.cost;
+    for (int mb = 7; mb >= 2; --mb) {
+      const GemmPlan q = gemm_plan(M, w->out_f, w->num_groups, mb, cus, ws_ok, schedule);
+      if (q.cost < 0.97 * p.cost && !((q.pick == 1 || q.pick == 2) && q.cost >= 0.93 * cost8)) p = q;
+    }
+  }
+  const int nt = p.tiles_n * p.tiles_m, mb = p.mb;
+  GemmArgs a{w->qweight, w->scale, w->zeros, A, C, nullptr, M, w->out_f, w->in_f,
+             w->num_groups, p.tiles_n, p.tiles_m, nt % 8 == 0, 32 * mb, nt, nt, 0,
+             epi, OUT == GEMM_GLU ? w->out_f / 2 : w->out_f};
+  int grid = nt;
+  if (p.pick == 3) {
+    a.slots = static_cast<float*>(ws->buf);
+    a.P = nt * p.S;
+    a.full = 0;
+    a.U = nt * w->num_groups;
+    a.map = 2;
+    grid = a.P;
+  } else if (p.pick) {
+    a.slots = static_cast<float*>(ws->buf);
+    a.P = cus;
+    a.full = p.pick == 2 ? nt - nt % cus : 0;
+    a.U = (nt - a.full) * w->num_groups;
+    a.map = 1;
+    grid = cus;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  if constexpr (OUT == GEMM_PLAIN) {
+    if (variant == 1)
+      launch_gemm<1, 8, 8>(a, grid, nt, s);
+    else if (variant == 2)
+      launch_gemm<2, 8, 8>(a, grid, nt, s);
+    else
+      launch_gemm_rows<OUT>(a, mb, grid, nt, s);
+  } else {
+    launch_gemm_rows<OUT>(a, mb, grid, nt, s);
+  }
+  QW4_LAUNCH_CHECK();
+  return QW4_OK;
+}
+
 }  // namespace
 }  // namespace qw4
 
@@ -766,73 +599,13 @@ int qw4_gemm(uint16_t* C, const qw4_weights* w, const uint16_t* A, int M, qw4_wo
   if (!C || !A) return QW4_ERR_NULL;
   if (M < 1) return QW4_ERR_M;
   if (((uintptr_t)A & 15) || ((uintptr_t)C & 7)) return QW4_ERR_ALIGN;
-  // Loads address A and the weights through 32-bit buffer offsets.
-  if ((size_t)M * w->in_f * 2 >= (1ull << 32) || (size_t)w->out_f * w->in_f / 2 >= (1ull << 32))
-    return QW4_ERR_SHAPE;
-  {
-    const int schedule = g_gemm_schedule.load(std::memory_order_relaxed);
-    const int variant = g_gemm_variant.load(std::memory_order_relaxed);
-    const int cus = device_cus();
-    const bool ws_ok = ws && ws->buf && ws->bytes >= gemm_workspace_need(cus) && cus % 8 == 0;
-    GemmPlan p = gemm_plan(M, w->out_f, w->num_groups, 8, cus, ws_ok, schedule);
-    // Tiles of fewer rows where that costs less: rows that do not fill 256-row
-    // tiles (us, 256-row tiles against the plan's: gate|up 34816x5120 at 64 / 128 /
-    // 300 rows 98 / 98 / 150 -> 55 / 70 / 126, down 5120x17408 53 / 55 / 87 -> 30 / 39 /
-    // 66, o 5120x4096 36 / 36 / 40 -> 19 / 23 / 31), and few tiles, cut in fewer
-    // slices (o at 256 rows 37 -> 28). By 3% at least, what the model resolves:
-    // down at 2000 rows costs 100.9 in 224-row tiles against 101.3 and is 3% slower.
-    // Stream-K and hybrid of lower tiles by 7% against 256 rows: the cost of a
-    // workgroup's second segment does not shrink with the tile (9472x8448 at 500 / 1000
-    // rows, 128-row tiles costed at 0.93 / 0.95 of 256-row ones: 96.7 / 164 us against
-    // 94.0 / 155).
-    if (schedule == -1) {
-      const double cost8 = p.cost;
-      for (int mb = 7; mb >= 2; --mb) {
-        const GemmPlan q = gemm_plan(M, w->out_f, w->num_groups, mb, cus, ws_ok, schedule);
-        if (q.cost < 0.97 * p.cost && !((q.pick == 1 || q.pick == 2) && q.cost >= 0.93 * cost8)) p = q;
-      }
-    }
-    const int nt = p.tiles_n * p.tiles_m, mb = p.mb;
-    GemmArgs a{w->qweight, w->scale, w->zeros, A, C, nullptr, M, w->out_f, w->in_f,
-                w->num_groups, p.tiles_n, p.tiles_m, nt % 8 == 0, 32 * mb, nt, nt, 0};
-    int grid = nt;
-    if (p.pick == 3) {
-      a.slots = static_cast<float*>(ws->buf);
-      a.P = nt * p.S;
-      a.full = 0;
-      a.U = nt * w->num_groups;
-      a.map = 2;
-      grid = a.P;
-    } else if (p.pick) {
-      a.slots = static_cast<float*>(ws->buf);
-      a.P = cus;
-      a.full = p.pick == 2 ? nt - nt % cus : 0;
-      a.U = (nt - a.full) * w->num_groups;
-      a.map = 1;
-      grid = cus;
-    }
-    hipStream_t s = (hipStream_t)stream;
-    if (variant == 1)
-      launch_gemm<1, 8, 8>(a, grid, nt, s);
-    else if (variant == 2)
-      launch_gemm<2, 8, 8>(a, grid, nt, s);
-    else if (mb == 2)
-      launch_gemm<2, 4, 2>(a, grid, nt, s);
-    else if (mb == 3)
-      launch_gemm<2, 4, 3>(a, grid, nt, s);
-    else if (mb == 4)
-      launch_gemm<2, 4, 4>(a, grid, nt, s);
-    else if (mb == 5)
-      launch_gemm<2, 4, 5>(a, grid, nt, s);
-    else if (mb == 6)
-      launch_gemm<2, 4, 6>(a, grid, nt, s);
-    else if (mb == 7)
-      launch_gemm<2, 4, 7>(a, grid, nt, s);
-    else
-      launch_gemm<2, 4, 8>(a, grid, nt, s);
-    QW4_LAUNCH_CHECK();
-    return QW4_OK;
-  }
+  return run_gemm<GEMM_PLAIN>(C, w, A, M, ws, Epilogue{}, stream);
 }
 
 }  // extern "C"
+
+int qw4::gemm_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_workspace* ws,
+                       const Epilogue& e, void* stream) {
+  return e.act == QW4_ACT_SWIGLU ? run_gemm<GEMM_GLU>(y, w, x, M, ws, e, stream)
+                                 : run_gemm<GEMM_EPI>(y, w, x, M, ws, e, stream);
+}

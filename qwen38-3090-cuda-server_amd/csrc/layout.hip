@@ -474,6 +474,7 @@ const char* qw4_status_string(int st) {
     case QW4_ERR_LAYOUT: return "unknown source layout";
     case QW4_ERR_IO: return "checkpoint file cannot be opened, mapped or parsed";
     case QW4_ERR_NOTFOUND: return "tensor not found in the checkpoint";
+    case QW4_ERR_ACT: return "unknown activation";
     default: return "unknown status";
   }
 }

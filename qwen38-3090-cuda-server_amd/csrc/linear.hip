@@ -5,7 +5,12 @@
 #include <atomic>
 
 #include "../../include/qwen_w4a16.h"
+#include "epilogue.h"
 #include "skinny.h"
+
+namespace qw4 {
+int check_weights_public(const qw4_weights* w);
+}
 
 namespace {
 
@@ -23,6 +28,38 @@ int lin_max_t(const qw4_weights* w) {
   const double mb = (double)w->out_f * w->in_f * (0.5 + 2.5 / 128) / 1e6;
   const int chunks = (int)((60.0 + 0.4 * mb) / (0.245 * mb + 5.8));
   return 16 * (chunks < 1 ? 1 : chunks);
+}
+
+// T rows of y [T][width] in skinny passes, with the epilogue e or without (null).
+int few_rows(uint16_t* y, int width, const qw4_weights* w, const uint16_t* x, int T, qw4_scratch* s,
+             const qw4::Epilogue* e, void* stream) {
+  const int chunk = s->max_m < 16 ? s->max_m : 16;
+  if (chunk < 1) return QW4_ERR_SCRATCH;
+  for (int i = 0, n; i < T; i += n) {
+    uint16_t* const yi = y + (size_t)i * width;
+    const uint16_t* const xi = x + (size_t)i * w->in_f;
+    qw4::Epilogue ei{};
+    if (e) {
+      ei = *e;
+      if (ei.res) ei.res += (size_t)i * width;
+    }
+    // two 16-row passes in one where it pays; a last single row stays a pass
+    // of its own (the GEMV's sums)
+    const int left = T - i;
+    n = left < 32 ? left : 32;
+    if (n % 16 == 1) --n;
+    if (chunk == 16 && n > 16) {
+      bool taken = false;
+      const int st = qw4::skinny_rows32(yi, w, xi, n, s, stream, e ? &ei : nullptr, &taken);
+      if (st) return st;
+      if (taken) continue;
+    }
+    n = left < chunk ? left : chunk;
+    const int st = e ? qw4::skinny_epilogue(yi, w, xi, n, s, ei, stream)
+                     : qw4_gemm_small(yi, w, xi, n, s, stream);
+    if (st) return st;
+  }
+  return QW4_OK;
 }
 
 }  // namespace
@@ -45,30 +82,23 @@ int qw4_linear(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T, qw4_
   if (!y || !w || !x) return QW4_ERR_NULL;
   if (T < 1) return QW4_ERR_M;
   if (T == 1) return qw4_gemv(y, w, x, s, stream);
-  if (T <= lin_max_t(w) && s) {
-    const int chunk = s->max_m < 16 ? s->max_m : 16;
-    if (chunk < 1) return QW4_ERR_SCRATCH;
-    for (int i = 0, n; i < T; i += n) {
-      // two 16-row passes in one where it pays; a last single row stays a pass
-      // of its own (the GEMV's sums)
-      const int left = T - i;
-      n = left < 32 ? left : 32;
-      if (n % 16 == 1) --n;
-      if (chunk == 16 && n > 16) {
-        bool taken = false;
-        const int st = qw4::skinny_rows32(y + (size_t)i * w->out_f, w, x + (size_t)i * w->in_f, n, s,
-                                          stream, &taken);
-        if (st) return st;
-        if (taken) continue;
-      }
-      n = left < chunk ? left : chunk;
-      const int st = qw4_gemm_small(y + (size_t)i * w->out_f, w, x + (size_t)i * w->in_f, n, s,
-                                    stream);
-      if (st) return st;
-    }
-    return QW4_OK;
-  }
+  if (T <= lin_max_t(w) && s) return few_rows(y, w->out_f, w, x, T, s, nullptr, stream);
   return qw4_gemm(y, w, x, T, ws, stream);
+}
+
+int qw4_linear_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T,
+                        const uint16_t* bias, int act, const uint16_t* residual, qw4_scratch* s,
+                        qw4_workspace* ws, void* stream) {
+  const int st = qw4::check_weights_public(w);
+  if (st) return st;
+  if (!y || !x) return QW4_ERR_NULL;
+  if (T < 1) return QW4_ERR_M;
+  if (act < QW4_ACT_NONE || act > QW4_ACT_SWIGLU) return QW4_ERR_ACT;
+  if (act == QW4_ACT_SWIGLU && w->out_f % (2 * qw4::kTileN)) return QW4_ERR_SHAPE;
+  if (((uintptr_t)y | (uintptr_t)x | (uintptr_t)bias | (uintptr_t)residual) & 15) return QW4_ERR_ALIGN;
+  const qw4::Epilogue e{bias, residual, act, act == QW4_ACT_SWIGLU ? w->out_f / 2 : 0};
+  if (s && T <= lin_max_t(w)) return few_rows(y, w->out_f - e.up, w, x, T, s, &e, stream);
+  return qw4::gemm_epilogue(y, w, x, T, ws, e, stream);
 }
 
 }  // extern "C"

@@ -283,6 +283,15 @@ void linear_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16
   check(qw4_linear(u16(y), &v, u16(x), T, &s.impl, &q, stream), "linear_w4a16");
 }
 
+void linear_epilogue_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int T,
+                           const __hip_bfloat16* bias, int act, const __hip_bfloat16* residual,
+                           GemvScratch& s, GemmWorkspace& ws, hipStream_t stream) {
+  const qw4_weights v = view(w);
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_linear_epilogue(u16(y), &v, u16(x), T, u16(bias), act, u16(residual), &s.impl, &q, stream),
+        "linear_epilogue_w4a16");
+}
+
 void expert_plan_alloc(qw4_plan& plan, int experts, int max_pairs) {
   check(qw4_plan_alloc(&plan, experts, max_pairs), "expert_plan_alloc");
 }

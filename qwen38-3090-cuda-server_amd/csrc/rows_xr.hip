@@ -43,6 +43,18 @@ __device__ __forceinline__ void xr_emit(const SkinnyArgs& a, int b, int st0, int
     return;
   }
   if (m >= a.M) return;
+  if constexpr (OUT == OUT_EPI || OUT == OUT_GLU) {
+    constexpr bool kGlu = OUT == OUT_GLU;
+    float f[kGlu ? 2 : 1][S], b[kGlu ? 2 : 1][S];
+#pragma unroll
+    for (int j = 0; j < (kGlu ? 2 : 1); ++j) {
+      load_cols<S>(b[j], a.epi.bias, (size_t)n0 + j * a.epi.up);
+#pragma unroll
+      for (int i = 0; i < S; ++i) f[j][i] = kGlu && j == 0 ? g[i] : v[i];
+    }
+    emit_epilogue<kGlu, S>(a, m, n0, f, b);
+    return;
+  }
   uint16_t* y = static_cast<uint16_t*>(a.y) + (size_t)m * a.ld + n0;
   uint32_t o[S];
 #pragma unroll
@@ -80,11 +92,11 @@ __global__ __launch_bounds__(64 * kXrW) void k_rows_xr(SkinnyArgs a) {
   const uint32_t wbase = Fmt<FMT>::woff(q, c);
   const int p = blockIdx.x;
   // OUT_SWIGLU: units 2v (gate v) and 2v + 1 (its up unit), never split
-  const int u0 = OUT == OUT_SWIGLU ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
+  const int u0 = out_paired(OUT) ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
   const int u1 =
-      OUT == OUT_SWIGLU ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
+      out_paired(OUT) ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
   auto real_unit = [&](int v) {
-    return OUT == OUT_SWIGLU ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
+    return out_paired(OUT) ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
   };
   const NibConst k = nib_const();
   const int nw = wave < a.G ? (a.G - 1 - wave) / W + 1 : 0;   // groups of this wave (<= NG)
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(64 * kXrW) void k_rows_xr(SkinnyArgs a) {
       }
     lds_barrier<true>();
     // one row block: the halves of the workgroup take turns; two: a half each
-    if (MB == 2 || (wave >> 2) == ((OUT == OUT_SWIGLU ? n >> 1 : n) & 1)) {
+    if (MB == 2 || (wave >> 2) == ((out_paired(OUT) ? n >> 1 : n) & 1)) {
       const int jj = wave & 3, mb = MB == 2 ? wave >> 2 : 0;
       float v[S];
 #pragma unroll
@@ -244,11 +256,11 @@ __global__ __launch_bounds__(64 * kXrW) void k_rows_xr(SkinnyArgs a) {
 #pragma unroll
         for (int w = 1; w < W; ++w) v[i] += reinterpret_cast<const float*>(red[w])[at];
       }
-      if (OUT == OUT_SWIGLU && (n & 1) == 0) {
+      if (out_paired(OUT) && (n & 1) == 0) {
 #pragma unroll
         for (int i = 0; i < S; ++i) gate[i] = v[i];
       } else {
-        const uint32_t ou = OUT == OUT_SWIGLU ? (uint32_t)u >> 1 : (uint32_t)u;   // output unit
+        const uint32_t ou = out_paired(OUT) ? (uint32_t)u >> 1 : (uint32_t)u;   // output unit
         xr_emit<OUT, S>(a, (int)(ou / kPer), (int)(ou % kPer) * S, 16 * mb + jj, v, gate, lane, bv, bn);
       }
     }
@@ -317,6 +329,12 @@ void launch_out(const SkinnyArgs& a, int S, bool prepare, hipStream_t st) {
   }
 }
 
+template <int OUT>
+void launch_two(const SkinnyArgs& a, bool prepare, hipStream_t st) {
+  if (prepare || a.G <= 3 * kXrW) launch<OUT, 4, 2, 3, 3, 2>(a, prepare, st);
+  if (prepare || a.G > 3 * kXrW) launch<OUT, 4, 2, 5, 3, 2>(a, prepare, st);
+}
+
 void dispatch(int out, int fmt, const SkinnyArgs& a, int S, bool prepare, hipStream_t st) {
   if (fmt == 8) {
     if (prepare || out == OUT_BF16) launch_out<OUT_BF16, 8>(a, S, prepare, st);
@@ -326,6 +344,8 @@ void dispatch(int out, int fmt, const SkinnyArgs& a, int S, bool prepare, hipStr
     if (prepare || out == OUT_ARGMAX) launch_out<OUT_ARGMAX, 4>(a, S, prepare, st);
     if (prepare || out == OUT_RES) launch_out<OUT_RES, 4>(a, S, prepare, st);
     if (prepare || out == OUT_SWIGLU) launch_out<OUT_SWIGLU, 4>(a, S, prepare, st);
+    if (prepare || out == OUT_EPI) launch_out<OUT_EPI, 4>(a, S, prepare, st);
+    if (prepare || out == OUT_GLU) launch_out<OUT_GLU, 4>(a, S, prepare, st);
   }
 }
 
@@ -346,9 +366,9 @@ void dispatch(int out, int fmt, const SkinnyArgs& a, int S, bool prepare, hipStr
 //    6.0 / 6.3 us, but at M = 2 4.9 against 5.5.
 bool rows_xr_launch(int out, int fmt, SkinnyArgs& a, int cus, hipStream_t st) {
   if (a.M < 2 || a.G > kXrW * kXrMaxGroups) return false;
-  if (out != OUT_BF16 && out != OUT_ARGMAX && (fmt == 8 || (out != OUT_RES && out != OUT_SWIGLU)))
+  if (out != OUT_BF16 && out != OUT_ARGMAX && (fmt == 8 || out == OUT_F32 || out == OUT_NORM))
     return false;
-  const bool small = out != OUT_SWIGLU && 4 * a.tiles < cus;   // 16-row units in k_rows
+  const bool small = !out_paired(out) && 4 * a.tiles < cus;   // 16-row units in k_rows
   if (!(2 * a.tiles > cus || (small && a.M >= 8))) return false;
   const int S = fmt == 8 || small ? 1 : 2;
   a.U = a.tiles * 4 / S;
@@ -358,7 +378,7 @@ bool rows_xr_launch(int out, int fmt, SkinnyArgs& a, int cus, hipStream_t st) {
   // 31.3, 29.2 / 31.7 / 31.7; 9472x5120 9.7 / 10.0 / 10.4, 9.3 / 9.9 / 10.6); the 8-bit heads own tens of units each, and with a short K every
   // workgroup streams for longer than it loads rows (151936x2560 at M = 9: 69.9 us
   // with 250 workgroups, 68.4 with 256)
-  const int n = out == OUT_SWIGLU ? a.U / 2 : a.U, most = (n + cus - 1) / cus;
+  const int n = out_paired(out) ? a.U / 2 : a.U, most = (n + cus - 1) / cus;
   a.P = fmt == 8 && a.G <= 3 * kXrW ? std::min(n, cus) : (n + most - 1) / most;
   dispatch(out, fmt, a, S, false, st);
   return true;
@@ -369,23 +389,25 @@ bool rows_xr_launch(int out, int fmt, SkinnyArgs& a, int cus, hipStream_t st) {
 // spills). Faster than two passes at every size measured (32 rows): gate|up
 // 34816x5120 40.0 -> 27.5 us, 7168x5120 15.5 -> 11.4, 5120x4096 12.9 -> 10.3,
 // 896x5120 12.3 -> 10.8, 5120x512 7.9 -> 6.0.
-bool rows_xr2_launch(SkinnyArgs& a, int cus, hipStream_t st) {
-  const int ng = (a.G + kXrW - 1) / kXrW;
-  if (a.M < 17 || a.M > 32 || ng > 5) return false;
+bool rows_xr2_launch(int out, SkinnyArgs& a, int cus, hipStream_t st) {
+  if (a.M < 17 || a.M > 32 || a.G > 5 * kXrW) return false;
   a.U = a.tiles * 2;
-  const int most = (a.U + cus - 1) / cus;
-  a.P = (a.U + most - 1) / most;
-  if (ng <= 3)
-    launch<OUT_BF16, 4, 2, 3, 3, 2>(a, false, st);
+  const int n = out_paired(out) ? a.U / 2 : a.U, most = (n + cus - 1) / cus;
+  a.P = (n + most - 1) / most;
+  if (out == OUT_GLU)
+    launch_two<OUT_GLU>(a, false, st);
+  else if (out == OUT_EPI)
+    launch_two<OUT_EPI>(a, false, st);
   else
-    launch<OUT_BF16, 4, 2, 5, 3, 2>(a, false, st);
+    launch_two<OUT_BF16>(a, false, st);
   return true;
 }
 
 void rows_xr_prepare() {
   SkinnyArgs a{};
-  launch<OUT_BF16, 4, 2, 3, 3, 2>(a, true, nullptr);
-  launch<OUT_BF16, 4, 2, 5, 3, 2>(a, true, nullptr);
+  launch_two<OUT_BF16>(a, true, nullptr);
+  launch_two<OUT_EPI>(a, true, nullptr);
+  launch_two<OUT_GLU>(a, true, nullptr);
   dispatch(0, 4, a, 0, true, nullptr);
   dispatch(0, 8, a, 0, true, nullptr);
 }

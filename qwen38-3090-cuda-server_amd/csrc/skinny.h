@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "../../include/qwen_w4a16.h"
+#include "epilogue.h"
 #include "w4a16_common.h"
 
 namespace qw4 {
@@ -25,7 +26,15 @@ constexpr int kWeightAux = 2;
 //   OUT_SWIGLU y = bf16(silu(bf16(acc_gate)) * bf16(acc_up)) over a fused
 //              [gate | up] weight: linear then swiglu (model.cu:776-778)
 //   OUT_NORM   bf16 y of rmsnorm(x): rmsnorm then linear (model.cu:773-777)
-enum { OUT_BF16 = 0, OUT_F32 = 1, OUT_ARGMAX = 2, OUT_RES = 3, OUT_SWIGLU = 4, OUT_NORM = 5 };
+//   OUT_EPI    y = bf16(act(acc + bias) + residual), rounded once
+//   OUT_GLU    y = bf16(silu(acc_gate + bias) * (acc_up + bias) + residual), rounded once
+enum {
+  OUT_BF16 = 0, OUT_F32 = 1, OUT_ARGMAX = 2, OUT_RES = 3, OUT_SWIGLU = 4, OUT_NORM = 5,
+  OUT_EPI = 6, OUT_GLU = 7
+};
+// Outputs of a fused [gate | up] weight: units go in (gate, up) pairs, and the output
+// has half the weight's columns.
+constexpr bool out_paired(int out) { return out == OUT_SWIGLU || out == OUT_GLU; }
 
 // Memory-side atomics on one cache line serialize; each counter gets its own line.
 constexpr int kCounterStride = 32;
@@ -46,7 +55,8 @@ struct SkinnyArgs {
   const uint16_t* res;     // OUT_RES: residual [M][N] (may be y)
   const uint16_t* nw;      // OUT_NORM: rmsnorm weight [K] (applied as 1 + w)
   float eps;               // OUT_NORM: rmsnorm epsilon
-  int ld;                  // row stride of y (N; the intermediate size for OUT_SWIGLU)
+  int ld;                  // row stride of y (N; the intermediate size for paired outputs)
+  Epilogue epi;            // OUT_EPI, OUT_GLU
 };
 
 // Monotonic key: larger value first, then lower index (elementwise.cu:103-104).
@@ -429,12 +439,53 @@ __device__ __forceinline__ void rows_mma(f32x4 (&acc)[S], const RowsData<FMT, S,
     for (int jj = 0; jj < JJ; ++jj) acc[i][jj] += sf[i] * (C[i][jj] - zf[i] * Cs[jj]);
 }
 
+// S values of a bf16 row from column n (S = 2, 4: 4- and 8-byte aligned), zeros for p null.
+template <int S>
+__device__ __forceinline__ void load_cols(float (&v)[S], const uint16_t* p, size_t at) {
+#pragma unroll
+  for (int i = 0; i < S; ++i) v[i] = 0.f;
+  if (!p) return;
+  if constexpr (S == 1) {
+    v[0] = bf16_bits_to_f32(p[at]);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p + at);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = bf16_bits_to_f32((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+  }
+}
+
+// OUT_EPI, OUT_GLU: columns n0 .. n0 + S - 1 of row m from the sums v (gate, up) and the
+// bias b.
+template <bool GLU, int S>
+__device__ __forceinline__ void emit_epilogue(const SkinnyArgs& a, int m, int n0,
+                                              float (&v)[GLU ? 2 : 1][S],
+                                              const float (&b)[GLU ? 2 : 1][S]) {
+  const size_t at = (size_t)m * a.ld + n0;
+  float r[S];
+  load_cols<S>(r, a.epi.res, at);
+#pragma unroll
+  for (int j = 0; j < (GLU ? 2 : 1); ++j)
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[j][i] += b[j][i];
+  epilogue_act<GLU, S>(v, a.epi.act);
+  uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+  if constexpr (S == 1) {
+    y[0] = to_bf16(v[0][0] + r[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < S / 2; ++i)
+      reinterpret_cast<uint32_t*>(y)[i] = pack_bf16x2(v[0][2 * i] + r[2 * i], v[0][2 * i + 1] + r[2 * i + 1]);
+  }
+}
+
 // Final values of one unit (wave 0): rows m = 4q + jj, columns b*64 + 4c + st0 + i.
 template <int OUT, int S>
 __device__ __forceinline__ void emit_rows(const SkinnyArgs& a, int b, int st0,
                                           const f32x4 (&acc)[S], int lane, Best& bs) {
   const int c = lane & 15, q = lane >> 4;
   const int n0 = b * kTileN + 4 * c + st0;
+  float bias[1][S];
+  if (OUT == OUT_EPI) load_cols<S>(bias[0], a.epi.bias, n0);
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
     const int m = 4 * q + jj;
@@ -444,7 +495,12 @@ __device__ __forceinline__ void emit_rows(const SkinnyArgs& a, int b, int st0,
       continue;
     }
     if (m >= a.M) continue;
-    if (OUT == OUT_RES) {
+    if (OUT == OUT_EPI) {
+      float v[1][S];
+#pragma unroll
+      for (int i = 0; i < S; ++i) v[0][i] = acc[i][jj];
+      emit_epilogue<false, S>(a, m, n0, v, bias);
+    } else if (OUT == OUT_RES) {
       // bf16(res + bf16(acc)), the reference's linear then residual_add
       uint16_t* y = static_cast<uint16_t*>(a.y) + (size_t)m * a.ld + n0;
       const uint16_t* r = a.res + (size_t)m * a.ld + n0;
@@ -469,17 +525,32 @@ __device__ __forceinline__ void emit_rows(const SkinnyArgs& a, int b, int st0,
 }
 
 
-// OUT_SWIGLU (wave 0): gate rows of tile b (the intermediate index), their up
+// OUT_SWIGLU, OUT_GLU (wave 0): gate rows of tile b (the intermediate index), their up
 // rows' sums in u.
-template <int S>
+template <int OUT, int S>
 __device__ __forceinline__ void emit_swiglu(const SkinnyArgs& a, int b, int st0,
                                             const f32x4 (&g)[S], const f32x4 (&u)[S], int lane) {
   const int c = lane & 15, q = lane >> 4;
   const int n0 = b * kTileN + 4 * c + st0;
+  float bias[2][S];
+  if (OUT == OUT_GLU) {
+    load_cols<S>(bias[0], a.epi.bias, n0);
+    load_cols<S>(bias[1], a.epi.bias, (size_t)n0 + a.epi.up);
+  }
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
     const int m = 4 * q + jj;
     if (m >= a.M) continue;
+    if (OUT == OUT_GLU) {
+      float v[2][S];
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        v[0][i] = g[i][jj];
+        v[1][i] = u[i][jj];
+      }
+      emit_epilogue<true, S>(a, m, n0, v, bias);
+      continue;
+    }
     uint16_t* y = static_cast<uint16_t*>(a.y) + (size_t)m * a.ld + n0;
 #pragma unroll
     for (int i = 0; i < S; ++i) y[i] = swiglu_bf16_bits(to_bf16(g[i][jj]), to_bf16(u[i][jj]));
@@ -519,11 +590,15 @@ void allow_lds(int bytes) {
 // k_rows_xr (rows_xr.hip): launches it for these arguments (P and U filled in)
 // and returns true, or returns false where it does not apply.
 bool rows_xr_launch(int out, int fmt, SkinnyArgs& a, int cus, hipStream_t st);
-bool rows_xr2_launch(SkinnyArgs& a, int cus, hipStream_t st);   // 17 to 32 rows
+bool rows_xr2_launch(int out, SkinnyArgs& a, int cus, hipStream_t st);   // 17 to 32 rows
 // qw4_linear's 17 to 32 rows over one reading of the weights, each bitwise a
-// 16-row pass's (skinny.hip); *taken false where that form does not apply.
+// 16-row pass's (skinny.hip); *taken false where that form does not apply. e: null, or
+// qw4_linear_epilogue's.
 int skinny_rows32(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_scratch* s,
-                  void* stream, bool* taken);
+                  void* stream, const Epilogue* e, bool* taken);
+// qw4_linear_epilogue's passes of 1 to 16 rows (skinny.hip).
+int skinny_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_scratch* s,
+                    const Epilogue& e, void* stream);
 void rows_xr_prepare();   // raises its kernels' dynamic LDS limits on this device
 
 }  // namespace qw4

@@ -113,11 +113,11 @@ __global__ __launch_bounds__(64 * W) void k_rows(SkinnyArgs a) {
   const int p = blockIdx.x;
   // OUT_SWIGLU: units come in pairs (gate unit v, its up unit v + U / 2),
   // numbered 2v and 2v + 1 and never split between workgroups
-  const int u0 = OUT == OUT_SWIGLU ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
+  const int u0 = out_paired(OUT) ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
   const int u1 =
-      OUT == OUT_SWIGLU ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
+      out_paired(OUT) ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
   auto real_unit = [&](int v) {
-    return OUT == OUT_SWIGLU ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
+    return out_paired(OUT) ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
   };
   const NibConst k = nib_const();
   Best bs;
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * W) void k_rows(SkinnyArgs a) {
 #pragma unroll
   for (int i = 0; i < S; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   int par = 0, closed = u0;
-  f32x4 gate[OUT == OUT_SWIGLU ? S : 1];   // OUT_SWIGLU: the gate unit's sums (wave 0)
+  f32x4 gate[out_paired(OUT) ? S : 1];   // OUT_SWIGLU: the gate unit's sums (wave 0)
   auto close_unit = [&]() {
     if (!kM1 || lane < kRedLanes) {
 #pragma unroll
@@ -285,16 +285,16 @@ __global__ __launch_bounds__(64 * W) void k_rows(SkinnyArgs a) {
       for (int w = 1; w < W; ++w)
 #pragma unroll
         for (int i = 0; i < S; ++i) t[i] += red[par % kRedBufs][w][i][rl];
-      if (OUT == OUT_SWIGLU) {
+      if (out_paired(OUT)) {
         const int gu = closed >> 1;   // the gate unit (= the output unit)
         if ((closed & 1) == 0) {
 #pragma unroll
-          for (int i = 0; i < S; ++i) gate[i & (OUT == OUT_SWIGLU ? 0xff : 0)] = t[i];
+          for (int i = 0; i < S; ++i) gate[i & (out_paired(OUT) ? 0xff : 0)] = t[i];
         } else {
           f32x4 g[S];
 #pragma unroll
-          for (int i = 0; i < S; ++i) g[i] = gate[i & (OUT == OUT_SWIGLU ? 0xff : 0)];
-          emit_swiglu<S>(a, (int)((uint32_t)gu / kPer), (int)((uint32_t)gu % kPer) * S, g, t,
+          for (int i = 0; i < S; ++i) g[i] = gate[i & (out_paired(OUT) ? 0xff : 0)];
+          emit_swiglu<OUT, S>(a, (int)((uint32_t)gu / kPer), (int)((uint32_t)gu % kPer) * S, g, t,
                          lane);
         }
       } else {
@@ -748,11 +748,11 @@ __global__ __launch_bounds__(64 * W) void k_dec(SkinnyArgs a) {
   const int p = blockIdx.x;
   const int G = a.G;
   // OUT_SWIGLU: units 2v (gate v) and 2v + 1 (its up unit), never split
-  const int u0 = OUT == OUT_SWIGLU ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
+  const int u0 = out_paired(OUT) ? 2 * (int)((long long)p * (a.U / 2) / a.P) : range_start(a, p);
   const int u1 =
-      OUT == OUT_SWIGLU ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
+      out_paired(OUT) ? 2 * (int)((long long)(p + 1) * (a.U / 2) / a.P) : range_start(a, p + 1);
   auto real_unit = [&](int v) {
-    return OUT == OUT_SWIGLU ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
+    return out_paired(OUT) ? ((v & 1) ? (v >> 1) + (int)((uint32_t)a.U / 2u) : (v >> 1)) : v;
   };
   Best bs;
   best_init(bs);
@@ -778,39 +778,51 @@ __global__ __launch_bounds__(64 * W) void k_dec(SkinnyArgs a) {
       ++lu;
     }
   };
-  // OUT_RES: the residual of eight units (wave 0, lane 16 h + c: columns 4 c + st0 ..
+  // OUT_RES, OUT_EPI, OUT_GLU: what the epilogue adds to eight output units -- the
+  // residual, the bias, the up rows' bias -- (wave 0, lane 16 h + c: columns 4 c + st0 ..
   // of units rb + h and rb + 4 + h; S = 1: the aligned word that holds the lane's
-  // value), loaded ahead of x. Past the range the loads return zeros without
-  // traffic: no branch that would copy, and so wait for, a loaded value. res_here:
-  // the compiler's wait for them stands there, where x has landed, not at every
+  // value), loaded ahead of x. Past the range, or with nothing to add, the loads return
+  // zeros without traffic: no branch that would copy, and so wait for, a loaded value.
+  // res_here: the compiler's wait for them stands there, where x has landed, not at every
   // close, where it would drain the items. us with the load at a unit's close / a
   // unit ahead with a wait at the close / so: 34816x10240 33.0 / 37.4 / 30.7,
   // 34816x5120 19.9 / 20.8 / 17.3, 5120x512 3.96 / 3.70 / 3.70.
   constexpr int kResW = (S + 1) / 2;
-  uint32_t res0[kResW] = {}, res1[kResW] = {};
-  int rb = u0;
-  const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.res), 0, OUT == OUT_RES ? a.N * 2 : 0, 0x00020000);
-  auto load_res4 = [&](uint32_t (&r)[kResW], int ub) __attribute__((always_inline)) {
+  constexpr int kAdds = OUT == OUT_RES ? 1 : OUT == OUT_EPI ? 2 : OUT == OUT_GLU ? 3 : 0;
+  constexpr int kPair = out_paired(OUT) ? 2 : 1;   // units of an output unit
+  uint32_t res0[kAdds + 1][kResW] = {}, res1[kAdds + 1][kResW] = {};
+  int rb = u0 / kPair;
+  auto add_rsrc = [&](int s) __attribute__((always_inline)) {
+    const uint16_t* p = OUT == OUT_RES ? a.res : s == 0 ? a.epi.res : a.epi.bias;
+    const int cols = OUT == OUT_RES ? a.N : p ? a.ld : 0;
+    if (s == 2 && p) p += a.epi.up;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, cols * 2, 0x00020000);
+  };
+  auto load_res4 = [&](uint32_t (&r)[kAdds + 1][kResW], int ub) __attribute__((always_inline)) {
     const uint32_t u = (uint32_t)(ub + q);
-    const uint32_t off = (int)u < u1 ? (u / kPer * kTileN + 4u * c + u % kPer * S) * 2u : 0x7ffffff0u;
-    if (S == 4) {
-      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rr, off, 0, 0);
-      r[0] = v[0];
-      r[kResW - 1] = v[1];
-    } else {
-      r[0] = __builtin_amdgcn_raw_buffer_load_b32(rr, off & ~3u, 0, 0);
+    const uint32_t off = (int)u < u1 / kPair ? (u / kPer * kTileN + 4u * c + u % kPer * S) * 2u : 0x7ffffff0u;
+#pragma unroll
+    for (int s = 0; s < kAdds; ++s) {
+      const __amdgpu_buffer_rsrc_t rr = add_rsrc(s);
+      if (S == 4) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rr, off, 0, 0);
+        r[s][0] = v[0];
+        r[s][kResW - 1] = v[1];
+      } else {
+        r[s][0] = __builtin_amdgcn_raw_buffer_load_b32(rr, off & ~3u, 0, 0);
+      }
     }
   };
   auto load_res = [&]() __attribute__((always_inline)) {
-    if (OUT != OUT_RES || wave != 0) return;
+    if (kAdds == 0 || wave != 0) return;
     load_res4(res0, rb);
-    if (rb + 4 < u1) load_res4(res1, rb + 4);
+    if (rb + 4 < u1 / kPair) load_res4(res1, rb + 4);
   };
   auto res_here = [&]() __attribute__((always_inline)) {
-    if (OUT != OUT_RES) return;
 #pragma unroll
-    for (int i = 0; i < kResW; ++i) asm volatile("" : "+v"(res0[i]), "+v"(res1[i]));
+    for (int s = 0; s < kAdds; ++s)
+#pragma unroll
+      for (int i = 0; i < kResW; ++i) asm volatile("" : "+v"(res0[s][i]), "+v"(res1[s][i]));
   };
   load_res();
   uint32_t* const xw = reinterpret_cast<uint32_t*>(xq);
@@ -902,7 +914,51 @@ __global__ __launch_bounds__(64 * W) void k_dec(SkinnyArgs a) {
 #pragma unroll
   for (int i = 0; i < S; ++i) acc[i] = 0.f;
   int par = 0;
-  float gate[OUT == OUT_SWIGLU ? S : 1];   // OUT_SWIGLU: the gate unit's sums (wave 0)
+  float gate[out_paired(OUT) ? S : 1];   // paired outputs: the gate unit's sums (wave 0)
+  // Output unit ou (columns 64 b + 4 c + st0 ..) from its sums t (OUT_GLU: gate sums g):
+  // OUT_RES bf16(res + bf16(t)), OUT_EPI and OUT_GLU rounded once.
+  auto add_close = [&](int ou, int st0, int b, const auto& g, const float (&t)[S])
+                       __attribute__((always_inline)) {
+    const int n = ou - rb;
+    if (q == (n & 3)) {
+      float add[kAdds + 1][S];
+#pragma unroll
+      for (int s = 0; s < kAdds; ++s)
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const uint32_t ra = res0[s][i >> 1], rc = res1[s][i >> 1], r = n & 4 ? rc : ra;
+          add[s][i] = bf16_bits_to_f32((r >> (16 * (S == 1 ? st0 & 1 : i & 1))) & 0xffffu);
+        }
+      uint32_t o[S];
+      if constexpr (OUT == OUT_RES) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) o[i] = to_bf16(add[0][i] + bf16_bits_to_f32(to_bf16(t[i])));
+      } else {
+        constexpr bool kGlu = OUT == OUT_GLU;
+        float v[kGlu ? 2 : 1][S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          v[0][i] = (kGlu ? g[i] : t[i]) + add[kAdds > 1 ? 1 : 0][i];
+          if (kGlu) v[kGlu ? 1 : 0][i] = t[i] + add[kAdds > 2 ? 2 : 0][i];
+        }
+        epilogue_act<kGlu, S>(v, a.epi.act);
+#pragma unroll
+        for (int i = 0; i < S; ++i) o[i] = to_bf16(v[0][i] + add[0][i]);
+      }
+      uint16_t* y = static_cast<uint16_t*>(a.y) + b * kTileN + 4 * c + st0;
+      if (S == 1)
+        y[0] = (uint16_t)o[0];
+      else
+#pragma unroll
+        for (int i = 0; i < S / 2; ++i)
+          reinterpret_cast<uint32_t*>(y)[i] = o[(2 * i) % S] | (o[(2 * i + 1) % S] << 16);
+    }
+    if (n == 7) {
+      rb += 8;
+      load_res();
+      res_here();
+    }
+  };
   // Close unit u: every wave passes here once per unit of the range, in order.
   auto close_unit = [&](int u) {
     if (lane < 16) {
@@ -920,45 +976,28 @@ __global__ __launch_bounds__(64 * W) void k_dec(SkinnyArgs a) {
       }
       const int ru = real_unit(u);
       const int b = (int)((uint32_t)ru / kPer), st0 = (int)((uint32_t)ru % kPer) * S;
-      if (OUT == OUT_SWIGLU) {
+      if (out_paired(OUT)) {
         if ((u & 1) == 0) {
 #pragma unroll
-          for (int i = 0; i < S; ++i) gate[i & (OUT == OUT_SWIGLU ? 0xff : 0)] = t[i];
+          for (int i = 0; i < S; ++i) gate[i & (out_paired(OUT) ? 0xff : 0)] = t[i];
         } else {
-          f32x4 gg[S], uu[S];
+          const int ou = u >> 1, ob = (int)((uint32_t)ou / kPer), ost = (int)((uint32_t)ou % kPer) * S;
+          if constexpr (OUT == OUT_GLU) {
+            add_close(ou, ost, ob, gate, t);
+          } else {
+            f32x4 gg[S], uu[S];
 #pragma unroll
-          for (int i = 0; i < S; ++i) {
-            gg[i] = f32x4{gate[i & (OUT == OUT_SWIGLU ? 0xff : 0)], 0.f, 0.f, 0.f};
-            uu[i] = f32x4{t[i], 0.f, 0.f, 0.f};
+            for (int i = 0; i < S; ++i) {
+              gg[i] = f32x4{gate[i & (out_paired(OUT) ? 0xff : 0)], 0.f, 0.f, 0.f};
+              uu[i] = f32x4{t[i], 0.f, 0.f, 0.f};
+            }
+            emit_swiglu<OUT, S>(a, ob, ost, gg, uu, lane);
           }
-          emit_swiglu<S>(a, (int)((uint32_t)(u >> 1) / kPer), (int)((uint32_t)(u >> 1) % kPer) * S,
-                         gg, uu, lane);
         }
-      } else if (OUT == OUT_RES) {
-        // bf16(res + bf16(acc)), as emit_rows, by the lanes that hold the unit's
-        // residual (every 16 lanes have its sums)
-        const int n = u - rb;
-        if (q == (n & 3)) {
-          uint32_t o[S];
-#pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const uint32_t ra = res0[i >> 1], rc = res1[i >> 1], r = n & 4 ? rc : ra;
-            o[i] = to_bf16(bf16_bits_to_f32((r >> (16 * (S == 1 ? st0 & 1 : i & 1))) & 0xffffu) +
-                           bf16_bits_to_f32(to_bf16(t[i])));
-          }
-          uint16_t* y = static_cast<uint16_t*>(a.y) + b * kTileN + 4 * c + st0;
-          if (S == 1)
-            y[0] = (uint16_t)o[0];
-          else
-#pragma unroll
-            for (int i = 0; i < S / 2; ++i)
-              reinterpret_cast<uint32_t*>(y)[i] = o[(2 * i) % S] | (o[(2 * i + 1) % S] << 16);
-        }
-        if (n == 7) {
-          rb += 8;
-          load_res();
-          res_here();
-        }
+      } else if (kAdds) {
+        // as emit_rows, by the lanes that hold what the unit adds (every 16 lanes
+        // have its sums)
+        add_close(u, st0, b, t, t);
       } else {
         f32x4 tv[S];
 #pragma unroll
@@ -1125,6 +1164,10 @@ int rows_occ(int S, bool xl) {
                   : rows_wgs_per_cu<OUT, FMT, 1, W>(xl);
 }
 
+// Outputs that k_rows has with 8 waves only: 16 leave 128 registers, and the argmax and
+// the epilogues would spill (M = 1 of a K that k_dec cannot stage is all they lose).
+constexpr bool rows_eight(int out) { return out == OUT_ARGMAX || out == OUT_EPI || out == OUT_GLU; }
+
 // Outputs that M > 1 rows have (fp32 logits are M = 1 only, OUT_NORM's rows are
 // normalized in the staging).
 template <int OUT>
@@ -1171,28 +1214,28 @@ Launch launch_for(int out_f, int G, int M) {
   const int tD = g_dec_tune.D.load(std::memory_order_relaxed);
   const bool regs = mode == 2;
   Launch l;
-  l.S = (OUT != OUT_SWIGLU && 4 * tiles < cus) ? 1 : (OUT == OUT_SWIGLU || tiles < cus) ? 2 : 4;
-  l.W = OUT == OUT_ARGMAX ? 8 : (M == 1 && G >= 64) ? 16 : 8;
-  if ((mode == 1 || mode == 2) && (tS == 1 || tS == 2 || tS == 4) && (OUT != OUT_SWIGLU || tS != 1))
+  l.S = (!out_paired(OUT) && 4 * tiles < cus) ? 1 : (out_paired(OUT) || tiles < cus) ? 2 : 4;
+  l.W = rows_eight(OUT) ? 8 : (M == 1 && G >= 64) ? 16 : 8;
+  if ((mode == 1 || mode == 2) && (tS == 1 || tS == 2 || tS == 4) && (!out_paired(OUT) || tS != 1))
     l.S = tS;
-  if (regs && OUT != OUT_ARGMAX && (tW == 8 || tW == 16)) l.W = tW;
+  if (regs && !rows_eight(OUT) && (tW == 8 || tW == 16)) l.W = tW;
   const int xbytes = M * G * kGroup * 2;
   // the kernel's static LDS + the activations within the CU's LDS
   int static_lds = 0;
-  if constexpr (OUT == OUT_ARGMAX)
+  if constexpr (rows_eight(OUT))
     static_lds = rows_static_lds<OUT, FMT, 8>(l.S);
   else
     static_lds = l.W == 8 ? rows_static_lds<OUT, FMT, 8>(l.S) : rows_static_lds<OUT, FMT, 16>(l.S);
   l.XL = xbytes <= kRowsXChunks * 16 * 64 * l.W && static_lds + xbytes <= kLdsBytes;
   const long long units = (long long)tiles * 4 / l.S;
   int occ = 1;
-  if constexpr (OUT == OUT_ARGMAX)
+  if constexpr (rows_eight(OUT))
     occ = rows_occ<OUT, FMT, 8>(l.S, l.XL);
   else
     occ = l.W == 8 ? rows_occ<OUT, FMT, 8>(l.S, l.XL) : rows_occ<OUT, FMT, 16>(l.S, l.XL);
   if (l.XL) occ = std::max(1, std::min(occ, kLdsBytes / (static_lds + xbytes)));
   // OUT_SWIGLU: whole (gate, up) unit pairs per workgroup
-  l.P = (int)std::max<long long>(1, std::min(OUT == OUT_SWIGLU ? units / 2 : units,
+  l.P = (int)std::max<long long>(1, std::min(out_paired(OUT) ? units / 2 : units,
                                              (long long)cus * occ));
   if (regs) return l;
   if (M == 1 && l.S != 1) {
@@ -1208,7 +1251,7 @@ Launch launch_for(int out_f, int G, int M) {
       l.XL = true;
       const long long u2 = (long long)tiles * 2;
       const long long pc2 = (long long)cus * (kLdsBytes / need);
-      l.P = (int)std::max<long long>(1, std::min(OUT == OUT_SWIGLU ? u2 / 2 : u2, pc2));
+      l.P = (int)std::max<long long>(1, std::min(out_paired(OUT) ? u2 / 2 : u2, pc2));
     }
   } else if (M > 1 && rows_many<OUT>() && l.S != 1) {
     // All M rows staged in LDS once (padded rows, 32-row units, 2 items per
@@ -1229,10 +1272,10 @@ Launch launch_for(int out_f, int G, int M) {
       l.XL = true;
       l.XM = true;
       const long long u2 = (long long)tiles * 2;
-      l.P = (int)std::max<long long>(1, std::min(OUT == OUT_SWIGLU ? u2 / 2 : u2, (long long)cus));
+      l.P = (int)std::max<long long>(1, std::min(out_paired(OUT) ? u2 / 2 : u2, (long long)cus));
       return l;
     }
-    if constexpr (FMT == 4 && (OUT == OUT_BF16 || OUT == OUT_RES)) {
+    if constexpr (FMT == 4 && (OUT == OUT_BF16 || OUT == OUT_RES || OUT == OUT_EPI)) {
       // Otherwise, several units per workgroup: group-major items, each
       // activation group fetched once per workgroup (k_rows_gm). Measured on
       // MI355X against the per-item loads, M = 9 / 16: 24576x8448 24.1 / 24.1 against
@@ -1267,7 +1310,7 @@ Launch launch_for(int out_f, int G, int M) {
       l.XL = false;
       const long long us = (long long)tiles * 4 / S;
       const long long pc2 = (long long)cus * (kLdsBytes / need);
-      l.P = (int)std::max<long long>(1, std::min(OUT == OUT_SWIGLU ? us / 2 : us, pc2));
+      l.P = (int)std::max<long long>(1, std::min(out_paired(OUT) ? us / 2 : us, pc2));
     }
   }
   return l;
@@ -1342,7 +1385,7 @@ bool dec_config(int out_f, int G, int OUTmode, DecCfg& c) {
   const bool fits4 = dec_lds_units(K, G, OUTmode == OUT_NORM, 4, 8, 2) * 16 + dec_static_lds(4, 8) <= kLdsBytes;
   const bool short_k = tiles <= cus && (G < 8 || (OUTmode == OUT_NORM && G < 20 && 4 * tiles > 3 * cus));
   if (v.W == 8) {
-    if (OUTmode == OUT_SWIGLU) {
+    if (out_paired(OUTmode)) {
       const int r1 = dec_swiglu_rows(tiles, 1, cus), r2 = dec_swiglu_rows(tiles, 2, cus),
                 r4 = dec_swiglu_rows(tiles, 4, cus);
       if (r4 <= r2 && fits4)
@@ -1378,7 +1421,7 @@ bool dec_config(int out_f, int G, int OUTmode, DecCfg& c) {
   // one workgroup per CU (gate|up: 256 workgroups 17.6 us, two per CU 19.1 us),
   // and no more than give none of them another unit (gate|up 218 workgroups of
   // 5 units 16.6 us, 256 of 4 or 5 17.1; 17408x5120 182 of 3 10.1, 256 of 2 or 3 10.9)
-  const long long cap = OUTmode == OUT_SWIGLU ? units / 2 : units;
+  const long long cap = out_paired(OUTmode) ? units / 2 : units;
   const long long most = (cap + cus - 1) / cus;
   const int tP = g_dec_tune.P.load(std::memory_order_relaxed);
   c.P = (int)std::max<long long>(1, tP > 0 ? std::min<long long>(cap, tP) : (cap + most - 1) / most);
@@ -1468,15 +1511,20 @@ void prepare_dma_lds() {
     prepare_dec<OUT_RES>();
     prepare_dec<OUT_SWIGLU>();
     prepare_dec<OUT_NORM>();
+    prepare_dec<OUT_EPI>();
+    prepare_dec<OUT_GLU>();
     rows_xr_prepare();
     prepare_gm<OUT_BF16>();
     prepare_gm<OUT_RES>();
+    prepare_gm<OUT_EPI>();
     prepare_dma_out<OUT_BF16, 4>();
     prepare_dma_out<OUT_F32, 4>();
     prepare_dma_out<OUT_ARGMAX, 4>();
     prepare_dma_out<OUT_RES, 4>();
     prepare_dma_out<OUT_SWIGLU, 4>();
     prepare_dma_out<OUT_NORM, 4>();
+    prepare_dma_out<OUT_EPI, 4>();
+    prepare_dma_out<OUT_GLU, 4>();
     prepare_dma_out<OUT_BF16, 8>();
     prepare_dma_out<OUT_ARGMAX, 8>();
   });
@@ -1492,7 +1540,7 @@ void launch_rows_gm(const SkinnyArgs& a, hipStream_t st) {
 
 template <int OUT, int FMT>
 void launch_rows(const SkinnyArgs& a, const Launch& l, hipStream_t st) {
-  if constexpr (FMT == 4 && (OUT == OUT_BF16 || OUT == OUT_RES)) {
+  if constexpr (FMT == 4 && (OUT == OUT_BF16 || OUT == OUT_RES || OUT == OUT_EPI)) {
     if (l.GM) {
       launch_rows_gm<OUT>(a, st);
       return;
@@ -1519,10 +1567,10 @@ void launch_rows(const SkinnyArgs& a, const Launch& l, hipStream_t st) {
       launch_rows_dma_d<OUT, FMT, 2, 8, 4, true>(a, st);
     return;
   }
-  if (OUT == OUT_ARGMAX || l.W == 8)
+  if (rows_eight(OUT) || l.W == 8)
     l.XL ? launch_rows_x<OUT, FMT, 8, true>(a, l.S, st) : launch_rows_x<OUT, FMT, 8, false>(a, l.S, st);
   else
-    if constexpr (OUT != OUT_ARGMAX)
+    if constexpr (!rows_eight(OUT))
       l.XL ? launch_rows_x<OUT, FMT, 16, true>(a, l.S, st)
            : launch_rows_x<OUT, FMT, 16, false>(a, l.S, st);
 }
@@ -1542,6 +1590,7 @@ struct Epi {
   const uint16_t* nw = nullptr;
   float eps = 0.f;
   bool tmp_ok = false;   // OUT_NORM: the caller can run rmsnorm into a buffer first
+  Epilogue epi = {};     // OUT_EPI, OUT_GLU
 };
 
 // run_skinny's internal status (never returned through the C-ABI): an rmsnorm
@@ -1561,7 +1610,7 @@ int run_skinny(void* y, const WeightView& w, const uint16_t* x, int M, qw4_scrat
   if (tiles > s->max_tiles || M > s->max_m || w.in_f > s->max_in) return QW4_ERR_SCRATCH;
   // loads address weights and x through 32-bit buffer offsets
   if (w.weight_bytes >= (1ull << 32)) return QW4_ERR_SHAPE;
-  if (OUT == OUT_SWIGLU && (w.out_f % (2 * kTileN))) return QW4_ERR_SHAPE;
+  if (out_paired(OUT) && (w.out_f % (2 * kTileN))) return QW4_ERR_SHAPE;
   if (OUT == OUT_RES && !e.res) return QW4_ERR_NULL;
   if (OUT == OUT_NORM && !e.nw) return QW4_ERR_NULL;
   SkinnyArgs a{};
@@ -1581,7 +1630,8 @@ int run_skinny(void* y, const WeightView& w, const uint16_t* x, int M, qw4_scrat
   a.res = e.res;
   a.nw = e.nw;
   a.eps = e.eps;
-  a.ld = OUT == OUT_SWIGLU ? w.out_f / 2 : w.out_f;
+  a.epi = e.epi;
+  a.ld = out_paired(OUT) ? w.out_f / 2 : w.out_f;
   const int mode = g_dec_tune.mode.load(std::memory_order_relaxed);
   if constexpr (FMT == 4) {
     DecCfg dc{};
@@ -1697,7 +1747,7 @@ using namespace qw4;
 
 // qw4_linear's pass of 17 to 32 rows over one reading of the weights: the checks of qw4_gemm_small, then k_rows_xr with two row blocks.
 int qw4::skinny_rows32(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_scratch* s,
-                       void* stream, bool* taken) {
+                       void* stream, const Epilogue* e, bool* taken) {
   *taken = false;
   int st = check_weights_public(w);
   if (st) return st;
@@ -1715,14 +1765,25 @@ int qw4::skinny_rows32(uint16_t* y, const qw4_weights* w, const uint16_t* x, int
   a.x = x;
   a.y = y;
   a.M = M;
-  a.N = a.ld = w->out_f;
+  const int out = !e ? OUT_BF16 : e->act == QW4_ACT_SWIGLU ? OUT_GLU : OUT_EPI;
+  if (e) a.epi = *e;
+  a.N = w->out_f;
+  a.ld = out_paired(out) ? w->out_f / 2 : w->out_f;
   a.K = w->in_f;
   a.G = w->num_groups;
   a.tiles = tiles;
   a.weight_bytes = (uint32_t)weight_bytes;
-  *taken = rows_xr2_launch(a, device_cus(), (hipStream_t)stream);
+  *taken = rows_xr2_launch(out, a, device_cus(), (hipStream_t)stream);
   if (*taken) QW4_LAUNCH_CHECK();
   return QW4_OK;
+}
+
+int qw4::skinny_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_scratch* s,
+                         const Epilogue& e, void* stream) {
+  Epi in;
+  in.epi = e;
+  return e.act == QW4_ACT_SWIGLU ? run_skinny<OUT_GLU>(y, w, x, M, s, stream, in)
+                                 : run_skinny<OUT_EPI>(y, w, x, M, s, stream, in);
 }
 
 extern "C" {

@@ -29,8 +29,14 @@ QW4_ERR_NOMEM = 8
 QW4_ERR_LAYOUT = 9
 QW4_ERR_IO = 10
 QW4_ERR_NOTFOUND = 11
+QW4_ERR_ACT = 12
 LAYOUT_AWQ_K = 1
 LAYOUT_AWQ_N = 2
+ACT_NONE = 0
+ACT_SILU = 1
+ACT_GELU = 2
+ACT_GELU_TANH = 3
+ACT_SWIGLU = 4
 
 # Every symbol include/qwen_w4a16.h declares.
 EXPORTS = (
@@ -48,7 +54,7 @@ EXPORTS = (
     "qw4_gemv_rmsnorm", "qw4_linear", "qw4_linear_max_t", "qw4_mfma_peak", "qw4_tune_decode",
     "qw4_tune_gemm", "qw4_tune_linear", "qw4_gemv_argmax_noalloc",
     "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
-    "qw4_route_ids", "qw4_combine",
+    "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue",
 )
 
 # safetensors dtype order (qw4_st_tensor.dtype)
@@ -190,6 +196,7 @@ def lib():
         "qw4_route": ([vp, vp, PL, vp, i, i, i, i, vp], i),
         "qw4_route_f32": ([vp, vp, PL, vp, i, i, i, i, vp], i),
         "qw4_route_ids": ([PL, vp, i, i, vp], i),
+        "qw4_linear_epilogue": ([vp, W, vp, i, vp, i, vp, S, WS, vp], i),
         "qw4_combine": ([vp, vp, PL, vp, i, i, i, vp, vp], i),
     }
     for name, (args, res) in sig.items():
@@ -444,6 +451,21 @@ def linear_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch, ws: GemmWorkspac
     _need(x, max(T, 0) * w.in_f * 2, "linear x")
     _chk(lib().qw4_linear(_ptr(y), C.byref(w), _ptr(x), T, C.byref(s),
                           C.byref(ws) if ws is not None else None, _stream(stream)), "linear")
+
+
+def linear_epilogue_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch | None = None,
+                          ws: GemmWorkspace | None = None, bias=None, act: int = ACT_NONE,
+                          residual=None, stream=None) -> None:
+    """qw4_linear_epilogue: y = bf16(act(x @ W^T + bias) + residual), one rounding."""
+    width = w.out_f // 2 if act == ACT_SWIGLU else w.out_f
+    _need(y, T * width * 2, "linear_epilogue y")
+    _need(x, T * w.in_f * 2, "linear_epilogue x")
+    _need(bias, w.out_f * 2, "linear_epilogue bias")
+    _need(residual, T * width * 2, "linear_epilogue residual")
+    _chk(lib().qw4_linear_epilogue(_ptr(y), C.byref(w), _ptr(x), T, _ptr(bias), act, _ptr(residual),
+                                   C.byref(s) if s is not None else None,
+                                   C.byref(ws) if ws is not None else None, _stream(stream)),
+         "linear_epilogue")
 
 
 def tune_decode(mode: int = 0, S: int = 0, W: int = 0, D: int = 0, P: int = 0) -> None:

@@ -90,3 +90,31 @@ def test_binding_checks(hip):
     with pytest.raises(hip.W4A16Error) as e:
         hip.route_experts(0x1000, 0x2000, 0x3000, 1, 8, 9, True, stream=0)
     assert e.value.status == hip.QW4_ERR_SHAPE
+
+
+def _weights(hip, out_f=256, in_f=512):
+    w = hip.W4A16Weights()
+    w.qweight, w.scale, w.zeros = 0x1000, 0x2000, 0x3000
+    w.out_f, w.in_f, w.group_size, w.num_groups = out_f, in_f, 128, in_f // 128
+    return w
+
+
+def test_linear_epilogue_refusals(hip):
+    L = hip.lib()
+    w = _weights(hip)
+
+    def call(T=4, act=0, y=0x10000, x=0x20000, b=None, r=None, w=w, s=None):
+        return L.qw4_linear_epilogue(P(y), C.byref(w) if w else None, P(x), T, P(b), act, P(r),
+                                     C.byref(s) if s else None, None, None)
+
+    assert call(T=0) == hip.QW4_ERR_M
+    assert call(y=None) == hip.QW4_ERR_NULL
+    assert call(x=None) == hip.QW4_ERR_NULL
+    assert call(w=None) == hip.QW4_ERR_NULL
+    assert call(act=5) == hip.QW4_ERR_ACT
+    assert call(act=-1) == hip.QW4_ERR_ACT
+    assert call(act=hip.ACT_SWIGLU, w=_weights(hip, out_f=192)) == hip.QW4_ERR_SHAPE
+    assert call(w=_weights(hip, out_f=200)) == hip.QW4_ERR_SHAPE
+    for name in ("y", "x", "b", "r"):
+        assert call(**{name: 0x40008}) == hip.QW4_ERR_ALIGN
+    assert call(T=1 << 23) == hip.QW4_ERR_SHAPE   # x beyond 32-bit offsets
