@@ -410,6 +410,19 @@ int qw4_route_f32(int32_t* ids, float* weights, const qw4_plan* plan, const floa
  * plan->experts) has no expert here (on this GPU). */
 int qw4_route_ids(const qw4_plan* plan, const int32_t* ids, int T, int top_k, void* stream);
 
+/* y [pairs][width]: row i in [offsets[e], offsets[e + 1]) is bf16(act(r W_e^T + bias_e)),
+ * r the row plan->tokens[i] of x (gather != 0; x [x_rows][in_f]) or row i of x (x_rows
+ * >= pairs). w holds the experts' weights one after the other (awq_repack_into at row
+ * offset e n): out_f = experts n, n % 64 == 0 (QW4_ACT_SWIGLU: n % 128, each expert
+ * [gate | up]); width = n, or n / 2. bias [out_f] bf16 may be NULL. fp32 up to the one
+ * rounding, weights rounded to bf16 where an expert has many rows. pairs = the T
+ * top_k the plan was made for: rows behind offsets[experts] are left as they were,
+ * a token outside x counts as zeros. Pointers 16-byte aligned; a gathered x below
+ * 4 GiB. ws may be NULL. */
+int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x_rows,
+                     const qw4_plan* plan, int pairs, int gather, const uint16_t* bias, int act,
+                     qw4_workspace* ws, void* stream);
+
 /* out [T][dim] = bf16(residual + sum_j weights[t][j] y[plan->pos[t top_k + j]]), in
  * fp32, slots in order; y [T top_k][dim] bf16 in plan order, pairs without an
  * expert add nothing. residual [T][dim] (may be NULL, may be out). dim % 8 == 0;

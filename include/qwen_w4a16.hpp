@@ -177,6 +177,9 @@ void route_experts_f32(int32_t* ids, float* weights, const qw4_plan* plan, const
                        int experts, int top_k, bool renorm, hipStream_t stream = 0);
 void route_expert_ids(const qw4_plan& plan, const int32_t* ids, int T, int top_k,
                       hipStream_t stream = 0);
+void gemm_grouped_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int x_rows,
+                        const qw4_plan& plan, int pairs, bool gather, const __hip_bfloat16* bias,
+                        int act, GemmWorkspace& ws, hipStream_t stream = 0);
 void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_plan& plan,
                      const float* weights, int T, int top_k, int dim, const __hip_bfloat16* residual,
                      hipStream_t stream = 0);

@@ -313,6 +313,15 @@ void route_expert_ids(const qw4_plan& plan, const int32_t* ids, int T, int top_k
   check(qw4_route_ids(&plan, ids, T, top_k, stream), "route_expert_ids");
 }
 
+void gemm_grouped_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int x_rows,
+                        const qw4_plan& plan, int pairs, bool gather, const __hip_bfloat16* bias,
+                        int act, GemmWorkspace& ws, hipStream_t stream) {
+  const qw4_weights v = view(w);
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_gemm_grouped(u16(y), &v, u16(x), x_rows, &plan, pairs, gather, u16(bias), act, &q, stream),
+        "gemm_grouped_w4a16");
+}
+
 void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_plan& plan,
                      const float* weights, int T, int top_k, int dim, const __hip_bfloat16* residual,
                      hipStream_t stream) {

@@ -54,7 +54,7 @@ EXPORTS = (
     "qw4_gemv_rmsnorm", "qw4_linear", "qw4_linear_max_t", "qw4_mfma_peak", "qw4_tune_decode",
     "qw4_tune_gemm", "qw4_tune_linear", "qw4_gemv_argmax_noalloc",
     "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
-    "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue",
+    "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue", "qw4_gemm_grouped",
 )
 
 # safetensors dtype order (qw4_st_tensor.dtype)
@@ -197,6 +197,7 @@ def lib():
         "qw4_route_f32": ([vp, vp, PL, vp, i, i, i, i, vp], i),
         "qw4_route_ids": ([PL, vp, i, i, vp], i),
         "qw4_linear_epilogue": ([vp, W, vp, i, vp, i, vp, S, WS, vp], i),
+        "qw4_gemm_grouped": ([vp, W, vp, i, PL, i, i, vp, i, WS, vp], i),
         "qw4_combine": ([vp, vp, PL, vp, i, i, i, vp, vp], i),
     }
     for name, (args, res) in sig.items():
@@ -622,6 +623,23 @@ def route_expert_ids(plan: ExpertPlan, ids, T: int, top_k: int, stream=None) -> 
     """qw4_route_ids: the plan of ids [T][top_k] chosen elsewhere."""
     _need(ids, T * top_k * 4, "route_expert_ids ids")
     _chk(lib().qw4_route_ids(C.byref(plan), _ptr(ids), T, top_k, _stream(stream)), "route_expert_ids")
+
+
+def gemm_grouped_w4a16(y, w: W4A16Weights, x, plan: ExpertPlan, pairs: int, gather: bool,
+                       bias=None, act: int = ACT_NONE, ws: GemmWorkspace | None = None,
+                       x_rows: int | None = None, stream=None) -> None:
+    """qw4_gemm_grouped: row i of expert e = bf16(act(r @ W_e^T + bias_e)), r the row
+    plan.tokens[i] (gather) or i of x. x_rows: rows of a raw-pointer x (a tensor's
+    first dimension otherwise)."""
+    if x_rows is None:
+        x_rows = x.numel() // w.in_f
+    width = w.out_f // max(plan.experts, 1) // (2 if act == ACT_SWIGLU else 1)
+    _need(y, pairs * width * 2, "gemm_grouped y")
+    _need(x, x_rows * w.in_f * 2, "gemm_grouped x")
+    _need(bias, w.out_f * 2, "gemm_grouped bias")
+    _chk(lib().qw4_gemm_grouped(_ptr(y), C.byref(w), _ptr(x), x_rows, C.byref(plan), pairs, int(gather),
+                                _ptr(bias), act, C.byref(ws) if ws is not None else None,
+                                _stream(stream)), "gemm_grouped")
 
 
 def combine_experts(out, y, weights, T: int, top_k: int, dim: int, plan: ExpertPlan, residual=None,

@@ -118,3 +118,34 @@ def test_linear_epilogue_refusals(hip):
     for name in ("y", "x", "b", "r"):
         assert call(**{name: 0x40008}) == hip.QW4_ERR_ALIGN
     assert call(T=1 << 23) == hip.QW4_ERR_SHAPE   # x beyond 32-bit offsets
+
+
+def test_gemm_grouped_refusals(hip):
+    L = hip.lib()
+    w = _weights(hip, out_f=1024)
+
+    def call(pairs=16, x_rows=16, gather=0, act=0, y=0x10000, x=0x20000, b=None, w=w, plan=_plan(hip)):
+        return L.qw4_gemm_grouped(P(y), C.byref(w) if w else None, P(x), x_rows,
+                                  C.byref(plan) if plan else None, pairs, gather, P(b), act, None, None)
+
+    assert call(w=None) == hip.QW4_ERR_NULL
+    assert call(plan=None) == hip.QW4_ERR_NULL
+    assert call(y=None) == hip.QW4_ERR_NULL
+    assert call(x=None) == hip.QW4_ERR_NULL
+    assert call(pairs=-1) == hip.QW4_ERR_M
+    assert call(pairs=65, x_rows=65) == hip.QW4_ERR_SCRATCH
+    assert call(x_rows=15) == hip.QW4_ERR_SHAPE                       # in order: a row for each position
+    assert call(act=7) == hip.QW4_ERR_ACT
+    assert call(act=hip.ACT_SWIGLU, w=_weights(hip, out_f=512)) == hip.QW4_ERR_SHAPE   # 64 rows an expert
+    assert call(plan=_plan(hip, experts=7)) == hip.QW4_ERR_SHAPE      # 1024 rows are no 7 experts
+    assert call(plan=_plan(hip, experts=32)) == hip.QW4_ERR_SHAPE     # 32 rows an expert
+    assert call(plan=_plan(hip, experts=0)) == hip.QW4_ERR_SHAPE
+    assert call(gather=1, x_rows=1 << 22) == hip.QW4_ERR_SHAPE        # 4 GiB of x
+    bad = _plan(hip)
+    bad.tokens = None
+    assert call(gather=1, plan=bad) == hip.QW4_ERR_NULL
+    bad.offsets = None
+    assert call(plan=bad) == hip.QW4_ERR_NULL
+    for name in ("y", "x", "b"):
+        assert call(**{name: 0x40008}) == hip.QW4_ERR_ALIGN
+    assert call(pairs=0, y=None, x=None) == hip.QW4_OK
