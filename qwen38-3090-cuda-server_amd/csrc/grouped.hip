@@ -9,6 +9,7 @@
 
 #include "../../include/qwen_w4a16.h"
 #include "gemm_tile.h"
+#include "grouped.h"
 #include "skinny.h"
 #include "w4a16_common.h"
 
@@ -16,86 +17,6 @@ namespace qw4 {
 int check_weights_public(const qw4_weights* w);
 
 namespace {
-
-constexpr int kMaxExperts = 1024;
-
-struct GroupedArgs {
-  const uint32_t* qw;
-  const uint16_t* sc;
-  const uint16_t* zr;
-  const uint16_t* x;
-  uint16_t* y;
-  const int32_t* offsets;   // [E + 1]
-  const int32_t* tokens;    // row of x at each position
-  Epilogue epi;             // bias and up of an expert's weight rows; no residual
-  int E, n, K, G;           // n weight rows an expert
-  int R;                    // positions (rows of y)
-  uint32_t x_bytes;         // of a gathered x
-  int ld;                   // columns of y
-  int tiles_n, P;           // column tiles of an expert, workgroups
-};
-
-// Expert e's positions. Offsets that are no plan's (negative, falling, past R) give
-// fewer or no rows, never one outside y.
-__device__ __forceinline__ void expert_rows(const GroupedArgs& a, int e, int& lo, int& hi) {
-  lo = min(max(a.offsets[e], 0), a.R);
-  hi = min(max(a.offsets[e + 1], lo), a.R);
-}
-
-// Blocks of `rows` positions: start[e] = those of the experts before e, returned: all.
-// 256 threads, four experts each.
-template <int ROWS>
-__device__ __forceinline__ int block_starts(const GroupedArgs& a, int* start, int* wsum) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  int n[4], sum = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = 4 * t + i;
-    n[i] = 0;
-    if (e < a.E) {
-      int lo, hi;
-      expert_rows(a, e, lo, hi);
-      n[i] = (hi - lo + ROWS - 1) / ROWS;
-    }
-    sum += n[i];
-  }
-  int run = sum;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int v = __shfl_up(run, off, 64);
-    if (lane >= off) run += v;
-  }
-  if (lane == 63) wsum[wave] = run;
-  __syncthreads();
-  int before = run - sum, all = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    before += w < wave ? wsum[w] : 0;
-    all += wsum[w];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (4 * t + i <= a.E) start[4 * t + i] = before;
-    before += n[i];
-  }
-  if (t == 255 && a.E == kMaxExperts) start[kMaxExperts] = before;
-  __syncthreads();
-  return all;
-}
-
-// The last expert whose first tile is at or before t (experts without rows start where
-// the next one does, so it has rows).
-__device__ __forceinline__ int expert_of(const int* start, int E, int tiles_n, int t) {
-  int lo = 0, hi = E;   // start[lo] tiles_n <= t < start[hi] tiles_n
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] * tiles_n <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
 
 // Many rows an expert: the MFMA tile of the prefill GEMM (gemm_tile.h) over (expert, row
 // block, column tile). Tiles go expert by expert, a column tile's row blocks together,
@@ -108,7 +29,7 @@ __global__ __launch_bounds__(256, 1) void k_grouped_tiles(GroupedArgs a) {
   __shared__ int start[kMaxExperts + 1];
   __shared__ int wsum[4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int all = __builtin_amdgcn_readfirstlane(block_starts<32 * MB>(a, start, wsum)) * a.tiles_n;
+  const int all = __builtin_amdgcn_readfirstlane(block_starts<32 * MB, 256>(a, start, wsum)) * a.tiles_n;
   const uint32_t row_bytes = (uint32_t)a.K * 2u;
   const int srow = 4 * wave + (lane >> 4);   // row within the 16-row swizzle period
   const uint32_t chunk = (uint32_t)((lane & 15) ^ srow) * 16u;
@@ -232,7 +153,11 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   a.ld = glu ? n / 2 : n;
   a.tiles_n = (n + G2_BN - 1) / G2_BN;
   const int cus = device_cus();
-  const int mb = 4;
+  if (grouped_rows_launch(a, glu, cus, (hipStream_t)stream)) {
+    QW4_LAUNCH_CHECK();
+    return QW4_OK;
+  }
+  constexpr int mb = 4;
   const long long most = ((long long)pairs / (32 * mb) + std::min(a.E, pairs)) * a.tiles_n;
   if (most > 0x7fffffffLL) return QW4_ERR_SHAPE;
   a.P = (int)std::min<long long>(most, cus);
