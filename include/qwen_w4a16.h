@@ -364,12 +364,19 @@ enum {
  * rounding (the separate steps, and qw4_gemv_residual / _swiglu, round the
  * projection to bf16 first). width = out_f; QW4_ACT_SWIGLU: out_f / 2, out_f % 128
  * == 0. bias [out_f] and residual [T][width] bf16, each may be NULL; residual may be
- * y. Any T >= 1, on qw4_linear's paths: whole weights in up to qw4_linear_max_t(w)
- * rows with a scratch, weights rounded to bf16 (qw4_gemm) beyond or without one. s
- * and ws may be NULL. All pointers 16-byte aligned. */
+ * y. Any T >= 1, on qw4_linear's paths: exact weights in up to qw4_linear_max_t(w)
+ * rows with a scratch; beyond or without one, weights rounded to bf16 (qw4_gemm), or,
+ * for QW4_ACT_SWIGLU with a 256-byte aligned workspace of at least
+ * qw4_epilogue_workspace(w, T) bytes, to 11 bits: each factor of a gated output carries
+ * the weights' rounding. s and ws may be NULL; calls that share one must be
+ * stream-ordered. All pointers 16-byte aligned. */
 int qw4_linear_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T,
                         const uint16_t* bias, int act, const uint16_t* residual, qw4_scratch* s,
                         qw4_workspace* ws, void* stream);
+/* Bytes of a workspace that a gated product over `rows` rows of x takes (x in 16 bits
+ * and the rows' exponents). qw4_linear_epilogue also splits tiles as qw4_gemm does when
+ * the workspace holds that on top. 0 for bad arguments. */
+size_t qw4_epilogue_workspace(const qw4_weights* w, int rows);
 
 /* ------------------------------------------------------- layers of experts
  * A token's feed-forward spread over experts (no reference counterpart: its
@@ -415,7 +422,10 @@ int qw4_route_ids(const qw4_plan* plan, const int32_t* ids, int T, int top_k, vo
  * >= pairs). w holds the experts' weights one after the other (awq_repack_into at row
  * offset e n): out_f = experts n, n % 64 == 0 (QW4_ACT_SWIGLU: n % 128, each expert
  * [gate | up]); width = n, or n / 2. bias [out_f] bf16 may be NULL. fp32 up to the one
- * rounding, weights rounded to bf16 where an expert has many rows. pairs = the T
+ * rounding. Weights are exact where experts have few rows (pairs / experts at most 32,
+ * in_f at most 8192); beyond, they are rounded to bf16, or, in a gated product with a
+ * 256-byte aligned workspace of qw4_epilogue_workspace(w, rows of x) bytes, to 11 bits.
+ * Calls that share a workspace must be stream-ordered. pairs = the T
  * top_k the plan was made for: rows behind offsets[experts] are left as they were,
  * a token outside x counts as zeros. Pointers 16-byte aligned; a gathered x below
  * 4 GiB. ws may be NULL. */

@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/qwen_w4a16.h"
 #include "gemm_tile.h"
@@ -28,8 +29,10 @@ int check_weights_public(const qw4_weights* w);
 namespace {
 
 // Outputs of k_gemm: the product in bf16; with an epilogue; with an epilogue that
-// joins gate and up (C, residual and ld of half the weight's rows).
-enum { GEMM_PLAIN = 0, GEMM_EPI = 1, GEMM_GLU = 2 };
+// joins gate and up (C, residual and ld of half the weight's rows), the operands in
+// bf16 or, with a workspace for them, in fp16.
+enum { GEMM_PLAIN = 0, GEMM_EPI = 1, GEMM_GLU = 2, GEMM_GLU16 = 3 };
+constexpr bool gemm_glu(int out) { return out == GEMM_GLU || out == GEMM_GLU16; }
 
 struct GemmArgs {
   const uint32_t* qw;
@@ -47,6 +50,7 @@ struct GemmArgs {
   int U;                // (tile, group) units of tiles [full, tiles), split over P
   Epilogue epi;
   int ld;               // row stride of C and the residual
+  const int *rexp, *cexp;   // GEMM_GLU16: exponents of rows and columns
 };
 
 // Linear tile index -> (tn, tm), in bands of 4 M-tiles: consecutive tiles
@@ -75,7 +79,7 @@ struct WaveTile {
 };
 template <int OUT>
 __device__ __forceinline__ WaveTile g2_wave_tile(const GemmArgs& a, int tn, int wt, int b0) {
-  if (OUT == GEMM_GLU) {
+  if (gemm_glu(OUT)) {
     const int t = tn * 2 + (wt >> 1);
     return {t, wt & 1, t * kTileN + 32 * (wt & 1), t * kTileN < a.ld};
   }
@@ -227,7 +231,7 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   g2_tile_coords(a, t, tn, tm);
   const WaveTile w = g2_wave_tile<OUT>(a, tn, wt, b0);
   if (!w.valid) return;
-  auto pair = [&](int e) { return OUT == GEMM_GLU ? e * MBW + part : part * kPer + e; };
+  auto pair = [&](int e) { return gemm_glu(OUT) ? e * MBW + part : part * kPer + e; };
   const __amdgpu_buffer_rsrc_t rs =
       __builtin_amdgcn_make_buffer_rsrc(a.slots, 0, (int)(2u * a.P * kSlotBytes), 0x00020000);
   f32x16v acc[kPer];
@@ -266,25 +270,29 @@ __global__ __launch_bounds__(64) void k_gemm_fixup(GemmArgs a) {
   const int m0 = tm * g2_tile_rows<NW, MB>(a);
   if constexpr (OUT != GEMM_PLAIN) {
     // straight from the accumulators' layout: 4 columns of a row at a time
-    constexpr int kOuts = OUT == GEMM_GLU ? 1 : kPer;
+    constexpr int kOuts = gemm_glu(OUT) ? 1 : kPer;
 #pragma unroll
     for (int e = 0; e < kOuts; ++e) {
       const int idx = pair(e), mb = idx % MBW;
       const int m = m0 + 32 * (mw + mb) + r;
       const bool in = m < g2_row_end<NW>(a, m0);
-      const int col = w.col + (OUT == GEMM_GLU ? 0 : 32 * (idx / MBW)) + 4 * h;
-      float v[OUT == GEMM_GLU ? 2 : 1][16];
+      const int col = w.col + (gemm_glu(OUT) ? 0 : 32 * (idx / MBW)) + 4 * h;
+      float v[gemm_glu(OUT) ? 2 : 1][16];
 #pragma unroll
-      for (int j = 0; j < (OUT == GEMM_GLU ? 2 : 1); ++j)
+      for (int j = 0; j < (gemm_glu(OUT) ? 2 : 1); ++j)
 #pragma unroll
         for (int jq = 0; jq < 4; ++jq) {
           u32x2 b = {0u, 0u};
           if (a.epi.bias) b = *reinterpret_cast<const u32x2*>(a.epi.bias + j * a.epi.up + col + 8 * jq);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[j][4 * jq + i] = acc[e + j][4 * jq + i] + bf16_bits_to_f32((b[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+          for (int i = 0; i < 4; ++i) {
+            float f = acc[e + j][4 * jq + i];
+            if (OUT == GEMM_GLU16 && in)
+              f = __builtin_ldexpf(f, a.rexp[m] + a.cexp[j * a.epi.up + col + 8 * jq + i]);
+            v[j][4 * jq + i] = f + bf16_bits_to_f32((b[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+          }
         }
-      epilogue_act<OUT == GEMM_GLU>(v, a.epi.act);
+      epilogue_act<gemm_glu(OUT)>(v, a.epi.act);
       if (!in) continue;
 #pragma unroll
       for (int jq = 0; jq < 4; ++jq) {
@@ -349,7 +357,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
   const uint32_t row_bytes = (uint32_t)a.K * 2u;
   const int srow = 4 * (wave & 3) + (lane >> 4);   // row within the 16-row swizzle period
   const G2Rows rows{(uint32_t)(lane >> 4) * row_bytes + (uint32_t)((lane & 15) ^ srow) * 16u, row_bytes};
-  constexpr bool kGlu = OUT == GEMM_GLU;
+  constexpr bool kGlu = gemm_glu(OUT);
+  using Op = std::conditional_t<OUT == GEMM_GLU16, G2F16, G2Bf16>;
   const int up = a.epi.up / kTileN;
   // groups [g0, g1) of tile t; stored if they are the whole tile
   auto segment = [&](int t, int g0, int g1) __attribute__((always_inline)) {
@@ -360,7 +369,9 @@ __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
     const int ltile = w.valid ? w.tile : (kGlu ? a.ld : a.N) / kTileN - 1;
     // Activation rows [m0, row end): the buffer's end turns rows past it into zeros.
     const uint16_t* A0 = a.A + (size_t)m0 * a.K;
-    g2_segment<NH, NW, MB, kGlu>(a.G, wr, none, g2_rsrc(A0, (uint32_t)(g2_row_end<NW>(a, m0) - m0) * row_bytes),
+    int norm[NH] = {};
+    if constexpr (Op::kNorm) g2_load_norms<NH, kGlu>(norm, a.cexp, ltile, up, w.b0, lane);
+    g2_segment<NH, NW, MB, kGlu, Op, 0>(a.G, norm, wr, none, g2_rsrc(A0, (uint32_t)(g2_row_end<NW>(a, m0) - m0) * row_bytes),
                                  g2_rsrc(A0, 0), rows, lds, acc, ltile, up, w.b0, mw, g0, g1, wave, lane);
     if (g0 != 0 || g1 != a.G) return false;
     if constexpr (OUT == GEMM_PLAIN) {
@@ -370,7 +381,8 @@ __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
       Epilogue e = a.epi;
       if (e.bias) e.bias += w.col;
       if (e.res) e.res += at;
-      g2_store_epilogue<MB, kGlu>(acc, &lds[0][0], a.C + at, e, a.ld, a.M - m0, w.valid, wave, lane);
+      g2_store_epilogue<MB, kGlu, Op, 0>(acc, &lds[0][0], a.C + at, e, a.rexp + m0, a.cexp + w.col, a.ld,
+                                         a.M - m0, w.valid, wave, lane);
     }
     return true;
   };
@@ -502,7 +514,15 @@ int run_gemm(uint16_t* C, const qw4_weights* w, const uint16_t* A, int M, qw4_wo
   const int schedule = g_gemm_schedule.load(std::memory_order_relaxed);
   const int variant = OUT == GEMM_PLAIN ? g_gemm_variant.load(std::memory_order_relaxed) : 0;
   const int cus = device_cus();
-  const bool ws_ok = ws && ws->buf && ws->bytes >= gemm_workspace_need(cus) && cus % 8 == 0;
+  // fp16 operands at the end of the workspace, partial tiles at its start
+  HalfRows half{};
+  size_t space = ws && ws->buf ? ws->bytes & ~(size_t)255 : 0;
+  if constexpr (OUT == GEMM_GLU16) {
+    space -= half_rows_bytes(M, w);
+    half = half_rows(static_cast<char*>(ws->buf) + space, A, M, w, (hipStream_t)stream);
+    A = half.x;
+  }
+  const bool ws_ok = space >= gemm_workspace_need(cus) && cus % 8 == 0;
   GemmPlan p = gemm_plan(M, w->out_f, w->num_groups, 8, cus, ws_ok, schedule);
   // Tiles of fewer rows where that costs less: rows that do not fill 256-row
   // tiles (us, 256-row tiles against the plan's: gate|up 34816x5120 at 64 / 128 /
@@ -524,7 +544,7 @@ int run_gemm(uint16_t* C, const qw4_weights* w, const uint16_t* A, int M, qw4_wo
   const int nt = p.tiles_n * p.tiles_m, mb = p.mb;
   GemmArgs a{w->qweight, w->scale, w->zeros, A, C, nullptr, M, w->out_f, w->in_f,
              w->num_groups, p.tiles_n, p.tiles_m, nt % 8 == 0, 32 * mb, nt, nt, 0,
-             epi, OUT == GEMM_GLU ? w->out_f / 2 : w->out_f};
+             epi, gemm_glu(OUT) ? w->out_f / 2 : w->out_f, half.rexp, half.cexp};
   int grid = nt;
   if (p.pick == 3) {
     a.slots = static_cast<float*>(ws->buf);
@@ -606,6 +626,9 @@ int qw4_gemm(uint16_t* C, const qw4_weights* w, const uint16_t* A, int M, qw4_wo
 
 int qw4::gemm_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_workspace* ws,
                        const Epilogue& e, void* stream) {
-  return e.act == QW4_ACT_SWIGLU ? run_gemm<GEMM_GLU>(y, w, x, M, ws, e, stream)
-                                 : run_gemm<GEMM_EPI>(y, w, x, M, ws, e, stream);
+  if (e.act != QW4_ACT_SWIGLU) return run_gemm<GEMM_EPI>(y, w, x, M, ws, e, stream);
+  if (ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && (size_t)M * w->in_f * 2 < (1ull << 32) &&
+      (ws->bytes & ~(size_t)255) >= half_rows_bytes(M, w))
+    return run_gemm<GEMM_GLU16>(y, w, x, M, ws, e, stream);
+  return run_gemm<GEMM_GLU>(y, w, x, M, ws, e, stream);
 }

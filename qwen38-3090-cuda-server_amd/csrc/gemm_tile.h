@@ -10,6 +10,17 @@
 
 namespace qw4 {
 
+// x in fp16 with an exponent a row, and an exponent for each weight row (k_half_rows).
+struct HalfRows {
+  const uint16_t* x;
+  const int *rexp, *cexp;
+};
+// Bytes of a workspace that they take.
+size_t half_rows_bytes(int T, const qw4_weights* w);
+// Fills them, from buf on (half_rows.hip).
+HalfRows half_rows(void* buf, const uint16_t* x, int T, const qw4_weights* w, hipStream_t s);
+
+
 // ---------------------------------------------------------------------------
 // k_gemm: 256 (M) x 256 (N) workgroup tile -- 32 MB (M) for MB = 2..7 m-blocks
 // where the rows do not fill 256 (gemm_plan) -- v_mfma_f32_32x32x16_bf16 (the
@@ -48,7 +59,8 @@ typedef float f32x16v __attribute__((ext_vector_type(16)));
 //    m-blocks (half the LDS reads, every weight dequantized once; its 256
 //    accumulator registers take the AGPR half of the register file).
 // MB: 32-row m-blocks of the workgroup's tile, 8 unless fewer rows need it.
-template <int NH, int NW, int MB>
+// DD: groups buffered, 0 for as many as the CU's LDS holds.
+template <int NH, int NW, int MB, int DD = 0>
 struct G2Split {
   static constexpr int MBW = 8 * MB / (NW * NH);     // m-blocks per wave
   static constexpr int UNITS = NH * MBW;             // (half, m-block) pairs per wave
@@ -57,7 +69,7 @@ struct G2Split {
   // groups buffered: as many 8 MB KiB activation buffers as LDS holds, 4 at most
   // (MB = 5: three buffers spill 14 VGPRs, 60 bytes a lane, and are still faster
   // than two without a spill: whole tiles 3%, split-K 1%, the others equal)
-  static constexpr int DEPTH = MB <= 4 ? 4 : MB == 5 ? 3 : 2;
+  static constexpr int DEPTH = DD ? DD : MB <= 4 ? 4 : MB == 5 ? 3 : 2;
   // k-step schedule (measured on MI355X at the config-4 shapes): VALU slots
   // after each MFMA, LDS operand reads after each of the first MFMAs, and the
   // k-steps that carry the next group's activation loads.
@@ -96,6 +108,18 @@ __device__ __forceinline__ G2Rsrc g2_weights(const uint32_t* qw, const uint16_t*
                                              int N, int G, bool some = true) {
   const uint32_t blocks = some ? (uint32_t)N / kTileN * (uint32_t)G : 0u;
   return {g2_rsrc(qw, blocks * 4096u), g2_rsrc(sc, blocks * (uint32_t)kMetaBytes), g2_rsrc(zr, blocks * 32u)};
+}
+
+// The exponents of a lane's weight rows (part j as in g2_load_weights), cexp [N].
+template <int NH, bool GLU>
+__device__ __forceinline__ void g2_load_norms(int (&norm)[NH], const int* cexp, int tile, int up, int b0,
+                                              int lane) {
+  const int r = lane & 31;
+#pragma unroll
+  for (int j = 0; j < NH; ++j) {
+    const int a16 = 8 * (GLU ? b0 : b0 + j) + 2 * (r >> 3) + ((r >> 2) & 1);
+    norm[j] = cexp[(GLU ? tile + j * up : tile) * kTileN + 4 * a16 + (r & 3)];
+  }
 }
 
 // part j < NH: the packed words of part j; part NH: the scales and zero
@@ -176,6 +200,63 @@ __device__ __forceinline__ bf16x8 g2_deq(uint32_t w, float s, float c) {
   return __builtin_bit_cast(bf16x8, o);
 }
 
+// The two operand types of the tile.
+//  * G2Bf16: activations as they are, weights RNE((q - z) s) to bf16 (8 bits), the
+//    reference's arithmetic.
+//  * G2F16: weights to 11 bits, RNE((q - z) s 2^-e), e the exponent of their row's
+//    largest scale, and activation rows times a power of two that brings their largest
+//    value to 2^14 (k_half_rows); both exact in fp16 but for what lies 2^-28 below a
+//    row's largest. The sums take the exponents back in the epilogue. For gated
+//    products, whose factors each carry the weights' rounding: 0.0027 of the output's
+//    rms in bf16, 0.0017 (the output's own rounding) so.
+struct G2Bf16 {
+  static constexpr bool kNorm = false;
+  struct Scale {
+    float s, c;
+  };
+  __device__ static Scale scale(uint32_t s, uint32_t z, int) {
+    const float sf = bf16_bits_to_f32(s);
+    return {sf, -(float)z * sf};
+  }
+  __device__ static bf16x8 deq(uint32_t w, const Scale& k) { return g2_deq(w, k.s, k.c); }
+  __device__ static f32x16v mfma(bf16x8 a, u32x4 b, f32x16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+
+struct G2F16 {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  static constexpr bool kNorm = true;
+  struct Scale {
+    uint32_t s, z;   // pairs of s 2^-e and of -(1024 + z)
+  };
+  __device__ static Scale scale(uint32_t s, uint32_t z, int e) {
+    const _Float16 h = (_Float16)__builtin_ldexpf(bf16_bits_to_f32(s), -e);
+    return {__builtin_bit_cast(uint32_t, f16x2{h, h}), (z * 0x10001u) | 0xE400E400u};
+  }
+  // A nibble in the low mantissa bits of 1024 is 1024 + q; minus 1024 + z it is exact,
+  // and the product with the scale rounds once: 15 VALU per word.
+  __device__ static bf16x8 deq(uint32_t w, const Scale& k) {
+    const f16x2 s = __builtin_bit_cast(f16x2, k.s), z = __builtin_bit_cast(f16x2, k.z);
+    // both constants in registers, for one v_and_or_b32 a pair (see NibConst)
+    uint32_t mask, magic;
+    asm("v_mov_b32 %0, 0x000f000f" : "=v"(mask));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f16x2 q = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & mask) | magic);
+      o[i] = __builtin_bit_cast(uint32_t, (q + z) * s);
+    }
+    return __builtin_bit_cast(bf16x8, o);   // the bits; mfma takes them as fp16
+  }
+  __device__ static f32x16v mfma(bf16x8 a, u32x4 b, f32x16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b),
+                                                  c, 0, 0, 0);
+  }
+};
+
 // s_waitcnt vmcnt(0) (expcnt and lgkmcnt left at their maxima).
 __device__ __forceinline__ void g2_wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
@@ -191,8 +272,10 @@ __device__ __forceinline__ int g2_xcd_order(int blk, int count) {
 // nbuf and weights into nxt (actn, rsn: zero-length resources where there is no
 // such group -- they fetch nothing and need no branch, which would split the
 // k-step schedule).
-template <int NH, int NW, int MB, bool GLU, class Rows>
-__device__ __forceinline__ void g2_group(int G, f32x16v (&acc)[NH][G2Split<NH, NW, MB>::MBW],
+// norm: G2F16's exponents of the lane's weight rows.
+template <int NH, int NW, int MB, bool GLU, class Op, class Rows>
+__device__ __forceinline__ void g2_group(int G, const int (&norm)[NH],
+                                         f32x16v (&acc)[NH][G2Split<NH, NW, MB>::MBW],
                                          const WeightGroup<NH>& cur, WeightGroup<NH>& nxt,
                                          const u32x4* buf, u32x4* nbuf,
                                          __amdgpu_buffer_rsrc_t actn, const G2Rsrc& rsn,
@@ -209,12 +292,9 @@ __device__ __forceinline__ void g2_group(int G, f32x16v (&acc)[NH][G2Split<NH, N
   // step; 4 waves: all 8 steps, equal to steps 0-3); its weights in k-steps
   // kWStep.. kWStep + NH (0.5-0.8% faster than all at the group's start, where
   // they delay its first MFMA).
-  float sf[NH], cf[NH];
+  typename Op::Scale sc[NH];
 #pragma unroll
-  for (int j = 0; j < NH; ++j) {
-    sf[j] = bf16_bits_to_f32(cur.s[j]);
-    cf[j] = -(float)((cur.z[j] >> zsh) & 0xFu) * sf[j];
-  }
+  for (int j = 0; j < NH; ++j) sc[j] = Op::scale(cur.s[j], (cur.z[j] >> zsh) & 0xFu, norm[j]);
   // Software pipeline over the group's 8 k-steps: the activation operands
   // and the dequantized weight operands of step u + 1 are produced while
   // step u's MFMAs run.
@@ -223,7 +303,7 @@ __device__ __forceinline__ void g2_group(int G, f32x16v (&acc)[NH][G2Split<NH, N
 #pragma unroll
   for (int mb = 0; mb < MBW; ++mb) xo[0][mb] = buf[mb * 512 + ((4 * h) ^ (r & 15))];
 #pragma unroll
-  for (int j = 0; j < NH; ++j) wd[0][j] = g2_deq(cur.q[j][0][0], sf[j], cf[j]);
+  for (int j = 0; j < NH; ++j) wd[0][j] = Op::deq(cur.q[j][0][0], sc[j]);
   // Fence: the prologue's reads must not fill the DS slots of the pattern below.
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -243,14 +323,13 @@ __device__ __forceinline__ void g2_group(int G, f32x16v (&acc)[NH][G2Split<NH, N
 #pragma unroll
       for (int mb = 0; mb < MBW; ++mb) xo[nu][mb] = buf[mb * 512 + slot];
 #pragma unroll
-      for (int j = 0; j < NH; ++j) wd[nu][j] = g2_deq(cur.q[j][s1][t1], sf[j], cf[j]);
+      for (int j = 0; j < NH; ++j) wd[nu][j] = Op::deq(cur.q[j][s1][t1], sc[j]);
     }
 #pragma unroll
     for (int mb = 0; mb < MBW; ++mb)
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        acc[j][mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            wd[cu][j], __builtin_bit_cast(bf16x8, xo[cu][mb]), acc[j][mb], 0, 0, 0);
+        acc[j][mb] = Op::mfma(wd[cu][j], xo[cu][mb], acc[j][mb]);
     if (u + 1 < 8) {
 #pragma unroll
       for (int i = 0; i < MBW * NH; ++i) {
@@ -270,13 +349,13 @@ __device__ __forceinline__ void g2_group(int G, f32x16v (&acc)[NH][G2Split<NH, N
 // [g0, g1) of this wave's weight rows x the tile's activation rows, which `rows`
 // finds in `act`. rs_none, act_none: the same of no length, for the loads past the
 // last group.
-template <int NH, int NW, int MB, bool GLU, class Rows>
-__device__ __forceinline__ void g2_segment(int G, const G2Rsrc& rs, const G2Rsrc& rs_none,
+template <int NH, int NW, int MB, bool GLU, class Op, int DD, class Rows>
+__device__ __forceinline__ void g2_segment(int G, const int (&norm)[NH], const G2Rsrc& rs, const G2Rsrc& rs_none,
                                            __amdgpu_buffer_rsrc_t act,
                                            __amdgpu_buffer_rsrc_t act_none, const Rows& rows, u32x4 (*lds)[32 * MB * 16],
                                            f32x16v (&acc)[NH][G2Split<NH, NW, MB>::MBW], int ltile,
                                            int up, int b0, int mw, int g0, int g1, int wave, int lane) {
-  using Sp = G2Split<NH, NW, MB>;
+  using Sp = G2Split<NH, NW, MB, DD>;
   constexpr int MBW = Sp::MBW, D = Sp::DEPTH;
   const int r = lane & 31;
 #pragma unroll
@@ -294,7 +373,7 @@ __device__ __forceinline__ void g2_segment(int G, const G2Rsrc& rs, const G2Rsrc
       __syncthreads();
       const int sb = (g - g0) & 1;
       const bool more = g + 1 < g1;
-      g2_group<NH, NW, MB, GLU>(G, acc, cur, nxt, lds[sb] + (32 * mw + r) * 16, lds[sb ^ 1],
+      g2_group<NH, NW, MB, GLU, Op>(G, norm, acc, cur, nxt, lds[sb] + (32 * mw + r) * 16, lds[sb ^ 1],
                                 more ? act : act_none, more ? rs : rs_none, rows, ltile, up, b0,
                                 g + 1, wave, lane);
       cur = nxt;
@@ -325,7 +404,7 @@ __device__ __forceinline__ void g2_segment(int G, const G2Rsrc& rs, const G2Rsrc
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 2) * kLoads) : "memory");
         constexpr int kBack = D - 1;
         const bool more = g + kBack < g1;
-        g2_group<NH, NW, MB, GLU>(G, acc, wg[d], wg[(d + kBack) % D], lds[d] + (32 * mw + r) * 16,
+        g2_group<NH, NW, MB, GLU, Op>(G, norm, acc, wg[d], wg[(d + kBack) % D], lds[d] + (32 * mw + r) * 16,
                                   lds[(d + kBack) % D], more ? act : act_none, more ? rs : rs_none,
                                   rows, ltile, up, b0, g + kBack, wave, lane);
       }
@@ -339,12 +418,13 @@ __device__ __forceinline__ void g2_segment(int G, const G2Rsrc& rs, const G2Rsrc
 // at c ^ (row % 16)), and come back row by row, 8 output columns a lane, so that bias
 // and residual are added and the result rounded once, in whole 128-byte (gated: 64-byte)
 // segments of a row. out and e.res point to the tile's first row and the wave's first
-// column, e.bias to that column; `rows` rows are stored.
-template <int MB, bool GLU>
+// column, e.bias to that column; `rows` rows are stored. G2F16: rexp are the exponents
+// of the tile's rows, cexp those of the wave's columns (up columns e.up on).
+template <int MB, bool GLU, class Op, int DD>
 __device__ __forceinline__ void g2_store_epilogue(const f32x16v (&acc)[2][MB], u32x4* lds, uint16_t* out,
-                                                  const Epilogue& e, int ld, int rows, bool valid,
-                                                  int wave, int lane) {
-  constexpr int kPass = G2Split<2, 4, MB>::DEPTH * MB / 4;   // m-blocks of 8 KiB in a wave's share
+                                                  const Epilogue& e, const int* rexp, const int* cexp,
+                                                  int ld, int rows, bool valid, int wave, int lane) {
+  constexpr int kPass = G2Split<2, 4, MB, DD>::DEPTH * MB / 4;   // m-blocks of 8 KiB in a wave's share
   constexpr int kLanes = GLU ? 4 : 8;                        // lanes of a row, 8 columns each
   constexpr int kStep = 64 / kLanes;                         // rows of one instruction
   constexpr int kBatch = 32 / kStep;                         // residual loads in flight: an m-block's
@@ -354,6 +434,11 @@ __device__ __forceinline__ void g2_store_epilogue(const f32x16v (&acc)[2][MB], u
   u32x4* reg = lds + wave * (kPass * 512);
   float bias[GLU ? 2 : 1][8];
   if (valid) load_bias<GLU>(bias, e, 8 * cl);
+  int ce[GLU ? 2 : 1][8];
+#pragma unroll
+  for (int j = 0; j < (GLU ? 2 : 1); ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ce[j][i] = Op::kNorm && valid ? cexp[j * e.up + 8 * cl + i] : 0;
 #pragma unroll
   for (int p0 = 0; p0 < MB; p0 += kPass) {
     const int blocks = p0 + kPass <= MB ? kPass : MB - p0;
@@ -376,10 +461,12 @@ __device__ __forceinline__ void g2_store_epilogue(const f32x16v (&acc)[2][MB], u
     if (valid) {
       for (int t0 = 0; t0 < 32 * blocks; t0 += kBatch * kStep) {
         u32x4 res[kBatch];
+        int re[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const int m = 32 * p0 + t0 + i * kStep + rl;
           res[i] = u32x4{0u, 0u, 0u, 0u};
+          re[i] = Op::kNorm && m < rows ? rexp[m] : 0;
           if (e.res && m < rows) res[i] = *reinterpret_cast<const u32x4*>(e.res + (size_t)m * ld + 8 * cl);
         }
 #pragma unroll
@@ -392,7 +479,11 @@ __device__ __forceinline__ void g2_store_epilogue(const f32x16v (&acc)[2][MB], u
             for (int c = 0; c < 2; ++c) {
               const u32x4 w = reg[row * 16 + ((8 * j + 2 * cl + c) ^ (row & 15))];
 #pragma unroll
-              for (int i2 = 0; i2 < 4; ++i2) v[j][4 * c + i2] = __uint_as_float(w[i2]) + bias[j][4 * c + i2];
+              for (int i2 = 0; i2 < 4; ++i2) {
+                float f = __uint_as_float(w[i2]);
+                if (Op::kNorm) f = __builtin_ldexpf(f, re[i] + ce[j][4 * c + i2]);
+                v[j][4 * c + i2] = f + bias[j][4 * c + i2];
+              }
             }
           epilogue_act<GLU>(v, e.act);
           if (m < rows) *reinterpret_cast<u32x4*>(out + (size_t)m * ld + 8 * cl) = add_round8(v[0], res[i]);

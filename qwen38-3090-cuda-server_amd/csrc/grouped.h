@@ -24,6 +24,7 @@ struct GroupedArgs {
   uint32_t x_bytes;         // of a gathered x
   int ld;                   // columns of y
   int tiles_n, P;           // column tiles of an expert, workgroups
+  const int *rexp, *cexp;   // fp16 operands: exponents of x's rows and of the weight rows
 };
 
 // Expert e's positions. Offsets that are no plan's (negative, falling, past R) give
@@ -33,50 +34,64 @@ __device__ __forceinline__ void expert_rows(const GroupedArgs& a, int e, int& lo
   hi = min(max(a.offsets[e + 1], lo), a.R);
 }
 
-// Blocks of ROWS positions: start[e] = those of the experts before e, returned: all.
-// For a workgroup of THREADS, start [kMaxExperts + 1] and wsum [THREADS / 64] in LDS.
-template <int ROWS, int THREADS>
-__device__ __forceinline__ int block_starts(const GroupedArgs& a, int* start, int* wsum) {
+// Running sums over the experts of N counts each, count(rows, which): start[which
+// (kMaxExperts + 1) + e] = those of the experts before e, all[which] = the total. For a
+// workgroup of THREADS; wsum [THREADS / 64 N].
+template <int THREADS, int N, class Count>
+__device__ __forceinline__ void expert_starts(const GroupedArgs& a, int* start, int* wsum, int (&all)[N],
+                                              const Count& count) {
   constexpr int kPer = kMaxExperts / THREADS;   // experts of a thread
+  constexpr int kWaves = THREADS / 64;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  int n[kPer], sum = 0;
+  int n[N][kPer], run[N];
+#pragma unroll
+  for (int w = 0; w < N; ++w) run[w] = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = kPer * t + i;
-    n[i] = 0;
-    if (e < a.E) {
-      int lo, hi;
-      expert_rows(a, e, lo, hi);
-      n[i] = (hi - lo + ROWS - 1) / ROWS;
+    int lo = 0, hi = 0;
+    if (e < a.E) expert_rows(a, e, lo, hi);
+#pragma unroll
+    for (int w = 0; w < N; ++w) {
+      n[w][i] = count(hi - lo, w);
+      run[w] += n[w][i];
     }
-    sum += n[i];
   }
-  int run = sum;
+  int before[N];
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int v = __shfl_up(run, off, 64);
-    if (lane >= off) run += v;
+  for (int w = 0; w < N; ++w) {
+    before[w] = -run[w];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(run[w], off, 64);
+      if (lane >= off) run[w] += v;
+    }
+    before[w] += run[w];
+    if (lane == 63) wsum[w * kWaves + wave] = run[w];
   }
-  if (lane == 63) wsum[wave] = run;
   __syncthreads();
-  int before = run - sum, all = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    before += w < wave ? wsum[w] : 0;
-    all += wsum[w];
-  }
+  for (int w = 0; w < N; ++w) {
+    int sum = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (kPer * t + i <= a.E) start[kPer * t + i] = before;
-    before += n[i];
+    for (int i = 0; i < kWaves; ++i) {
+      before[w] += i < wave ? wsum[w * kWaves + i] : 0;
+      sum += wsum[w * kWaves + i];
+    }
+    all[w] = __builtin_amdgcn_readfirstlane(sum);
+    int* const s = start + w * (kMaxExperts + 1);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      s[kPer * t + i] = before[w];
+      before[w] += n[w][i];
+    }
+    if (t == THREADS - 1) s[kMaxExperts] = before[w];
   }
-  if (t == THREADS - 1 && a.E == kMaxExperts) start[kMaxExperts] = before;
   __syncthreads();
-  return all;
 }
 
-// The last expert whose first tile is at or before t (experts without rows start where
-// the next one does, so it has rows).
+// The last expert whose first tile is at or before t (experts without tiles start where
+// the next one does, so it has some).
 __device__ __forceinline__ int expert_of(const int* start, int E, int tiles_n, int t) {
   int lo = 0, hi = E;   // start[lo] tiles_n <= t < start[hi] tiles_n
   while (hi - lo > 1) {

@@ -19,34 +19,79 @@ int check_weights_public(const qw4_weights* w);
 namespace {
 
 // Many rows an expert: the MFMA tile of the prefill GEMM (gemm_tile.h) over (expert, row
-// block, column tile). Tiles go expert by expert, a column tile's row blocks together,
-// and an XCD takes a run of them: its weights and rows stay in its L2. Every workgroup
-// takes every P-th tile.
-template <int MB, bool GLU, bool GATHER>
-__global__ __launch_bounds__(256, 1) void k_grouped_tiles(GroupedArgs a) {
-  using Sp = G2Split<2, 4, MB>;
-  __shared__ u32x4 lds[Sp::DEPTH][32 * MB * 16];
-  __shared__ int start[kMaxExperts + 1];
-  __shared__ int wsum[4];
+// block, column tile). First the tiles of whole row blocks, expert by expert in bands of
+// four blocks (a column tile's four together), then those of the blocks that experts end
+// with, which compute a half or a quarter of the tile where that covers their rows, the
+// shorter ones last. Rounds of P tiles go over the workgroups back and forth, so that
+// who had a long one gets a short one; an XCD takes a run of a round, so that weights
+// and rows stay in its L2.
+//
+// LDS for groups of M m-blocks: 8 M KiB each, up to four.
+template <int MB, int DD>
+constexpr int tile_depth(int m) {
+  return MB * DD / m < 4 ? MB * DD / m : 4;
+}
+
+// Heights of an ending block: the whole tile, a half, at MB = 8 also a quarter.
+template <int MB>
+constexpr int tile_ends() {
+  return MB >= 8 ? 3 : 2;
+}
+
+template <int MB, int DD, int OCC, bool GLU, bool GATHER, class Op>
+__global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
+  // One LDS object for everything: of several, the compiler tells their accesses apart
+  // and waits for all loads into one before it reads the next (vmcnt(0) at every k-step;
+  // 32768 rows of 64 experts, 2048 x 2048: 339 us).
+  constexpr int kBufs = DD * 32 * MB * 16, kRows = GATHER ? 32 * MB : 0;
+  constexpr int kEnds = tile_ends<MB>(), kLists = 1 + kEnds;
+  __shared__ u32x4 lds[kBufs + (4 * kRows + kLists * (kMaxExperts + 1 + 4) + 3) / 4];
+  // gathered rows: x's row and its exponent at each of the tile's positions, in turns:
+  // a buffer is filled again a barrier after every wave is done with it
+  int* const from = reinterpret_cast<int*>(lds + kBufs);
+  int* const rexp = from + 2 * kRows;
+  int* const start = rexp + 2 * kRows;
+  int* const wsum = start + kLists * (kMaxExperts + 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int all = __builtin_amdgcn_readfirstlane(block_starts<32 * MB, 256>(a, start, wsum)) * a.tiles_n;
+  int blocks[kLists];   // whole, and ending by height
+  expert_starts<256>(a, start, wsum, blocks, [](int rows, int which) {
+    const int end = rows % (32 * MB);
+    // height 32 MB >> (which - 1): above the next lower one, if there is one
+    const int high = 32 * MB >> (which - 1), low = which == kEnds ? 0 : high >> 1;
+    return which == 0 ? rows / (32 * MB) : (int)(end > low && end <= high);
+  });
+  int all = 0;
+#pragma unroll
+  for (int l = 0; l < kLists; ++l) all += blocks[l] * a.tiles_n;
   const uint32_t row_bytes = (uint32_t)a.K * 2u;
   const int srow = 4 * wave + (lane >> 4);   // row within the 16-row swizzle period
   const uint32_t chunk = (uint32_t)((lane & 15) ^ srow) * 16u;
   const int up = a.epi.up / kTileN;
   const int width = GLU ? a.ld : a.n;   // columns the column tiles run over
-  f32x16v acc[2][MB];
-  for (int t = a.P % 8 ? (int)blockIdx.x : (int)((blockIdx.x & 7) * (a.P >> 3) + (blockIdx.x >> 3)); t < all;
-       t += a.P) {
-    const int e = expert_of(start, a.E, a.tiles_n, t);
+  int turn = 0;
+  const int vp = a.P % 8 ? (int)blockIdx.x : (int)((blockIdx.x & 7) * (a.P >> 3) + (blockIdx.x >> 3));
+  for (int base = 0, round = 0; base < all; base += a.P, ++round) {
+    int t = base + (round & 1 ? a.P - 1 - vp : vp);
+    if (t >= all) continue;
+    int list = 0;
+    while (list + 1 < kLists && t >= blocks[list] * a.tiles_n) t -= blocks[list++] * a.tiles_n;
+    const int* const first = start + list * (kMaxExperts + 1);
+    const int e = expert_of(first, a.E, a.tiles_n, t);
     int lo, hi;
     expert_rows(a, e, lo, hi);
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    const int blocks = max(1, (hi - lo + 32 * MB - 1) / (32 * MB));
-    const int at = t - __builtin_amdgcn_readfirstlane(start[e]) * a.tiles_n;
-    if ((uint32_t)at >= (uint32_t)(blocks * a.tiles_n)) continue;   // offsets of no plan
-    const int tn = at / blocks, m0 = lo + (at - tn * blocks) * 32 * MB;
+    const int n_whole = (hi - lo) / (32 * MB);
+    const int at = t - __builtin_amdgcn_readfirstlane(first[e]) * a.tiles_n;
+    if ((uint32_t)at >= (uint32_t)((list ? 1 : n_whole) * a.tiles_n)) continue;   // offsets of no plan
+    int tn = at, block = n_whole;
+    if (list == 0) {
+      const int band = at / (4 * a.tiles_n), in_band = at - band * 4 * a.tiles_n;
+      const int high = min(4, n_whole - 4 * band);
+      tn = in_band / high;
+      block = 4 * band + in_band - tn * high;
+    }
+    const int m0 = lo + block * 32 * MB;
     const int rows = hi - m0;
     // a wave's weight tile, half and first output column, as the dense product's
     const int wt = GLU ? tn * 2 + (wave >> 1) : tn * 4 + wave;
@@ -58,27 +103,51 @@ __global__ __launch_bounds__(256, 1) void k_grouped_tiles(GroupedArgs a) {
     const G2Rsrc wr = g2_weights(a.qw + blk * kWordsPerBlock, a.sc + blk * kMetaU16, a.zr + blk * 16, a.n, a.G);
     const G2Rsrc none =
         g2_weights(a.qw + blk * kWordsPerBlock, a.sc + blk * kMetaU16, a.zr + blk * 16, a.n, a.G, false);
+    const int* cexp = Op::kNorm ? a.cexp + (size_t)e * a.n : nullptr;
+    int norm[2] = {};
+    if constexpr (Op::kNorm) g2_load_norms<2, GLU>(norm, cexp, ltile, up, b0, lane);
+    turn ^= 1;
     if constexpr (GATHER) {
-      G2Gather<Sp::ACT> from;
-#pragma unroll
-      for (int i = 0; i < Sp::ACT; ++i) {
-        const int r = 4 * (4 * i + wave) + (lane >> 4);
+      for (int r = threadIdx.x; r < 32 * MB; r += 256) {
         const int row = r < rows ? a.tokens[m0 + r] : -1;
-        const uint64_t off = (uint64_t)(uint32_t)row * row_bytes;   // past x: reads as zeros
-        from.off[i] = off < a.x_bytes ? (uint32_t)off + chunk : a.x_bytes;
+        from[turn * kRows + r] = row;
+        if (Op::kNorm) rexp[turn * kRows + r] = (uint64_t)(uint32_t)row * row_bytes < a.x_bytes ? a.rexp[row] : 0;
       }
-      g2_segment<2, 4, MB, GLU>(a.G, wr, none, g2_rsrc(a.x, a.x_bytes), g2_rsrc(a.x, 0), from, lds, acc,
-                                ltile, up, b0, 0, 0, a.G, wave, lane);
-    } else {
-      const uint16_t* x0 = a.x + (size_t)m0 * a.K;
-      const G2Rows from{(uint32_t)(lane >> 4) * row_bytes + chunk, row_bytes};
-      g2_segment<2, 4, MB, GLU>(a.G, wr, none, g2_rsrc(x0, (uint32_t)min(rows, 32 * MB) * row_bytes),
-                                g2_rsrc(x0, 0), from, lds, acc, ltile, up, b0, 0, 0, a.G, wave, lane);
+      __syncthreads();
     }
     Epilogue ep = a.epi;
     if (ep.bias) ep.bias += (size_t)e * a.n + col;
-    g2_store_epilogue<MB, GLU>(acc, &lds[0][0], a.y + (size_t)m0 * a.ld + col, ep, a.ld, rows, valid, wave,
-                               lane);
+    auto tile = [&](auto mc) __attribute__((always_inline)) {
+      constexpr int M = decltype(mc)::value, D = tile_depth<MB, DD>(M);
+      constexpr int kAct = G2Split<2, 4, M, D>::ACT;
+      f32x16v acc[2][M];
+      auto* const buf = reinterpret_cast<u32x4(*)[32 * M * 16]>(lds);
+      if constexpr (GATHER) {
+        G2Gather<kAct> g;
+#pragma unroll
+        for (int i = 0; i < kAct; ++i) {
+          // past the block, or past x: reads as zeros
+          const uint64_t off = (uint64_t)(uint32_t)from[turn * kRows + 4 * (4 * i + wave) + (lane >> 4)] * row_bytes;
+          g.off[i] = off < a.x_bytes ? (uint32_t)off + chunk : a.x_bytes;
+        }
+        g2_segment<2, 4, M, GLU, Op, D>(a.G, norm, wr, none, g2_rsrc(a.x, a.x_bytes), g2_rsrc(a.x, 0), g, buf,
+                                        acc, ltile, up, b0, 0, 0, a.G, wave, lane);
+      } else {
+        const uint16_t* x0 = a.x + (size_t)m0 * a.K;
+        const G2Rows g{(uint32_t)(lane >> 4) * row_bytes + chunk, row_bytes};
+        g2_segment<2, 4, M, GLU, Op, D>(a.G, norm, wr, none, g2_rsrc(x0, (uint32_t)min(rows, 32 * M) * row_bytes),
+                                        g2_rsrc(x0, 0), g, buf, acc, ltile, up, b0, 0, 0, a.G, wave, lane);
+      }
+      const int* re = !Op::kNorm ? nullptr : GATHER ? rexp + turn * kRows : a.rexp + m0;
+      g2_store_epilogue<M, GLU, Op, D>(acc, lds, a.y + (size_t)m0 * a.ld + col, ep, re, cexp + col, a.ld, rows,
+                                       valid, wave, lane);
+    };
+    if (list <= 1)
+      tile(std::integral_constant<int, MB>{});
+    else if (kEnds == 2 || list == 2)
+      tile(std::integral_constant<int, MB / 2>{});
+    else
+      tile(std::integral_constant<int, MB / (kEnds == 3 ? 4 : 2)>{});
   }
 }
 
@@ -96,14 +165,10 @@ int device_cus() {
   return n;
 }
 
-template <int MB>
-void launch_tiles(const GroupedArgs& a, bool glu, hipStream_t s) {
-  if (glu)
-    a.tokens ? k_grouped_tiles<MB, true, true><<<a.P, 256, 0, s>>>(a)
-             : k_grouped_tiles<MB, true, false><<<a.P, 256, 0, s>>>(a);
-  else
-    a.tokens ? k_grouped_tiles<MB, false, true><<<a.P, 256, 0, s>>>(a)
-             : k_grouped_tiles<MB, false, false><<<a.P, 256, 0, s>>>(a);
+template <int MB, int DD, int OCC, bool GLU, class Op>
+void launch_tiles(const GroupedArgs& a, hipStream_t s) {
+  a.tokens ? k_grouped_tiles<MB, DD, OCC, GLU, true, Op><<<a.P, 256, 0, s>>>(a)
+           : k_grouped_tiles<MB, DD, OCC, GLU, false, Op><<<a.P, 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -116,7 +181,6 @@ extern "C" {
 int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x_rows,
                      const qw4_plan* plan, int pairs, int gather, const uint16_t* bias, int act,
                      qw4_workspace* ws, void* stream) {
-  (void)ws;
   const int st = check_weights_public(w);
   if (st) return st;
   if (!plan || !plan->offsets) return QW4_ERR_NULL;
@@ -127,12 +191,12 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   if (n % (glu ? 2 * kTileN : kTileN)) return QW4_ERR_SHAPE;
   if (pairs < 0) return QW4_ERR_M;
   if (pairs > plan->max_pairs) return QW4_ERR_SCRATCH;
-  if (x_rows < 0 || (!gather && x_rows < pairs)) return QW4_ERR_SHAPE;
+  if (pairs > 0 && x_rows < (gather ? 1 : pairs)) return QW4_ERR_SHAPE;
   // an expert's weights, and a gathered x, through 32-bit buffer offsets
   const size_t row = (size_t)w->in_f * 2;
-  if ((size_t)n * w->in_f / 2 >= (1ull << 32) || (gather && (size_t)x_rows * row >= (1ull << 32) - row))
+  if ((size_t)n * w->in_f / 2 >= (1ull << 32) || (gather && pairs > 0 && (size_t)x_rows * row >= (1ull << 32) - row))
     return QW4_ERR_SHAPE;
-  if (pairs == 0 || x_rows == 0) return QW4_OK;
+  if (pairs == 0) return QW4_OK;
   if (!y || !x || (gather && !plan->tokens)) return QW4_ERR_NULL;
   if (((uintptr_t)y | (uintptr_t)x | (uintptr_t)bias) & 15) return QW4_ERR_ALIGN;
   GroupedArgs a{};
@@ -157,11 +221,33 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
-  constexpr int mb = 4;
+  const int x_used = gather ? x_rows : pairs;
+  if (glu && ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && ws->bytes >= half_rows_bytes(x_used, w)) {
+    const HalfRows h = half_rows(ws->buf, x, x_used, w, (hipStream_t)stream);
+    a.x = h.x;
+    a.rexp = h.rexp;
+    a.cexp = h.cexp;
+  }
+  // 128-row tiles, two workgroups a CU, one's start and end behind the other's products;
+  // or 256-row tiles, one a CU, which cost less a row but waste more where an expert ends
+  // and hide nothing. us (128 / 256): ungated, 16 experts of 768 / 1024 rows in the mean,
+  // skewed, 2048x2048 129 / 125, 159 / 150; 64 of 512, skewed, 2048x1024 159 / 162, even,
+  // 2048x4096 502 / 456; gated, whose epilogue is longer, 64 of 512 even 278 / 297, 16 of
+  // 1536 skewed 241 / 267.
+  const int mb = !glu && (long long)pairs >= 640LL * a.E ? 8 : 4;
+  const int occ = mb == 8 ? 1 : 2;
   const long long most = ((long long)pairs / (32 * mb) + std::min(a.E, pairs)) * a.tiles_n;
-  if (most > 0x7fffffffLL) return QW4_ERR_SHAPE;
-  a.P = (int)std::min<long long>(most, cus);
-  launch_tiles<mb>(a, glu, (hipStream_t)stream);
+  if (most > 0x3fffffffLL) return QW4_ERR_SHAPE;
+  a.P = (int)std::min<long long>(most, cus * occ);
+  hipStream_t s = (hipStream_t)stream;
+  if (mb == 8)
+    launch_tiles<8, 2, 1, false, G2Bf16>(a, s);
+  else if (!glu)
+    launch_tiles<4, 2, 2, false, G2Bf16>(a, s);
+  else if (a.cexp)
+    launch_tiles<4, 2, 2, true, G2F16>(a, s);
+  else
+    launch_tiles<4, 2, 2, true, G2Bf16>(a, s);
   QW4_LAUNCH_CHECK();
   return QW4_OK;
 }

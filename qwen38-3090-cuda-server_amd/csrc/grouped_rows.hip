@@ -34,17 +34,22 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
   constexpr int kL = L::kLoads;
   constexpr uint32_t kPer = 4 / S;
   constexpr int kArea = 2 * MB * S * 64;   // a wave's sums of a unit, two buffers
-  __shared__ f32x4 red[kW][kArea];
-  __shared__ f32x4 csum[MB == 1 ? 1 : kW][NG][MB][4];   // MB > 1: the row sums (no registers left)
-  __shared__ int start[kMaxExperts + 1];
-  __shared__ int wsum[kW];
-  __shared__ u32x4 slots[kW * D * L::kUnits];
+  constexpr int kSums = MB == 1 ? 0 : NG * MB * 4;   // MB > 1: a wave's row sums (no registers left)
+  // One LDS object: of several the compiler tells the accesses apart and waits for every
+  // load into the slots before it reads the sums (vmcnt(0) in place of the counted waits).
+  __shared__ u32x4 lds[kW * (D * L::kUnits + kArea + kSums) + (kMaxExperts + 1 + kW + 3) / 4];
+  u32x4* const slots = lds;
+  f32x4* const red = reinterpret_cast<f32x4*>(slots + kW * D * L::kUnits);
+  f32x4* const csum = red + kW * kArea;
+  int* const start = reinterpret_cast<int*>(csum + kW * kSums);
+  int* const wsum = start + kMaxExperts + 1;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, q = lane >> 4;
-  const int all = __builtin_amdgcn_readfirstlane(block_starts<16 * MB, 64 * kW>(a, start, wsum));
+  int all[1];
+  expert_starts<64 * kW>(a, start, wsum, all, [](int rows, int) { return (rows + 16 * MB - 1) / (16 * MB); });
   // units of a block (gated: pairs), and this workgroup's run of them
   const int per = (GLU ? a.ld : a.n) / (16 * S);
-  const long long total = (long long)all * per;
+  const long long total = (long long)all[0] * per;
   const int p = blockIdx.x;
   const long long u0 = p * total / a.P, u1 = (p + 1) * total / a.P;
   int left_units = (int)(u1 - u0);
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
         if (MB == 1)
           Cs[MB == 1 ? i : 0] = cs;
         else if (c == 0)   // the same for all 16 columns; read by this wave alone
-          csum[MB == 1 ? 0 : wave][i][mb][q] = cs;
+          csum[wave * kSums + (i * MB + mb) * 4 + q] = cs;
       }
   };
   load_x();
@@ -209,7 +214,7 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
           }
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const f32x4 cs = MB == 1 ? Cs[MB == 1 ? gi : 0] : csum[MB == 1 ? 0 : wave][gi][mb][q];
+          const f32x4 cs = MB == 1 ? Cs[MB == 1 ? gi : 0] : csum[wave * kSums + (gi * MB + mb) * 4 + q];
 #pragma unroll
           for (int i = 0; i < S; ++i) {
             const uint32_t sbits = (d.s[i >> 1] >> (16 * (S == 1 ? (st0 & 1) : (i & 1)))) & 0xffffu;
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-          red[wave][((par * MB + mb) * S + i) * 64 + lane] = acc[mb][i];
+          red[wave * kArea + ((par * MB + mb) * S + i) * 64 + lane] = acc[mb][i];
           acc[mb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
       lds_barrier<true>();
@@ -244,9 +249,9 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
           const int from = (((par * MB + mb) * S + i) * 64 + lane) * 4 + jj;
-          v[i] = reinterpret_cast<const float*>(red[0])[from];
+          v[i] = reinterpret_cast<const float*>(red)[from];
 #pragma unroll
-          for (int w = 1; w < kW; ++w) v[i] += reinterpret_cast<const float*>(red[w])[from];
+          for (int w = 1; w < kW; ++w) v[i] += reinterpret_cast<const float*>(red + w * kArea)[from];
         }
         if (GLU && half == 0) {
 #pragma unroll

@@ -55,6 +55,7 @@ EXPORTS = (
     "qw4_tune_gemm", "qw4_tune_linear", "qw4_gemv_argmax_noalloc",
     "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
     "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue", "qw4_gemm_grouped",
+    "qw4_epilogue_workspace",
 )
 
 # safetensors dtype order (qw4_st_tensor.dtype)
@@ -197,6 +198,7 @@ def lib():
         "qw4_route_f32": ([vp, vp, PL, vp, i, i, i, i, vp], i),
         "qw4_route_ids": ([PL, vp, i, i, vp], i),
         "qw4_linear_epilogue": ([vp, W, vp, i, vp, i, vp, S, WS, vp], i),
+        "qw4_epilogue_workspace": ([W, i], sz),
         "qw4_gemm_grouped": ([vp, W, vp, i, PL, i, i, vp, i, WS, vp], i),
         "qw4_combine": ([vp, vp, PL, vp, i, i, i, vp, vp], i),
     }
@@ -467,6 +469,11 @@ def linear_epilogue_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch | None =
                                    C.byref(s) if s is not None else None,
                                    C.byref(ws) if ws is not None else None, _stream(stream)),
          "linear_epilogue")
+
+
+def epilogue_workspace(w: W4A16Weights, rows: int) -> int:
+    """qw4_epilogue_workspace: workspace bytes of a gated product over `rows` rows of x."""
+    return lib().qw4_epilogue_workspace(C.byref(w), rows)
 
 
 def tune_decode(mode: int = 0, S: int = 0, W: int = 0, D: int = 0, P: int = 0) -> None:

@@ -135,6 +135,7 @@ def test_gemm_grouped_refusals(hip):
     assert call(pairs=-1) == hip.QW4_ERR_M
     assert call(pairs=65, x_rows=65) == hip.QW4_ERR_SCRATCH
     assert call(x_rows=15) == hip.QW4_ERR_SHAPE                       # in order: a row for each position
+    assert call(gather=1, x_rows=0) == hip.QW4_ERR_SHAPE
     assert call(act=7) == hip.QW4_ERR_ACT
     assert call(act=hip.ACT_SWIGLU, w=_weights(hip, out_f=512)) == hip.QW4_ERR_SHAPE   # 64 rows an expert
     assert call(plan=_plan(hip, experts=7)) == hip.QW4_ERR_SHAPE      # 1024 rows are no 7 experts
@@ -149,3 +150,12 @@ def test_gemm_grouped_refusals(hip):
     for name in ("y", "x", "b"):
         assert call(**{name: 0x40008}) == hip.QW4_ERR_ALIGN
     assert call(pairs=0, y=None, x=None) == hip.QW4_OK
+
+
+def test_epilogue_workspace(hip):
+    w = _weights(hip, out_f=256, in_f=512)
+    # x in 16 bits, an exponent a row and a weight row, each from a multiple of 256 bytes
+    assert hip.epilogue_workspace(w, 100) == 100 * 512 * 2 + 512 + 1024
+    assert hip.epilogue_workspace(w, 0) == 1024
+    assert hip.epilogue_workspace(w, -1) == 0
+    assert hip.lib().qw4_epilogue_workspace(None, 4) == 0

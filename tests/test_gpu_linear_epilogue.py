@@ -47,10 +47,10 @@ def activation(v, act):
     return g * torch.sigmoid(g) * u
 
 
-def check(y, x, wq, bias, act, residual, rows, rounded):
+def check(y, x, wq, bias, act, residual, rows, rounded, bits=8):
     """y[rows] against the formula. Errors: the product's (fp32 sums: K 2^-24 of the
-    terms' absolute sum at most; weights rounded to bf16: 2^-8 of each term, which over
-    K random terms stays below 2^-8 sqrt(sum of squares) x 6), through the activation
+    terms' absolute sum at most; weights rounded to `bits` bits: 2^-bits of each term, which
+    over K random terms stays below 2^-bits sqrt(sum of squares) x 6), through the activation
     (|f'| <= 1.13 for the smooth ones; swiglu: each factor's error times the other), f's
     own few ulp, and the rounding to bf16 (half a step: 2^-8)."""
     import torch
@@ -60,7 +60,7 @@ def check(y, x, wq, bias, act, residual, rows, rounded):
     sumabs = xf.abs() @ wq.abs().t()
     ev = 2.0 ** -24 * (wq.shape[1] ** 0.5 + 8) * sumabs
     if rounded:
-        ev = ev + 6 * 2.0 ** -8 * ((xf ** 2) @ (wq ** 2).t()).sqrt()
+        ev = ev + 6 * 2.0 ** -bits * ((xf ** 2) @ (wq ** 2).t()).sqrt()
     if bias is not None:
         v = v + bias.double()
         ev = ev + 2.0 ** -24 * v.abs()
@@ -133,7 +133,9 @@ def test_epilogue(hip, orc, ws, N, K, act):
                           f"ws={space is not None}", flush=True)
                     y = run(hip, w, x, T, s, space, b, act, r, alias=residual and bias)
                     small = s is not None and T <= hip.linear_max_t(w)
-                    check(y, x, wq, b, act, r, rows, rounded=not small)
+                    # a gated product with a workspace has fp16 operands
+                    bits = 11 if act == "swiglu" and space is not None else 8
+                    check(y, x, wq, b, act, r, rows, rounded=not small, bits=bits)
     hip.awq_free(w)
     hip.gemv_scratch_free(scratch)
 
@@ -150,7 +152,9 @@ HEIGHTS = [(60, 33280, 384), (70, 33280, 384), (98, 33280, 384), (133, 33280, 38
 def test_epilogue_tiles(hip, orc, ws, T, N, K):
     """The plain product of the same call (qw4_gemm), through the epilogue's formula:
     both sum in the same order, so without bias, activation or residual they are equal
-    bit for bit, and gated they are the product's halves up to its rounding."""
+    bit for bit, and gated -- fp16 operands -- they are the product's halves up to its
+    rounding and that of its bf16 weights: 2^-8 of each term, over K random terms below 6
+    times 2^-8 of the root of their squares' sum."""
     import torch
 
     G = K // 128
@@ -181,9 +185,58 @@ def test_epilogue_tiles(hip, orc, ws, T, N, K):
     f = v * torch.sigmoid(v) + p
     tol = 1.13 * ep + 2.0 ** -8 * (f.abs() + 2 * ep) + 1e-6
     assert ((full.double() - f).abs() <= tol).all()
+    wd = torch.empty(N, K, dtype=torch.bfloat16, device="cuda")
+    hip.w4a16_dequant_rows(wd, w, 0, N)
+    wd = wd.float() ** 2
+    ep = ep + 6 * 2.0 ** -8 * (x.float() ** 2 @ wd.t()).sqrt().double()
     (a, u), (ea, eu) = v.chunk(2, dim=1), ep.chunk(2, dim=1)
     sa = a * torch.sigmoid(a)
     f = sa * u + half.double()
     e = 1.13 * ea * (u.abs() + eu) + sa.abs() * eu
     assert ((glu.double() - f).abs() <= e + 2.0 ** -8 * (f.abs() + e) + 1e-6).all()
+    hip.awq_free(w)
+
+
+@pytest.mark.parametrize("T", [130, 1000])
+def test_gated_range(hip, orc, ws, T):
+    """The fp16 operands of a gated product over bf16's range: rows and weight rows of
+    very large and very small values, a scale far above the others of its row, rows of
+    zeros; rows with Inf or NaN are NaN or Inf at every output and leave the others alone."""
+    import torch
+
+    I, K = 320, 1024
+    N = 2 * I
+    q, zp, s = orc.gen_weights(N, K, seed=T)
+    sf = (s.astype(np.uint32) << 16).view(np.float32).copy()
+    g = torch.Generator().manual_seed(T)
+    # gate rows keep their size (silu would saturate), up rows spread over 2^-90 .. 2^60
+    sf[I:] *= 2.0 ** np.random.default_rng(T).integers(-90, 60, (I, 1))
+    sf[I::7, 3] *= 2.0 ** 20
+    s = (sf.view(np.uint32) >> 16).astype(np.uint16)
+    w = repack_from_logical(hip, orc, q, zp, s, "ct")
+    sd = (s.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    wq = torch.from_numpy((q.astype(np.float64) - np.repeat(zp, 128, axis=1)) * np.repeat(sd, 128, axis=1))
+    x = torch.randn(T, K, generator=g) * (8.0 / K ** 0.5)
+    x[1::9] *= 2.0 ** -60
+    x[2::9] = 0
+    x[3::9, ::2] *= 2.0 ** -30
+    x[4::9, 5] = 2.0 ** 10
+    x = bf(x)
+    bad = x.clone()
+    bad[7, 3], bad[60, 9], bad[61, 0] = float("inf"), float("nan"), -float("inf")
+    for xi in (x, bad):
+        print(f"gated range T={T}", flush=True)
+        y = torch.full((T + 2, I), 7.0, dtype=torch.bfloat16, device="cuda")
+        hip.linear_epilogue_w4a16(y[1:T + 1], w, xi.cuda(), T, None, ws, act=hip.ACT_SWIGLU)
+        torch.cuda.synchronize()
+        assert (y[0] == 7.0).all() and (y[T + 1] == 7.0).all()
+        got = y[1:T + 1].cpu()
+        if xi is bad:
+            hit = torch.zeros(T, dtype=torch.bool)
+            hit[[7, 60, 61]] = True
+            assert not torch.isfinite(got[60]).any()
+            assert torch.equal(got[~hit], clean[~hit])
+        else:
+            clean = got
+            check(got, x, wq, None, "swiglu", None, list(range(0, T, 3)) + [1, 2, 4, T - 1], rounded=True, bits=11)
     hip.awq_free(w)
