@@ -422,8 +422,8 @@ int qw4_route_ids(const qw4_plan* plan, const int32_t* ids, int T, int top_k, vo
  * >= pairs). w holds the experts' weights one after the other (awq_repack_into at row
  * offset e n): out_f = experts n, n % 64 == 0 (QW4_ACT_SWIGLU: n % 128, each expert
  * [gate | up]); width = n, or n / 2. bias [out_f] bf16 may be NULL. fp32 up to the one
- * rounding. Weights are exact where experts have few rows (pairs / experts at most 32,
- * in_f at most 8192); beyond, they are rounded to bf16, or, in a gated product with a
+ * rounding. Weights are exact where experts have few rows (pairs / experts up to about
+ * 40, in_f up to 8192); beyond, they are rounded to bf16, or, in a gated product with a
  * 256-byte aligned workspace of qw4_epilogue_workspace(w, rows of x) bytes, to 11 bits.
  * Calls that share a workspace must be stream-ordered. pairs = the T
  * top_k the plan was made for: rows behind offsets[experts] are left as they were,

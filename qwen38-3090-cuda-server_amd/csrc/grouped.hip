@@ -71,7 +71,8 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
   int turn = 0;
   const int vp = a.P % 8 ? (int)blockIdx.x : (int)((blockIdx.x & 7) * (a.P >> 3) + (blockIdx.x >> 3));
   for (int base = 0, round = 0; base < all; base += a.P, ++round) {
-    int t = base + (round & 1 ? a.P - 1 - vp : vp);
+    // the last round in launch order: its tiles spread over the XCDs and CUs
+    int t = base + (base + a.P > all ? (int)blockIdx.x : round & 1 ? a.P - 1 - vp : vp);
     if (t >= all) continue;
     int list = 0;
     while (list + 1 < kLists && t >= blocks[list] * a.tiles_n) t -= blocks[list++] * a.tiles_n;

@@ -3,14 +3,17 @@
 //
 // Bound by the chosen experts' weights, each of which a call reads once. The split and
 // the sums are k_rows_xr's (rows_xr.hip): blocks of 16 MB rows of an expert against units
-// of S row quads of its weight over all of K (gated: a gate unit, then its up unit);
-// workgroup p owns a run of units, wave w the groups w, w + 8, ...; the block's
-// activations sit in registers while the weights stream through LDS slots, D items
-// ahead, across units, blocks and experts; the waves' sums meet in LDS in wave order.
-// Weights are used exactly: 128 + q as a bf16 operand, scale and zero point in fp32.
+// of S row quads of its weight over all of K -- gated, half of them gate quads and half
+// the up quads of the same columns, so that a lane has both sums of a column and a unit
+// is half as wide; workgroup p owns a run of units, wave w the groups w, w + 8, ...; the
+// block's activations sit in registers while the weights stream through LDS slots, D
+// items ahead, across units, blocks and experts; the waves' sums meet in LDS in wave
+// order. Weights are used exactly: 128 + q as a bf16 operand, scale and zero point in
+// fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/qwen_w4a16.h"
 #include "grouped.h"
@@ -28,16 +31,27 @@ struct Place {
   int block, unit, e;
 };
 
+// Item slot (16-byte units): S x 64 weight chunks, then a 256-byte area for each scale
+// and zero-point record (gated: the gate tile's and the up tile's).
+template <bool GLU, int S>
+struct ItemSlot {
+  static constexpr int kRecords = GLU ? 2 : 1;
+  static constexpr int kQuads = S / kRecords;   // quads of a record
+  static constexpr int kUnits = S * 64 + kRecords * 16;
+  static constexpr int kLoads = S + kRecords;
+};
+
 template <bool GLU, int S, int NG, int D, int MB>
 __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
-  using L = DmaSlot<4, S>;
-  constexpr int kL = L::kLoads;
-  constexpr uint32_t kPer = 4 / S;
+  using L = ItemSlot<GLU, S>;
+  constexpr int kL = L::kLoads, Q = L::kQuads;
+  constexpr uint32_t kPer = 4 / Q;         // units of a weight tile
   constexpr int kArea = 2 * MB * S * 64;   // a wave's sums of a unit, two buffers
   constexpr int kSums = MB == 1 ? 0 : NG * MB * 4;   // MB > 1: a wave's row sums (no registers left)
   // One LDS object: of several the compiler tells the accesses apart and waits for every
   // load into the slots before it reads the sums (vmcnt(0) in place of the counted waits).
   __shared__ u32x4 lds[kW * (D * L::kUnits + kArea + kSums) + (kMaxExperts + 1 + kW + 3) / 4];
+  static_assert(sizeof(lds) <= kLdsBytes, "the CU's LDS");
   u32x4* const slots = lds;
   f32x4* const red = reinterpret_cast<f32x4*>(slots + kW * D * L::kUnits);
   f32x4* const csum = red + kW * kArea;
@@ -46,17 +60,23 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, q = lane >> 4;
   int all[1];
-  expert_starts<64 * kW>(a, start, wsum, all, [](int rows, int) { return (rows + 16 * MB - 1) / (16 * MB); });
-  // units of a block (gated: pairs), and this workgroup's run of them
-  const int per = (GLU ? a.ld : a.n) / (16 * S);
+  auto blocks_of = [](int rows, int) { return (rows + 16 * MB - 1) / (16 * MB); };
+  if (a.offsets) {
+    expert_starts<64 * kW>(a, start, wsum, all, blocks_of);
+  } else {
+    all[0] = blocks_of(a.R, 0);
+    if (threadIdx.x < 2) start[threadIdx.x] = threadIdx.x ? all[0] : 0;
+    __syncthreads();
+  }
+  // units of a block, and this workgroup's run of them
+  const int per = a.ld / (16 * Q);
   const long long total = (long long)all[0] * per;
   const int p = blockIdx.x;
   const long long u0 = p * total / a.P, u1 = (p + 1) * total / a.P;
   int left_units = (int)(u1 - u0);
   if (left_units <= 0) return;
   const int nw = wave < a.G ? (a.G - 1 - wave) / kW + 1 : 0;   // groups of this wave (<= NG)
-  constexpr int kPair = GLU ? 2 : 1;
-  int left = nw * left_units * kPair;                           // items not yet done
+  int left = nw * left_units;                                   // items not yet done
 
   // a place moves on to the next unit, block and expert
   auto begin = [&](Place& v) __attribute__((always_inline)) {
@@ -72,10 +92,10 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
     }
   };
 
-  // The load cursor: unit, its half (gated: gate or up), group; weights of its expert.
+  // The load cursor: unit, group; weights of its expert.
   Place lp;
   begin(lp);
-  int lhalf = 0, lg = wave, lunits = left_units;
+  int lg = wave, lunits = left_units;
   __amdgpu_buffer_rsrc_t lqw, lsc;
   const uint32_t blocks = (uint32_t)(a.n / kTileN) * (uint32_t)a.G;   // weight blocks of an expert
   auto weights = [&]() __attribute__((always_inline)) {
@@ -88,26 +108,23 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
   weights();
   u32x4* const ring = slots + wave * D * L::kUnits;
   const uint32_t wbase = Fmt<4>::woff(q, c);
-  const int up_units = a.epi.up / (16 * S);
+  const uint32_t up_blocks = (uint32_t)(a.epi.up / kTileN) * (uint32_t)a.G;
   auto load_slot = [&](int j) __attribute__((always_inline)) {
-    const bool in = lunits > 0;
-    const uint32_t ru = (uint32_t)(lp.unit + lhalf * up_units);
-    const uint32_t st0 = ru % kPer * S;
+    const uint32_t ru = (uint32_t)lp.unit, st0 = ru % kPer * Q;
     // past the run: a block past the weights, which loads nothing
-    const uint32_t blk = in ? ru / kPer * (uint32_t)a.G + (uint32_t)lg : blocks;
+    const uint32_t blk = lunits > 0 ? ru / kPer * (uint32_t)a.G + (uint32_t)lg : blocks;
     const uint32_t voff = wbase + st0 * 256u;
     u32x4* const slot = ring + j * L::kUnits;
 #pragma unroll
-    for (int i = 0; i < S; ++i) dma_load16(lqw, slot + i * 64, voff + i * 256u, blk * 4096u);
-    dma_load4(lsc, slot + L::kNQ * 64, lane < 40 ? (uint32_t)lane * 4u : 0u, blk * (uint32_t)kMetaBytes);
+    for (int h = 0; h < L::kRecords; ++h) {
+      const uint32_t b = lunits > 0 ? blk + h * up_blocks : blocks;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) dma_load16(lqw, slot + (h * Q + i) * 64, voff + i * 256u, b * 4096u);
+      dma_load4(lsc, slot + S * 64 + h * 16, lane < 40 ? (uint32_t)lane * 4u : 0u, b * (uint32_t)kMetaBytes);
+    }
     lg += kW;
     if (lg < a.G) return;
     lg = wave;
-    if (GLU && lhalf == 0) {
-      lhalf = 1;
-      return;
-    }
-    lhalf = 0;
     if (--lunits > 0) {
       const int e = lp.e;
       next(lp);
@@ -120,7 +137,6 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
   }
 
   const NibConst k = nib_const();
-  const int zsh = 16 * (c & 1);
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3F803F80u, 0x3F803F80u,
                                                        0x3F803F80u, 0x3F803F80u});
   u32x4 x[NG][MB][4];
@@ -183,105 +199,105 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int i = 0; i < S; ++i) acc[mb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float gate[S];   // gated: the gate unit's sums
-#pragma unroll
-  for (int i = 0; i < S; ++i) gate[i] = 0.f;
   int j = 0, n = 0;   // slot of the next item; units closed
   while (true) {
-    const int st0 = (int)((uint32_t)at.unit % kPer) * S;
-    for (int half = 0; half < kPair; ++half) {
-      static_for<0, NG>([&](auto ic) __attribute__((always_inline)) {
-        constexpr int gi = decltype(ic)::value;
-        if (gi >= nw) return;   // wave-uniform
-        // this item has landed; the min(D - 1, left - 1) behind it may be in flight
-        if (left >= D)
-          wait_vm<(D - 1) * kL>();
-        else
-          wait_items<kL, D>(left - 1);
-        RowsData<4, S, true> d;
-        dma_read<4, S, true>(d, ring + j * L::kUnits, lane, st0);
-        f32x4 C[MB][S];
+    const int st0 = (int)((uint32_t)at.unit % kPer) * Q;
+    static_for<0, NG>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int gi = decltype(ic)::value;
+      if (gi >= nw) return;   // wave-uniform
+      // this item has landed; the min(D - 1, left - 1) behind it may be in flight
+      if (left >= D)
+        wait_vm<(D - 1) * kL>();
+      else
+        wait_items<kL, D>(left - 1);
+      const u32x4* const slot = ring + j * L::kUnits;
+      u32x4 w[S];
+      float sf[S], zf[S];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < S; ++i) w[i] = slot[i * 64 + lane];
 #pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const bf16x8 B = nib8(d.w[i][0][t], k);
+      for (int h = 0; h < L::kRecords; ++h) {
+        const uint32_t* const rec = reinterpret_cast<const uint32_t*>(slot + S * 64 + h * 16);
+        const uint32_t z = rec[32 + (c >> 1)] >> (16 * (c & 1) + 4 * st0);
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-              C[mb][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8, x[gi][mb][t]), B,
-                  t == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : C[mb][i], 0, 0, 0);
-          }
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          const f32x4 cs = MB == 1 ? Cs[MB == 1 ? gi : 0] : csum[wave * kSums + (gi * MB + mb) * 4 + q];
-#pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const uint32_t sbits = (d.s[i >> 1] >> (16 * (S == 1 ? (st0 & 1) : (i & 1)))) & 0xffffu;
-            const float sf = bf16_bits_to_f32(sbits);
-            const float zf = 128.0f + (float)((d.z >> (zsh + 4 * (st0 + i))) & 0xFu);
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj) acc[mb][i][jj] += sf * (C[mb][i][jj] - zf * cs[jj]);
-          }
-        }
-        // the slot's reads have returned: load the item D ahead into it
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (left > D) load_slot(j);
-        j = j + 1 == D ? 0 : j + 1;
-        --left;
-      });
-      // Unit sums in wave order; row 4 q + jj by wave jj (mod 4) of one half of the
-      // workgroup, the halves taking turns by output unit (MB = 2: a half each row
-      // block). Two buffers, one barrier a unit: a buffer is written again two
-      // barriers after it was read.
-      const int par = n & 1;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          red[wave * kArea + ((par * MB + mb) * S + i) * 64 + lane] = acc[mb][i];
-          acc[mb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-      lds_barrier<true>();
-      if (MB == 2 || (wave >> 2) == ((GLU ? n >> 1 : n) & 1)) {
-        const int jj = wave & 3, mb = MB == 2 ? wave >> 2 : 0;
-        float v[S];
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          const int from = (((par * MB + mb) * S + i) * 64 + lane) * 4 + jj;
-          v[i] = reinterpret_cast<const float*>(red)[from];
-#pragma unroll
-          for (int w = 1; w < kW; ++w) v[i] += reinterpret_cast<const float*>(red + w * kArea)[from];
-        }
-        if (GLU && half == 0) {
-#pragma unroll
-          for (int i = 0; i < S; ++i) gate[i] = v[i];
-        } else {
-          const int m = 16 * mb + 4 * q + jj;
-          const int n0 = (int)((uint32_t)at.unit / kPer) * kTileN + 4 * c + st0;
-          float f[GLU ? 2 : 1][S];
-#pragma unroll
-          for (int h = 0; h < (GLU ? 2 : 1); ++h) {
-            float b[S];
-            load_cols<S>(b, a.epi.bias, (size_t)at.e * a.n + h * a.epi.up + n0);
-#pragma unroll
-            for (int i = 0; i < S; ++i) f[h][i] = (GLU && h == 0 ? gate[i] : v[i]) + b[i];
-          }
-          epilogue_act<GLU, S>(f, a.epi.act);
-          if (m < rows) {
-            uint16_t* y = a.y + (size_t)(m0 + m) * a.ld + n0;
-            if constexpr (S == 1) {
-              y[0] = to_bf16(f[0][0]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < S / 2; ++i)
-                reinterpret_cast<uint32_t*>(y)[i] = pack_bf16x2(f[0][2 * i], f[0][2 * i + 1]);
-            }
-          }
+        for (int i = 0; i < Q; ++i) {   // row 4 c + st0 + i
+          const uint32_t s2 = rec[(4 * c + st0 + i) >> 1];
+          sf[h * Q + i] = bf16_bits_to_f32((s2 >> (16 * (Q == 1 ? st0 & 1 : i & 1))) & 0xffffu);
+          zf[h * Q + i] = 128.0f + (float)((z >> (4 * i)) & 0xFu);
         }
       }
-      ++n;
+      f32x4 C[MB][S];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const bf16x8 B = nib8(w[i][t], k);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+            C[mb][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, x[gi][mb][t]), B,
+                t == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : C[mb][i], 0, 0, 0);
+        }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const f32x4 cs = MB == 1 ? Cs[MB == 1 ? gi : 0] : csum[wave * kSums + (gi * MB + mb) * 4 + q];
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) acc[mb][i][jj] += sf[i] * (C[mb][i][jj] - zf[i] * cs[jj]);
+      }
+      // the slot's reads have returned: load the item D ahead into it
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (left > D) load_slot(j);
+      j = j + 1 == D ? 0 : j + 1;
+      --left;
+    });
+    // Unit sums in wave order; row 4 q + jj by wave jj (mod 4) of one half of the
+    // workgroup, the halves taking turns (MB = 2: a half each row block). Two buffers, one
+    // barrier a unit: a buffer is written again two barriers after it was read.
+    const int par = n & 1;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        red[wave * kArea + ((par * MB + mb) * S + i) * 64 + lane] = acc[mb][i];
+        acc[mb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    lds_barrier<true>();
+    if (MB == 2 || (wave >> 2) == (n & 1)) {
+      const int jj = wave & 3, mb = MB == 2 ? wave >> 2 : 0;
+      const int m = 16 * mb + 4 * q + jj;
+      const int n0 = (int)((uint32_t)at.unit / kPer) * kTileN + 4 * c + st0;
+      float f[L::kRecords][Q];
+#pragma unroll
+      for (int h = 0; h < L::kRecords; ++h) {
+        float b[Q];
+        load_cols<Q>(b, a.epi.bias, (size_t)at.e * a.n + h * a.epi.up + n0);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const int from = (((par * MB + mb) * S + h * Q + i) * 64 + lane) * 4 + jj;
+          float v = reinterpret_cast<const float*>(red)[from];
+#pragma unroll
+          for (int w = 1; w < kW; ++w) v += reinterpret_cast<const float*>(red + w * kArea)[from];
+          f[h][i] = v + b[i];
+        }
+      }
+      epilogue_act<GLU, Q>(f, a.epi.act);
+      if (m < rows) {
+        const size_t to = (size_t)(m0 + m) * a.ld + n0;
+        float res[Q];
+        load_cols<Q>(res, a.epi.res, to);
+        if constexpr (Q == 1) {
+          a.y[to] = to_bf16(f[0][0] + res[0]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < Q / 2; ++i)
+            reinterpret_cast<uint32_t*>(a.y + to)[i] =
+                pack_bf16x2(f[0][2 * i] + res[2 * i], f[0][2 * i + 1] + res[2 * i + 1]);
+        }
+      }
     }
+    ++n;
     if (--left_units == 0) break;
     const int block = at.block;
     next(at);
@@ -295,32 +311,64 @@ void launch(const GroupedArgs& a, hipStream_t st) {
   k_grouped_rows<GLU, S, NG, D, MB><<<a.P, 64 * kW, 0, st>>>(a);
 }
 
-template <bool GLU, int S, int MB>
+// Registers for 2, 5 or 8 groups a wave (K up to 2048, 5120, 8192).
+template <bool GLU, int S, int D>
 void launch_ng(const GroupedArgs& a, hipStream_t st) {
   const int ng = (a.G + kW - 1) / kW;
-  if (ng <= 3)
-    launch<GLU, S, 3, 3, MB>(a, st);
+  if (ng <= 2)
+    launch<GLU, S, 2, D, 1>(a, st);
   else if (ng <= 5)
-    launch<GLU, S, 5, 3, MB>(a, st);
-  else if constexpr (MB == 1)
-    launch<GLU, S, kMaxGroups, 3, MB>(a, st);
+    launch<GLU, S, 5, D, 1>(a, st);
+  else
+    launch<GLU, S, kMaxGroups, D, 1>(a, st);
+}
+
+template <bool GLU>
+void launch_rows(const GroupedArgs& a, int MB, int S, hipStream_t st) {
+  if (MB == 2)
+    launch<GLU, 2, 5, 4, 2>(a, st);
+  else if (S == 4)
+    launch_ng<GLU, 4, 2>(a, st);
+  else
+    launch_ng<GLU, 2, 3>(a, st);
 }
 
 }  // namespace
 
+// Where it is the faster form, by the mean rows of an expert (us, blocks of 16 rows / of 32
+// / the tiles of grouped.hip; experts, K -> weight rows):
+//   64, 2048 -> 2048 gated   24 rows  64 / 59 / 69,     48 rows  89 / 88 / 86
+//   64, 1024 -> 2048         32      41 / 46 / 44,      48       55 / 61 / 45
+//   32, 5120 -> 4352 gated   16      98 / 104 / 147,    32       158 / 140 / 180,   64  289 / 210 / 191
+//   16, 4096 -> 4096         24      41 / 55 / 64,      48       84 / 77 / 79
+//   32, 2176 -> 5120         24      72 / 73 / 74,      32       84 / 84 / 75
+// so up to 40 rows, fewer where the last of a wave's groups are missing (2176 is 17 groups
+// for 8 waves). Blocks of 32 rows read the weights of such experts once, but pay more for
+// every unit: from 20 rows on, where K is long. Beyond 5 groups a wave, whose registers
+// 32 rows do not fit, up to 24 rows.
+//
+// Blocks of 16: units of four row quads, two items ahead, or of two, three ahead, where
+// that leaves the fullest workgroup less. us (4 / 2 quads), 8 of 64 experts: 2048 -> 2 x 1024
+// of 1 / 16 / 64 tokens 7.1 / 21.9 / 30.4, 7.6 / 24.5 / 33.4, 1024 -> 2048 of 16 15.4, 17.5; 4 of 32,
+// 5120 -> 2 x 2176 of 1 token (272 and 544 units on 256 CUs) 15.4, 14.4. Two workgroups a
+// CU were slower throughout (18 to 28 us for 16 tokens).
 bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, hipStream_t s) {
   const int ng = (a.G + kW - 1) / kW;
-  const int mean = a.R / a.E;
-  if (ng > kMaxGroups || mean > 32) return false;
-  const int MB = mean > 12 && ng <= 5 ? 2 : 1;
-  const int width = glu ? a.ld : a.n;
+  const double mean = (double)a.R / a.E;
+  if (ng > kMaxGroups || mean > (ng > 5 ? 24. : 40.) * (a.G < kW ? 1. : (double)a.G / (ng * kW))) return false;
+  const int MB = mean > 20 && (ng == 4 || ng == 5) ? 2 : 1;
+  // experts in use: a token's are different ones; many tokens' as if drawn evenly
+  const double used = 4 * (long long)a.R <= a.E ? a.R : a.E * (1.0 - std::exp(-mean));
+  auto fullest = [&](int S) {   // row quads of the fullest workgroup
+    const double units = used * (a.ld / (16 * (glu ? S / 2 : S)));
+    return std::ceil(units / cus) * S;
+  };
   a.P = cus;
-  if (glu) {
-    MB == 2 ? launch_ng<true, 2, 2>(a, s) : launch_ng<true, 2, 1>(a, s);
-  } else {
-    MB == 2 ? launch_ng<false, 2, 2>(a, s) : launch_ng<false, 2, 1>(a, s);
-  }
-  (void)width;
+  const int S = fullest(4) <= fullest(2) ? 4 : 2;
+  if (glu)
+    launch_rows<true>(a, MB, S, s);
+  else
+    launch_rows<false>(a, MB, S, s);
   return true;
 }
 

@@ -43,11 +43,11 @@ int few_rows(uint16_t* y, int width, const qw4_weights* w, const uint16_t* x, in
       ei = *e;
       if (ei.res) ei.res += (size_t)i * width;
     }
-    // two 16-row passes in one where it pays; a last single row stays a pass
-    // of its own (the GEMV's sums)
+    // two 16-row passes in one where it pays; in qw4_linear a last single row stays
+    // a pass of its own (the GEMV's sums)
     const int left = T - i;
     n = left < 32 ? left : 32;
-    if (n % 16 == 1) --n;
+    if (!e && n % 16 == 1) --n;
     if (chunk == 16 && n > 16) {
       bool taken = false;
       const int st = qw4::skinny_rows32(yi, w, xi, n, s, stream, e ? &ei : nullptr, &taken);
