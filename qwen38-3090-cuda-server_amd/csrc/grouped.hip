@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
   int* const rexp = from + 2 * kRows;
   int* const start = rexp + 2 * kRows;
   int* const wsum = start + kLists * (kMaxExperts + 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int blocks[kLists];   // whole, and ending by height
   expert_starts<256>(a, start, wsum, blocks, [](int rows, int which) {
     const int end = rows % (32 * MB);
@@ -64,8 +64,6 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
 #pragma unroll
   for (int l = 0; l < kLists; ++l) all += blocks[l] * a.tiles_n;
   const uint32_t row_bytes = (uint32_t)a.K * 2u;
-  const int srow = 4 * wave + (lane >> 4);   // row within the 16-row swizzle period
-  const uint32_t chunk = (uint32_t)((lane & 15) ^ srow) * 16u;
   const int up = a.epi.up / kTileN;
   const int width = GLU ? a.ld : a.n;   // columns the column tiles run over
   int turn = 0;
@@ -99,6 +97,12 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
     const int b0 = GLU ? wave & 1 : 0;
     const int col = wt * kTileN + 32 * b0;
     const bool valid = wt * kTileN < width;
+    // opaque, so that the addresses of every height are formed where they are used and
+    // not kept, spilled, from before the loop
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int srow = 4 * wave + (lane >> 4);   // row within the 16-row swizzle period
+    const uint32_t chunk = (uint32_t)((lane & 15) ^ srow) * 16u;
     const int ltile = valid ? wt : width / kTileN - 1;
     const size_t blk = (size_t)e * (a.n / kTileN) * a.G;   // the expert's first weight block
     const G2Rsrc wr = g2_weights(a.qw + blk * kWordsPerBlock, a.sc + blk * kMetaU16, a.zr + blk * 16, a.n, a.G);
