@@ -16,9 +16,12 @@ namespace {
 
 constexpr int kMaxExperts = 1024;   // 16 logits a lane
 constexpr int kMaxTopK = 16;        // a row of 16 lanes holds a token's choice
-// Pairs that one workgroup routes and plans in a single launch: a thread each, whose
-// place among its expert's pairs is counted over all pairs before it.
-constexpr int kSmallPairs = 256;
+// Pairs that one workgroup plans: a thread each, whose place among its expert's pairs is
+// counted over all pairs before it (256 pairs: 1.5 us slower than k_plan).
+constexpr int kSmallPairs = 128;
+// Tokens of such a plan that it routes as well, in a single launch, a wave each (32 tokens
+// over 128 experts: 11.7 us, in two launches 7.0; 16 over 64: 6.8 and 6.9).
+constexpr int kSmallTokens = 16;
 
 struct PlanArgs {
   int32_t *offsets, *tokens, *pos;   // offsets null: no plan wanted
@@ -156,17 +159,19 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   }
 }
 
-// The plan of R <= kSmallPairs pairs by one workgroup of 1024 threads, from their
-// experts in LDS: a histogram (integer atomics: any order gives the same counts), its
+// The plan of R <= kSmallPairs pairs by one workgroup of 64 W threads, at least E and
+// R, from their experts in LDS: a histogram (integer atomics: any order gives the same counts), its
 // running sum, and for each pair the earlier pairs of its expert counted.
+template <int W>
 struct SmallPlan {
   int ids[kSmallPairs];
-  int start[kMaxExperts + 1];
-  int wsum[16];
+  int start[64 * W];
+  int wsum[W];
 };
-__device__ __forceinline__ void plan_small(const PlanArgs& p, SmallPlan& s, int R, int E, int k) {
+template <int W>
+__device__ __forceinline__ void plan_small(const PlanArgs& p, SmallPlan<W>& s, int R, int E, int k) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  s.start[t] = 0;   // one entry per thread: kMaxExperts threads
+  s.start[t] = 0;   // one entry per thread
   __syncthreads();
   const int id = t < R ? s.ids[t] : -1;
   const bool live = (unsigned)id < (unsigned)E;
@@ -183,7 +188,7 @@ __device__ __forceinline__ void plan_small(const PlanArgs& p, SmallPlan& s, int 
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < W; ++w) {
     const int v = s.wsum[w];
     before += w < wave ? v : 0;
     all += v;
@@ -204,12 +209,13 @@ __device__ __forceinline__ void plan_small(const PlanArgs& p, SmallPlan& s, int 
 }
 
 // Few tokens: choice and plan in one launch. A decoded token's router is all latency,
-// and a second launch would add as much again.
-template <class T, int PER>
-__global__ __launch_bounds__(1024) void k_route_small(RouteArgs a) {
-  __shared__ SmallPlan s;
+// and a second launch would add as much again; of few waves where they do (4 instead of
+// 16, one token over 64 experts: 3.8 us instead of 4.0).
+template <class T, int PER, int W>
+__global__ __launch_bounds__(64 * W) void k_route_small(RouteArgs a) {
+  __shared__ SmallPlan<W> s;
   const int lane = threadIdx.x & 63;
-  for (int t = threadIdx.x >> 6; t < a.T; t += 16) {
+  for (int t = threadIdx.x >> 6; t < a.T; t += W) {
     int id;
     float w;
     route_row<T, PER>(a, t, lane, id, w);
@@ -224,7 +230,7 @@ __global__ __launch_bounds__(1024) void k_route_small(RouteArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void k_plan_small(PlanArgs p, const int32_t* ids, int R, int E, int k) {
-  __shared__ SmallPlan s;
+  __shared__ SmallPlan<16> s;
   if ((int)threadIdx.x < R) s.ids[threadIdx.x] = ids[threadIdx.x];
   __syncthreads();
   plan_small(p, s, R, E, k);
@@ -234,8 +240,9 @@ __global__ __launch_bounds__(1024) void k_plan_small(PlanArgs p, const int32_t* 
 // the w-th sixteenth of the pairs' experts, kPlanAhead rounds of 64 at once: first it
 // counts those below e (they come before e's first position) and those equal to e, then
 // it gives the equal ones their places; up to 16 x 64 kPlanAhead pairs stay in registers
-// in between. No workgroup waits for another. Bound by the latency of the loads: 32768
-// pairs of 128 experts 22.2 us with a round at a time, 5.4 so.
+// in between. No workgroup waits for another. Bound by the instructions of a workgroup's
+// 16 waves: 32768 pairs of 128 experts 22.2 us with a load at a time, 11.5 with all in
+// flight, 9.4 without a division for every hit.
 constexpr int kPlanAhead = 32;
 
 __global__ __launch_bounds__(1024) void k_plan(PlanArgs p, const int32_t* ids, int R, int E, int k) {
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(1024) void k_plan(PlanArgs p, const int32_t* ids, i
   const long long first = (long long)wave * seg;
   const int i0 = (int)std::min<long long>(first, R), i1 = (int)std::min<long long>(first + seg, R);
   int id[kPlanAhead];
-  auto load = [&](int i) {
+  auto load = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < kPlanAhead; ++r) {
       const int at = i + 64 * r + lane;
@@ -284,20 +291,31 @@ __global__ __launch_bounds__(1024) void k_plan(PlanArgs p, const int32_t* ids, i
     p.offsets[e] = start;
     if (e == E - 1) p.offsets[E] = start + total;
   }
+  // x / k = x inv / 2^16 for x < kRound + k: inv k - 2^16 < k <= 16 moves it by x / 2^16 < 1 / k
+  const uint32_t inv = (65536u + (uint32_t)k - 1u) / (uint32_t)k;
+  static_assert((kRound + kMaxTopK) * kMaxTopK < 65536, "exact");
   for (int i = i0; i < i1; i += kRound) {
     if (!kept) load(i);
+    const int tok0 = i / k;
+    const uint32_t x0 = (uint32_t)(i - tok0 * k + lane);
 #pragma unroll
     for (int r = 0; r < kPlanAhead; ++r) {
       if (i + 64 * r >= i1) break;
-      const int pair = i + 64 * r + lane;
       const unsigned long long hit = __ballot(id[r] == e);
-      if (id[r] == e) {
-        const int to = at + (int)__popcll(hit & ((1ull << lane) - 1ull));
-        p.tokens[to] = pair / k;
-        p.pos[pair] = to;
+      if (hit) {   // wave-uniform
+        if (id[r] == e) {
+          const int to = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
+                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+          p.tokens[to] = tok0 + (int)((x0 + 64u * r) * inv >> 16);
+          p.pos[i + 64 * r + lane] = to;
+        }
+        at += (int)__popcll(hit);
       }
-      if (e == 0 && pair < i1 && (unsigned)id[r] >= (unsigned)E) p.pos[pair] = -1;
-      at += (int)__popcll(hit);
+    }
+    if (e == 0) {   // the pairs of no expert
+#pragma unroll
+      for (int r = 0; r < kPlanAhead; ++r)
+        if (i + 64 * r + lane < i1 && (unsigned)id[r] >= (unsigned)E) p.pos[i + 64 * r + lane] = -1;
     }
     if (i1 - i <= kRound) break;
   }
@@ -375,8 +393,11 @@ void launch_plan(const PlanArgs& p, const int32_t* ids, int R, int E, int k, hip
 
 template <class T, int PER>
 void launch_route(const RouteArgs& a, hipStream_t s) {
-  if (a.plan.offsets && a.T * a.k <= kSmallPairs) {
-    k_route_small<T, PER><<<1, 1024, 0, s>>>(a);
+  if (a.plan.offsets && a.T <= kSmallTokens && a.T * a.k <= kSmallPairs) {
+    if (PER <= 4 && a.T <= 4)
+      k_route_small<T, PER, 4><<<1, 256, 0, s>>>(a);
+    else
+      k_route_small<T, PER, 16><<<1, 1024, 0, s>>>(a);
     return;
   }
   if (a.T > 0) k_route<T, PER><<<(a.T + 3) / 4, 256, 0, s>>>(a);
