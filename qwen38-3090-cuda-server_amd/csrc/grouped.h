@@ -16,9 +16,9 @@ struct GroupedArgs {
   const uint16_t* zr;
   const uint16_t* x;
   uint16_t* y;
-  const int32_t* offsets;   // [E + 1], or null: one expert with R rows
+  const int32_t* offsets;   // [E + 1]
   const int32_t* tokens;    // row of x at each position
-  Epilogue epi;             // bias and up of an expert's weight rows; residual [R][ld]
+  Epilogue epi;             // bias and up of an expert's weight rows; no residual
   int E, n, K, G;           // n weight rows an expert
   int R;                    // positions (rows of y)
   uint32_t x_bytes;         // of a gathered x
@@ -27,14 +27,9 @@ struct GroupedArgs {
   const int *rexp, *cexp;   // fp16 operands: exponents of x's rows and of the weight rows
 };
 
-// Expert e's positions; without offsets, one expert's: all. Offsets that are no plan's
-// (negative, falling, past R) give fewer or no rows, never one outside y.
+// Expert e's positions. Offsets that are no plan's (negative, falling, past R) give
+// fewer or no rows, never one outside y.
 __device__ __forceinline__ void expert_rows(const GroupedArgs& a, int e, int& lo, int& hi) {
-  if (!a.offsets) {
-    lo = 0;
-    hi = a.R;
-    return;
-  }
   lo = min(max(a.offsets[e], 0), a.R);
   hi = min(max(a.offsets[e + 1], lo), a.R);
 }
