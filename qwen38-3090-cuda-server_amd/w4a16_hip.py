@@ -216,18 +216,17 @@ def _chk(status: int, where: str) -> None:
 
 
 def _ptr(t) -> int | None:
-    if t is None:
-        return None
+    if t is None or t.__class__ is int:
+        return t
     return t.data_ptr() if hasattr(t, "data_ptr") else int(t)
 
 
 def _need(t, nbytes: int, where: str) -> None:
     """Host-side bounds check before a launch: a torch tensor argument must hold
     at least nbytes (raw integer pointers cannot be checked and are trusted)."""
-    if t is not None and hasattr(t, "numel") and hasattr(t, "element_size"):
-        have = t.numel() * t.element_size()
-        if have < nbytes:
-            raise ValueError(f"{where}: buffer holds {have} bytes, needs {nbytes}")
+    have = getattr(t, "nbytes", nbytes)
+    if have < nbytes:
+        raise ValueError(f"{where}: buffer holds {have} bytes, needs {nbytes}")
 
 
 _torch = None
