@@ -218,7 +218,10 @@ def _chk(status: int, where: str) -> None:
 def _ptr(t) -> int | None:
     if t is None or t.__class__ is int:
         return t
-    return t.data_ptr() if hasattr(t, "data_ptr") else int(t)
+    try:
+        return t.data_ptr()
+    except AttributeError:
+        return int(t)
 
 
 def _need(t, nbytes: int, where: str) -> None:
