@@ -369,7 +369,8 @@ enum {
  * for QW4_ACT_SWIGLU with a 256-byte aligned workspace of at least
  * qw4_epilogue_workspace(w, T) bytes, to 11 bits: each factor of a gated output carries
  * the weights' rounding. s and ws may be NULL; calls that share one must be
- * stream-ordered. All pointers 16-byte aligned. */
+ * stream-ordered. All pointers 16-byte aligned; beyond qw4_linear_max_t rows, x below
+ * 4 GiB. */
 int qw4_linear_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T,
                         const uint16_t* bias, int act, const uint16_t* residual, qw4_scratch* s,
                         qw4_workspace* ws, void* stream);

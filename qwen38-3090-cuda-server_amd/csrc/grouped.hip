@@ -60,9 +60,10 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
     const int high = 32 * MB >> (which - 1), low = which == kEnds ? 0 : high >> 1;
     return which == 0 ? rows / (32 * MB) : (int)(end > low && end <= high);
   });
-  int all = 0;
+  long long tiles = 0;
 #pragma unroll
-  for (int l = 0; l < kLists; ++l) all += blocks[l] * a.tiles_n;
+  for (int l = 0; l < kLists; ++l) tiles += (long long)blocks[l] * a.tiles_n;
+  const int all = (int)min(tiles, 0x3fffffffLL);   // more: offsets of no plan
   const uint32_t row_bytes = (uint32_t)a.K * 2u;
   const int up = a.epi.up / kTileN;
   const int width = GLU ? a.ld : a.n;   // columns the column tiles run over
