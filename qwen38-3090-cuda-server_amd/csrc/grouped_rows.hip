@@ -107,12 +107,19 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
     }
   };
 
-  // The load cursor: unit, group; weights of its expert.
+  // The load cursor: the unit's place, its group as byte offsets into the expert's
+  // weights and scales, and the lanes' offsets. A wave has only one other on its SIMD, so
+  // its scalar work is not hidden: what an item needs is kept up to date by additions.
   Place lp;
   begin(lp);
   int lg = wave, lunits = left_units;
   __amdgpu_buffer_rsrc_t lqw, lsc;
   const uint32_t blocks = (uint32_t)(a.n / kTileN) * (uint32_t)a.G;   // weight blocks of an expert
+  const uint32_t up_blocks = (uint32_t)(a.epi.up / kTileN) * (uint32_t)a.G;
+  const uint32_t wbase = Fmt<4>::woff(q, c);
+  uint32_t wsoff = 0, msoff = 0;
+  uint32_t wvoff = 0;
+  const uint32_t mvoff = lane < 40 ? (uint32_t)lane * 4u : 0u;
   auto weights = [&]() __attribute__((always_inline)) {
     const size_t blk = (size_t)lp.e * blocks;
     lqw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(a.qw + blk * kWordsPerBlock), 0,
@@ -120,23 +127,26 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
     lsc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.sc + blk * kMetaU16), 0,
                                             (int)(blocks * (uint32_t)kMetaBytes), 0x00020000);
   };
+  auto unit = [&]() __attribute__((always_inline)) {
+    const uint32_t ru = (uint32_t)lp.unit, blk = ru / kPer * (uint32_t)a.G + (uint32_t)wave;
+    wsoff = (uint32_t)__builtin_amdgcn_readfirstlane(blk * 4096u);
+    msoff = (uint32_t)__builtin_amdgcn_readfirstlane(blk * (uint32_t)kMetaBytes);
+    wvoff = wbase + ru % kPer * Q * 256u;
+  };
   weights();
+  unit();
   u32x4* const ring = slots + wave * D * L::kUnits;
-  const uint32_t wbase = Fmt<4>::woff(q, c);
-  const uint32_t up_blocks = (uint32_t)(a.epi.up / kTileN) * (uint32_t)a.G;
   auto load_slot = [&](int j) __attribute__((always_inline)) {
-    const uint32_t ru = (uint32_t)lp.unit, st0 = ru % kPer * Q;
-    // past the run: a block past the weights, which loads nothing
-    const uint32_t blk = lunits > 0 ? ru / kPer * (uint32_t)a.G + (uint32_t)lg : blocks;
-    const uint32_t voff = wbase + st0 * 256u;
     u32x4* const slot = ring + j * L::kUnits;
 #pragma unroll
     for (int h = 0; h < L::kRecords; ++h) {
-      const uint32_t b = lunits > 0 ? blk + h * up_blocks : blocks;
 #pragma unroll
-      for (int i = 0; i < Q; ++i) dma_load16(lqw, slot + (h * Q + i) * 64, voff + i * 256u, b * 4096u);
-      dma_load4(lsc, slot + S * 64 + h * 16, lane < 40 ? (uint32_t)lane * 4u : 0u, b * (uint32_t)kMetaBytes);
+      for (int i = 0; i < Q; ++i)
+        dma_load16(lqw, slot + (h * Q + i) * 64, wvoff + i * 256u, wsoff + h * (up_blocks * 4096u));
+      dma_load4(lsc, slot + S * 64 + h * 16, mvoff, msoff + h * (up_blocks * (uint32_t)kMetaBytes));
     }
+    wsoff = (uint32_t)__builtin_amdgcn_readfirstlane(wsoff + kW * 4096u);
+    msoff = (uint32_t)__builtin_amdgcn_readfirstlane(msoff + kW * (uint32_t)kMetaBytes);
     lg += kW;
     if (lg < a.G) return;
     lg = wave;
@@ -144,11 +154,13 @@ __global__ __launch_bounds__(64 * kW) void k_grouped_rows(GroupedArgs a) {
       const int e = lp.e;
       next(lp);
       if (lp.e != e) weights();
+      unit();
     }
   };
   if (nw > 0) {
 #pragma unroll
-    for (int j = 0; j < D; ++j) load_slot(j);
+    for (int j = 0; j < D; ++j)
+      if (j < left) load_slot(j);
   }
 
   const NibConst k = nib_const();
