@@ -216,7 +216,7 @@ def _chk(status: int, where: str) -> None:
 
 
 def _ptr(t) -> int | None:
-    if t is None or t.__class__ is int:
+    if t is None or type(t) is int:
         return t
     try:
         return t.data_ptr()
@@ -233,6 +233,19 @@ def _need(t, nbytes: int, where: str) -> None:
 
 
 _torch = None
+
+
+def _buf(t, nbytes: int, where: str) -> int | None:
+    """The address of a buffer of nbytes at least: _need and _ptr in one, 0.1 us less an
+    argument of a call that takes 6 us."""
+    if t is None or type(t) is int:
+        return t
+    try:
+        if t.nbytes < nbytes:
+            raise ValueError(f"{where}: buffer holds {t.nbytes} bytes, needs {nbytes}")
+        return t.data_ptr()
+    except AttributeError:
+        return int(t)
 
 
 def _current_stream() -> int:
@@ -463,11 +476,10 @@ def linear_epilogue_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch | None =
                           residual=None, stream=None) -> None:
     """qw4_linear_epilogue: y = bf16(act(x @ W^T + bias) + residual), one rounding."""
     width = w.out_f // 2 if act == ACT_SWIGLU else w.out_f
-    _need(y, T * width * 2, "linear_epilogue y")
-    _need(x, T * w.in_f * 2, "linear_epilogue x")
-    _need(bias, w.out_f * 2, "linear_epilogue bias")
-    _need(residual, T * width * 2, "linear_epilogue residual")
-    _chk(lib().qw4_linear_epilogue(_ptr(y), C.byref(w), _ptr(x), T, _ptr(bias), act, _ptr(residual),
+    _chk(lib().qw4_linear_epilogue(_buf(y, T * width * 2, "linear_epilogue y"), C.byref(w),
+                                   _buf(x, T * w.in_f * 2, "linear_epilogue x"), T,
+                                   _buf(bias, w.out_f * 2, "linear_epilogue bias"), act,
+                                   _buf(residual, T * width * 2, "linear_epilogue residual"),
                                    C.byref(s) if s is not None else None,
                                    C.byref(ws) if ws is not None else None, _stream(stream)),
          "linear_epilogue")
@@ -621,17 +633,15 @@ def route_experts_f32(ids, weights, logits, T: int, experts: int, top_k: int, re
 
 
 def _route(call, size, where, ids, weights, logits, T, experts, top_k, renorm, plan, stream):
-    _need(ids, T * top_k * 4, where)
-    _need(weights, T * top_k * 4, where)
-    _need(logits, T * experts * size, where)
-    _chk(call(_ptr(ids), _ptr(weights), C.byref(plan) if plan is not None else None, _ptr(logits), T,
+    _chk(call(_buf(ids, T * top_k * 4, where), _buf(weights, T * top_k * 4, where),
+              C.byref(plan) if plan is not None else None, _buf(logits, T * experts * size, where), T,
               experts, top_k, int(renorm), _stream(stream)), where)
 
 
 def route_expert_ids(plan: ExpertPlan, ids, T: int, top_k: int, stream=None) -> None:
     """qw4_route_ids: the plan of ids [T][top_k] chosen elsewhere."""
-    _need(ids, T * top_k * 4, "route_expert_ids ids")
-    _chk(lib().qw4_route_ids(C.byref(plan), _ptr(ids), T, top_k, _stream(stream)), "route_expert_ids")
+    _chk(lib().qw4_route_ids(C.byref(plan), _buf(ids, T * top_k * 4, "route_expert_ids ids"), T, top_k,
+                             _stream(stream)), "route_expert_ids")
 
 
 def gemm_grouped_w4a16(y, w: W4A16Weights, x, plan: ExpertPlan, pairs: int, gather: bool,
@@ -643,23 +653,20 @@ def gemm_grouped_w4a16(y, w: W4A16Weights, x, plan: ExpertPlan, pairs: int, gath
     if x_rows is None:
         x_rows = x.numel() // w.in_f
     width = w.out_f // max(plan.experts, 1) // (2 if act == ACT_SWIGLU else 1)
-    _need(y, pairs * width * 2, "gemm_grouped y")
-    _need(x, x_rows * w.in_f * 2, "gemm_grouped x")
-    _need(bias, w.out_f * 2, "gemm_grouped bias")
-    _chk(lib().qw4_gemm_grouped(_ptr(y), C.byref(w), _ptr(x), x_rows, C.byref(plan), pairs, int(gather),
-                                _ptr(bias), act, C.byref(ws) if ws is not None else None,
-                                _stream(stream)), "gemm_grouped")
+    _chk(lib().qw4_gemm_grouped(_buf(y, pairs * width * 2, "gemm_grouped y"), C.byref(w),
+                                _buf(x, x_rows * w.in_f * 2, "gemm_grouped x"), x_rows, C.byref(plan), pairs,
+                                int(gather), _buf(bias, w.out_f * 2, "gemm_grouped bias"), act,
+                                C.byref(ws) if ws is not None else None, _stream(stream)), "gemm_grouped")
 
 
 def combine_experts(out, y, weights, T: int, top_k: int, dim: int, plan: ExpertPlan, residual=None,
                     stream=None) -> None:
     """qw4_combine: out = bf16(residual + sum_j weights[t][j] * y[pos of (t, j)])."""
-    _need(out, T * dim * 2, "combine_experts out")
-    _need(y, T * top_k * dim * 2, "combine_experts y")
-    _need(weights, T * top_k * 4, "combine_experts weights")
-    _need(residual, T * dim * 2, "combine_experts residual")
-    _chk(lib().qw4_combine(_ptr(out), _ptr(y), C.byref(plan), _ptr(weights), T, top_k, dim,
-                           _ptr(residual), _stream(stream)), "combine_experts")
+    _chk(lib().qw4_combine(_buf(out, T * dim * 2, "combine_experts out"),
+                           _buf(y, T * top_k * dim * 2, "combine_experts y"), C.byref(plan),
+                           _buf(weights, T * top_k * 4, "combine_experts weights"), T, top_k, dim,
+                           _buf(residual, T * dim * 2, "combine_experts residual"), _stream(stream)),
+         "combine_experts")
 
 
 # ------------------------------------------------------ synthetic inputs
