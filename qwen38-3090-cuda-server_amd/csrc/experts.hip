@@ -76,6 +76,15 @@ __device__ __forceinline__ float wave_add(float v) {
   return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
 }
 
+__device__ __forceinline__ int wave_add_int(int v) {
+  v += (int)dpp<0xB1>((uint32_t)v);
+  v += (int)dpp<0x4E>((uint32_t)v);
+  v += (int)dpp<0x141>((uint32_t)v);
+  v += (int)dpp<0x140>((uint32_t)v);
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+
 template <class T>
 __device__ __forceinline__ float logit(const T* p) {
   if constexpr (std::is_same_v<T, float>)
@@ -237,43 +246,65 @@ __global__ __launch_bounds__(1024) void k_plan_small(PlanArgs p, const int32_t* 
 }
 
 // The plan of many pairs: workgroup e gathers expert e's pairs, in order. Wave w takes
-// the w-th sixteenth of the pairs' experts, kPlanAhead rounds of 64 at once: first it
-// counts those below e (they come before e's first position) and those equal to e, then
-// it gives the equal ones their places; up to 16 x 64 kPlanAhead pairs stay in registers
-// in between. No workgroup waits for another. Bound by the instructions of a workgroup's
-// 16 waves: 32768 pairs of 128 experts 22.2 us with a load at a time, 11.5 with all in
-// flight, 9.4 without a division for every hit.
-constexpr int kPlanAhead = 32;
+// the w-th sixteenth of the pairs' experts, kPlanAhead loads of 256 at once, four pairs a
+// lane: first it counts those below e (they come before e's first position) and those equal
+// to e, then it gives the equal ones their places; up to 16 x 256 kPlanAhead pairs stay in
+// registers in between. No workgroup waits for another. Bound by the instructions of a
+// workgroup's 16 waves: 32768 pairs of 128 experts 22.2 us with a load at a time, 11.5 with
+// all in flight, 9.4 without a division for every hit, 8.0 with four pairs a load.
+constexpr int kPlanAhead = 8;
 
 __global__ __launch_bounds__(1024) void k_plan(PlanArgs p, const int32_t* ids, int R, int E, int k) {
   __shared__ int below[16], equal[16];
   const int e = blockIdx.x, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int seg = ((R + 1023) / 1024) * 64;   // pairs of a wave, in whole rounds
+  const int seg = ((R - 1) / 4096 + 1) * 256;   // pairs of a wave, in whole loads
   const long long first = (long long)wave * seg;
   const int i0 = (int)std::min<long long>(first, R), i1 = (int)std::min<long long>(first + seg, R);
-  int id[kPlanAhead];
+  typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int kRound = 256 * kPlanAhead;
+  int id[kPlanAhead][4];   // pair i + 256 r + 4 lane + c
   auto load = [&](int i) __attribute__((always_inline)) {
+    auto four = [&](int r) __attribute__((always_inline)) {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(ids + i + 256 * r + 4 * lane);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) id[r][c] = v[c];
+    };
+    if (i1 - i >= kRound) {   // without a branch a load
+#pragma unroll
+      for (int r = 0; r < kPlanAhead; ++r) four(r);
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < kPlanAhead; ++r) {
-      const int at = i + 64 * r + lane;
-      id[r] = -1;
-      if (i + 64 * r < i1 && at < i1) id[r] = ids[at];   // the first test is wave-uniform
+      const int left = i1 - i - 256 * r;   // wave-uniform
+      if (left >= 256) {
+        four(r);
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        id[r][c] = -1;
+        if (left > 0 && 4 * lane + c < left) id[r][c] = ids[i + 256 * r + 4 * lane + c];
+      }
     }
   };
-  constexpr int kRound = 64 * kPlanAhead;
   const bool kept = i1 - i0 <= kRound;
   int nb = 0, ne = 0;
   for (int i = i0; i < i1; i += kRound) {
     load(i);
 #pragma unroll
     for (int r = 0; r < kPlanAhead; ++r) {
-      if (i + 64 * r >= i1) break;
-      nb += (int)__popcll(__ballot((unsigned)id[r] < (unsigned)e));
-      ne += (int)__popcll(__ballot(id[r] == e));
+      if (i1 - i <= 256 * r) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        nb += (unsigned)id[r][c] < (unsigned)e;
+        ne += (int)__popcll(__ballot(id[r][c] == e));
+      }
     }
     if (i1 - i <= kRound) break;   // no overflow of i
   }
+  nb = wave_add_int(nb);
   if (lane == 0) {
     below[wave] = nb;
     equal[wave] = ne;
@@ -297,25 +328,38 @@ __global__ __launch_bounds__(1024) void k_plan(PlanArgs p, const int32_t* ids, i
   for (int i = i0; i < i1; i += kRound) {
     if (!kept) load(i);
     const int tok0 = i / k;
-    const uint32_t x0 = (uint32_t)(i - tok0 * k + lane);
+    const uint32_t x0 = (uint32_t)(i - tok0 * k + 4 * lane);
 #pragma unroll
     for (int r = 0; r < kPlanAhead; ++r) {
-      if (i + 64 * r >= i1) break;
-      const unsigned long long hit = __ballot(id[r] == e);
-      if (hit) {   // wave-uniform
-        if (id[r] == e) {
-          const int to = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
-                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
-          p.tokens[to] = tok0 + (int)((x0 + 64u * r) * inv >> 16);
-          p.pos[i + 64 * r + lane] = to;
+      if (i1 - i <= 256 * r) break;
+      unsigned long long hit[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) hit[c] = __ballot(id[r][c] == e);
+      if (hit[0] | hit[1] | hit[2] | hit[3]) {   // wave-uniform
+        int to = at;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          to = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit[c] >> 32),
+                                              __builtin_amdgcn_mbcnt_lo((uint32_t)hit[c], (uint32_t)to));
+          at += (int)__popcll(hit[c]);
         }
-        at += (int)__popcll(hit);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (id[r][c] == e) {
+            p.tokens[to] = tok0 + (int)((x0 + 256u * r + c) * inv >> 16);
+            p.pos[i + 256 * r + 4 * lane + c] = to;
+            ++to;
+          }
       }
     }
     if (e == 0) {   // the pairs of no expert
 #pragma unroll
       for (int r = 0; r < kPlanAhead; ++r)
-        if (i + 64 * r + lane < i1 && (unsigned)id[r] >= (unsigned)E) p.pos[i + 64 * r + lane] = -1;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int left = i1 - i - 256 * r;
+          if (4 * lane + c < left && (unsigned)id[r][c] >= (unsigned)E) p.pos[i + 256 * r + 4 * lane + c] = -1;
+        }
     }
     if (i1 - i <= kRound) break;
   }

@@ -147,6 +147,29 @@ def test_route_ids(hip, T, E, k):
     hip.expert_plan_free(p)
 
 
+@pytest.mark.parametrize("E,k", [(8, 1), (129, 3)])
+def test_plan_edges(hip, E, k):
+    """Pair counts around the plan's loads (4 a lane, 256 a wave, 8 loads ahead, 16 waves),
+    ids on a 4-byte boundary, the arrays' ends left alone."""
+    import torch
+
+    rng = np.random.default_rng(E)
+    for pairs in (129, 255, 256, 257, 4095, 4096, 4097, 4353, 30719, 32767, 32768, 32769, 36865, 70001):
+        T = -(-pairs // k)
+        n = T * k
+        ids = rng.integers(-1, E + 1, (T, k))
+        buf = torch.full((n + 1,), -9, dtype=torch.int32, device="cuda")
+        buf[1:] = torch.tensor(ids.reshape(-1), dtype=torch.int32)
+        out = [torch.full((m + 3,), -77, dtype=torch.int32, device="cuda") for m in (E + 1, n, n)]
+        plan = hip.expert_plan_over(*[o[:-3] for o in out])
+        print(f"plan edges {n} pairs E={E}", flush=True)
+        hip.route_expert_ids(plan, buf[1:], T, k)
+        torch.cuda.synchronize()
+        for o, ref in zip(out, plan_ref(ids, E)):
+            assert np.array_equal(o[:-3].cpu().numpy(), ref)
+            assert (o[-3:] == -77).all()
+
+
 @pytest.mark.parametrize("residual", ["none", "other", "out"])
 @pytest.mark.parametrize("T,k,dim", [(1, 1, 8), (1, 8, 2048), (9, 2, 2056), (5, 16, 5120), (130, 7, 88), (700, 8, 2048)])
 def test_combine(hip, T, k, dim, residual):
