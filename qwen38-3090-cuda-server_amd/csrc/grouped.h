@@ -105,7 +105,7 @@ __device__ __forceinline__ int expert_of(const int* start, int E, int tiles_n, i
 }
 
 // Few rows an expert (grouped_rows.hip): launches it and returns true, or returns false
-// where it does not apply.
-bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, hipStream_t s);
+// where it does not apply or the tiles are faster. form: qw4_tune_grouped's.
+bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s);
 
 }  // namespace qw4

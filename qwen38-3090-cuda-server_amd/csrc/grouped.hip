@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/qwen_w4a16.h"
 #include "gemm_tile.h"
@@ -157,6 +158,8 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
   }
 }
 
+std::atomic<int> g_form{0};   // qw4_tune_grouped
+
 int device_cus() {
   static std::atomic<int> cus[kMaxDevices];
   std::atomic<int>& v = cus[current_device()];
@@ -183,6 +186,12 @@ void launch_tiles(const GroupedArgs& a, hipStream_t s) {
 using namespace qw4;
 
 extern "C" {
+
+int qw4_tune_grouped(int form) {
+  if (form < 0 || form > 4) return QW4_ERR_SHAPE;
+  g_form.store(form, std::memory_order_relaxed);
+  return QW4_OK;
+}
 
 int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x_rows,
                      const qw4_plan* plan, int pairs, int gather, const uint16_t* bias, int act,
@@ -223,7 +232,8 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   a.ld = glu ? n / 2 : n;
   a.tiles_n = (n + G2_BN - 1) / G2_BN;
   const int cus = device_cus();
-  if (grouped_rows_launch(a, glu, cus, (hipStream_t)stream)) {
+  const int form = g_form.load(std::memory_order_relaxed);
+  if (grouped_rows_launch(a, glu, cus, form, (hipStream_t)stream)) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
@@ -234,20 +244,23 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
     a.rexp = h.rexp;
     a.cexp = h.cexp;
   }
-  // 128-row tiles, two workgroups a CU, one's start and end behind the other's products;
-  // or 256-row tiles, one a CU, which cost less a row but waste more where an expert ends
-  // and hide nothing. us (128 / 256): ungated, 16 experts of 768 / 1024 rows in the mean,
-  // skewed, 2048x2048 129 / 125, 159 / 150; 64 of 512, skewed, 2048x1024 159 / 162, even,
-  // 2048x4096 502 / 456; gated, whose epilogue is longer, 64 of 512 even 278 / 297, 16 of
-  // 1536 skewed 241 / 267.
-  const int mb = !glu && (long long)pairs >= 640LL * a.E ? 8 : 4;
+  // 128-row tiles, two workgroups a CU, one's start and end behind the other's products; or
+  // 256-row tiles, one a CU, which cost less a row but waste more where an expert ends, hide
+  // nothing, and need rounds enough not to idle in the last. us (128 / 256), experts, K -> weight
+  // rows, rows an expert: 32, 5120 -> 2048 ungated 768 / 1024 / 1536 511 / 531, 667 / 635, 981 / 915;
+  // 64, 2048 -> 4096 512 / 1024 / 1536 583 / 603, 1106 / 1077, 1636 / 1579; gated 64, 2048 -> 2048
+  // 768 / 1024 / 1536 488 / 525, 569 / 535, 827 / 782; few rounds: 16, 2048 -> 2048 1024 148 / 163, 64,
+  // 2048 -> 1024 768 226 / 253. The gated one has fp16 operands only.
+  const double tiles8 = (pairs / 256. + 0.5 * a.E) * a.tiles_n;
+  const bool high = (long long)pairs >= 900LL * a.E && tiles8 >= 4. * cus && (!glu || a.cexp);
+  const int mb = form == 4 || (form != 3 && high) ? (glu && !a.cexp ? 4 : 8) : 4;
   const int occ = mb == 8 ? 1 : 2;
   const long long most = ((long long)pairs / (32 * mb) + std::min(a.E, pairs)) * a.tiles_n;
   if (most > 0x3fffffffLL) return QW4_ERR_SHAPE;
   a.P = (int)std::min<long long>(most, cus * occ);
   hipStream_t s = (hipStream_t)stream;
   if (mb == 8)
-    launch_tiles<8, 2, 1, false, G2Bf16>(a, s);
+    glu ? launch_tiles<8, 2, 1, true, G2F16>(a, s) : launch_tiles<8, 2, 1, false, G2Bf16>(a, s);
   else if (!glu)
     launch_tiles<4, 2, 2, false, G2Bf16>(a, s);
   else if (a.cexp)

@@ -366,40 +366,51 @@ void launch_rows(const GroupedArgs& a, int MB, int S, hipStream_t st) {
 
 }  // namespace
 
-// Where it is the faster form, by the mean rows of an expert (us, blocks of 16 rows / of 32
-// / the tiles of grouped.hip; experts, K -> weight rows):
-//   64, 2048 -> 2048 gated   24 rows  64 / 59 / 69,     48 rows  89 / 88 / 86
-//   64, 1024 -> 2048         32      41 / 46 / 44,      48       55 / 61 / 45
-//   32, 5120 -> 4352 gated   16      98 / 104 / 147,    32       158 / 140 / 180,   64  289 / 210 / 191
-//   16, 4096 -> 4096         24      41 / 55 / 64,      48       84 / 77 / 79
-//   32, 2176 -> 5120         24      72 / 73 / 74,      32       84 / 84 / 75
-// so up to 40 rows, fewer where the last of a wave's groups are missing (2176 is 17 groups
-// for 8 waves). Blocks of 32 rows read the weights of such experts once, but pay more for
-// every unit: from 20 rows on, where K is long. Beyond 5 groups a wave, whose registers
-// 32 rows do not fit, up to 24 rows.
+// The faster form by the estimated times (us) of this kernel over blocks of 16 rows (in
+// units of two or of four row quads), over blocks of 32 (4 and 5 groups a wave: fewer do
+// not pay, more do not fit the registers) and of the tiles (grouped.hip). R rows in random
+// shares make E (R / (E h) + 1/2) blocks of h rows; a unit costs its groups and its close, a
+// tile its groups by the share of its rows in use (ending ones start at a half) and its
+// start and store, whole rounds of two a CU; the tiles read the weights before they compute.
+// Fitted over 330 shapes (4 to 128 experts, K of 256 to 8192, 192 to 5120 weight rows, 3 to
+// 200 rows an expert); over 400 others it is 1.5% in the geometric mean from the fastest form;
+// by the mean rows of an expert alone (40, or 24 with long K) it was 10%, and up to six times
+// where the tiles are few. E, K -> weight rows, rows an expert: blocks of 16 / of 32 / tiles:
+//   64, 2048 -> 2048 gated   24 rows  63 / 57 / 62,     48 rows  87 / 85 / 76
+//   64, 1024 -> 2048         32      38 / 45 / 45,      48       52 / 58 / 45
+//   32, 5120 -> 4352 gated   16      98 / 101 / 131,    32       152 / 136 / 170,   64  284 / 206 / 183
+//   16, 6144 -> 2048 gated   32      52 / - / 89,       64       83 / - / 91
+//    4, 7808 -> 320          50      18 / - / 108
 //
-// Blocks of 16: units of four row quads, two items ahead, or of two, three ahead, where
-// that leaves the fullest workgroup less. us (4 / 2 quads), 8 of 64 experts: 2048 -> 2 x 1024
-// of 1 / 16 / 64 tokens 7.1 / 21.9 / 30.4, 7.6 / 24.5 / 33.4, 1024 -> 2048 of 16 15.4, 17.5; 4 of 32,
-// 5120 -> 2 x 2176 of 1 token (272 and 544 units on 256 CUs) 15.4, 14.4. Two workgroups a
-// CU were slower throughout (18 to 28 us for 16 tokens).
-bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, hipStream_t s) {
+// Blocks of 16 in units of four row quads, two items ahead, or of two, three ahead: us (4 / 2),
+// 8 of 64 experts: 2048 -> 2 x 1024 of 1 / 16 / 64 tokens 7.1 / 21.9 / 30.4, 7.6 / 24.5 / 33.4;
+// 4 of 32, 5120 -> 2 x 2176 of 1 token (272 and 544 units on 256 CUs) 15.4, 14.4. Two workgroups
+// a CU were slower throughout (18 to 28 us for 16 tokens).
+bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s) {
   const int ng = (a.G + kW - 1) / kW;
-  const double mean = (double)a.R / a.E;
-  if (ng > kMaxGroups || mean > (ng > 5 ? 24. : 40.) * (a.G < kW ? 1. : (double)a.G / (ng * kW))) return false;
-  const int MB = mean > 20 && (ng == 4 || ng == 5) ? 2 : 1;
+  if (ng > kMaxGroups || form > 2 || (form == 2 && ng > 5)) return false;
+  const double E = a.E, mean = a.R / E;
   // experts in use: a token's are different ones; many tokens' as if drawn evenly
-  const double used = 4 * (long long)a.R <= a.E ? a.R : a.E * (1.0 - std::exp(-mean));
-  auto fullest = [&](int S) {   // row quads of the fullest workgroup
-    const double units = used * (a.ld / (16 * (glu ? S / 2 : S)));
-    return std::ceil(units / cus) * S;
+  const double used = 4 * (long long)a.R <= a.E ? a.R : E * (1.0 - std::exp(-mean));
+  auto blocks = [&](int h) { return std::max(used, mean < 1 ? 0. : E * (mean / h + 0.5)); };
+  auto units = [&](int h, int S) {   // of the fullest workgroup
+    return std::ceil(blocks(h) * (a.ld / (16 * (glu ? S / 2 : S))) / cus);
   };
+  auto sixteen = [&](int S) { return 6 + units(16, S) * (0.26 + 0.3 * S * ng); };
+  const double t32 = ng == 4 || ng == 5 ? 16 + units(32, 2) * (0.4 + 0.7 * ng) : 1e30;
+  const int S = sixteen(4) <= sixteen(2) ? 4 : 2;
+  const bool two = form ? form == 2 : t32 < sixteen(S);
+  if (!form) {
+    const double rounds = std::max(1., blocks(128) * a.tiles_n / (2. * cus));
+    const double bytes = used * a.n * a.G * (64 + 2.5);
+    const double tiles = bytes / 5.2e6 + rounds * (10.7 + 1.6 * std::min(1., std::max(0.5, mean / 32)) * a.G);
+    if (tiles < (two ? t32 : sixteen(S))) return false;
+  }
   a.P = cus;
-  const int S = fullest(4) <= fullest(2) ? 4 : 2;
   if (glu)
-    launch_rows<true>(a, MB, S, s);
+    launch_rows<true>(a, two ? 2 : 1, S, s);
   else
-    launch_rows<false>(a, MB, S, s);
+    launch_rows<false>(a, two ? 2 : 1, S, s);
   return true;
 }
 

@@ -52,7 +52,7 @@ EXPORTS = (
     "qw4_w8_gemm_small", "qw4_w8_gemv_argmax",
     "qw4_rmsnorm", "qw4_residual_add", "qw4_swiglu", "qw4_gemv_residual", "qw4_gemv_swiglu",
     "qw4_gemv_rmsnorm", "qw4_linear", "qw4_linear_max_t", "qw4_mfma_peak", "qw4_tune_decode",
-    "qw4_tune_gemm", "qw4_tune_linear", "qw4_gemv_argmax_noalloc",
+    "qw4_tune_gemm", "qw4_tune_linear", "qw4_tune_grouped", "qw4_gemv_argmax_noalloc",
     "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
     "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue", "qw4_gemm_grouped",
     "qw4_epilogue_workspace",
@@ -192,6 +192,7 @@ def lib():
         "qw4_gemv_argmax_noalloc": ([vp, W, vp, i, vp], i),
         "qw4_quantize_w4a16": ([W, vp, i, i, i, vp], i),
         "qw4_tune_linear": ([i], i),
+        "qw4_tune_grouped": ([i], i),
         "qw4_plan_alloc": ([PL, i, i], i),
         "qw4_plan_free": ([PL], i),
         "qw4_route": ([vp, vp, PL, vp, i, i, i, i, vp], i),
@@ -525,6 +526,12 @@ def tune_gemm(schedule: int = -1, variant: int = 0) -> None:
 def tune_linear(max_t: int = 0) -> None:
     """qw4_linear crossover override (qw4_tune_linear), 0 = the measured rule."""
     _chk(lib().qw4_tune_linear(max_t), "tune_linear")
+
+
+def tune_grouped(form: int = 0) -> None:
+    """Override of gemm_grouped_w4a16's kernel (qw4_tune_grouped): 0 the estimated
+    fastest, 1 blocks of 16 rows, 2 of 32, 3 tiles of 128 rows, 4 of 256."""
+    _chk(lib().qw4_tune_grouped(form), "tune_grouped")
 
 
 def linear_max_t(w: W4A16Weights) -> int:

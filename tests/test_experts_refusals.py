@@ -152,6 +152,14 @@ def test_gemm_grouped_refusals(hip):
     assert call(pairs=0, y=None, x=None) == hip.QW4_OK
 
 
+def test_tune_grouped(hip):
+    for form in (-1, 5):
+        with pytest.raises(hip.W4A16Error):
+            hip.tune_grouped(form)
+    hip.tune_grouped(4)
+    hip.tune_grouped()
+
+
 def test_epilogue_workspace(hip):
     w = _weights(hip, out_f=256, in_f=512)
     # x in 16 bits, an exponent a row and a weight row, each from a multiple of 256 bytes

@@ -239,6 +239,7 @@ def test_workspace_sizes(hip, orc):
         "gathered": lambda y, ws: hip.gemm_grouped_w4a16(y, w, x, plan, T, True, act=hip.ACT_SWIGLU, ws=ws),
         "dense": lambda y, ws: hip.linear_epilogue_w4a16(y, w, x, T, None, ws, act=hip.ACT_SWIGLU),
     }
+    hip.tune_grouped(3)   # the tiles, which take them
     for name, call in calls.items():
         width = E * n // 2 if name == "dense" else n // 2
 
@@ -260,4 +261,5 @@ def test_workspace_sizes(hip, orc):
         assert torch.equal(out(base, need - 1), none)
         assert torch.equal(out(base + 128, need), none)
         assert torch.equal(out(base, 0), none)
+    hip.tune_grouped(0)
     hip.awq_free(w)

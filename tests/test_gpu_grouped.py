@@ -98,6 +98,85 @@ def test_grouped(hip, orc, case):
     hip.awq_free(w)
 
 
+@pytest.mark.parametrize("form", [1, 2, 3, 4])
+@pytest.mark.parametrize("case", CASES)
+def test_grouped_forms(hip, orc, case, form):
+    """Every kernel of the call (qw4_tune_grouped) on every case; the two that stream the
+    weights use them exactly, and give the same bits."""
+    import torch
+
+    E, n, K, counts = CASES[case]
+    exact = form == 1 and K <= 8192 or form == 2 and K <= 5120
+    g = torch.Generator().manual_seed(E + n + K)
+    w, wq = make(hip, orc, E * n, K, E + K)
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    R = int(offsets[-1])
+    tokens = torch.randint(0, R + 2, (R + 3,), generator=g).to(torch.int32)
+    ws = hip.gemm_workspace_alloc(hip.epilogue_workspace(w, R + 3))
+    do, dt = i32(offsets), tokens.cuda()
+    plan = hip.expert_plan_over(do, dt, dt)
+    bias = bf(torch.randn(E * n, generator=g))
+    xs = bf(torch.randn(R + 3, K, generator=g) * (8.0 / K ** 0.5))
+    dx, db = xs.cuda(), bias.cuda()
+    try:
+        for act in ("none", "swiglu", "gelu"):
+            width = n // 2 if act == "swiglu" else n
+            for gather in (False, True):
+                rows = xs[tokens[:R].long()] if gather else xs
+                outs = []
+                for f in ((form, 3 - form) if exact and K <= 5120 else (form,)):
+                    print(f"grouped form {f} {case}: {act} gather={gather}", flush=True)
+                    y = torch.full((R + 4, width), 7.0, dtype=torch.bfloat16, device="cuda")
+                    hip.tune_grouped(f)
+                    hip.gemm_grouped_w4a16(y[:R + 3], w, dx, plan, R + 3, gather, bias=db,
+                                           act=getattr(hip, "ACT_" + act.upper()), ws=ws)
+                    torch.cuda.synchronize()
+                    assert (y[R:] == 7.0).all()
+                    outs.append(y.cpu())
+                assert all(torch.equal(o, outs[0]) for o in outs)
+                seen = 0
+                for e in range(E):
+                    lo, hi = int(offsets[e]), int(offsets[e + 1])
+                    if lo == hi or (seen > 20 and hi - lo < 3):
+                        continue
+                    seen += 1
+                    pick = sorted({lo, hi - 1, (lo + hi) // 2, min(lo + 63, hi - 1), min(lo + 64, hi - 1)})
+                    check(outs[0], rows, wq[e * n:(e + 1) * n], bias[e * n:(e + 1) * n], act, None, pick,
+                          rounded=not exact, bits=11 if act == "swiglu" and form > 2 else 8)
+    finally:
+        hip.tune_grouped(0)
+    hip.gemm_workspace_free(ws)
+    hip.awq_free(w)
+
+
+@pytest.mark.parametrize("form", [1, 2, 3, 4])
+def test_grouped_forms_bad_offsets(hip, orc, form):
+    """As below, through every kernel."""
+    import torch
+
+    E, n, K, R = 4, 128, 256, 600
+    w, _ = make(hip, orc, E * n, K, 5)
+    x = bf(torch.randn(R, K)).cuda()
+    ws = hip.gemm_workspace_alloc(hip.epilogue_workspace(w, R))
+    tokens = i32(np.random.default_rng(1).integers(-(1 << 31), (1 << 31) - 1, R))
+    try:
+        hip.tune_grouped(form)
+        for offsets in ([-5, 10, 3, 700, 1 << 30], [600, 500, 40, 30, 20], [0, 0, 0, 0, -1], [1 << 30] * 5,
+                        [-(1 << 31), (1 << 31) - 1, 0, (1 << 31) - 1, 0]):
+            plan = hip.expert_plan_over(i32(offsets), tokens, tokens)
+            for act in (hip.ACT_NONE, hip.ACT_SWIGLU):
+                for gather in (False, True):
+                    print(f"form {form} bad offsets {offsets} {act} {gather}", flush=True)
+                    y = torch.full((R + 2, n // 2 if act else n), 7.0, dtype=torch.bfloat16, device="cuda")
+                    hip.gemm_grouped_w4a16(y[1:R + 1], w, x, plan, R, gather, act=act, ws=ws)
+                    torch.cuda.synchronize()
+                    assert (y[0] == 7.0).all() and (y[R + 1] == 7.0).all()
+    finally:
+        hip.tune_grouped(0)
+    hip.gemm_workspace_free(ws)
+    hip.awq_free(w)
+
+
 def test_grouped_bad_offsets(hip, orc):
     """Offsets that no plan has write no row outside y and read none outside x."""
     import torch
