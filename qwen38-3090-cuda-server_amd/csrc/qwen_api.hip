@@ -292,6 +292,11 @@ void linear_epilogue_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip
         "linear_epilogue_w4a16");
 }
 
+size_t epilogue_workspace(const W4A16Weights& w, int rows) {
+  const qw4_weights v = view(w);
+  return qw4_epilogue_workspace(&v, rows);
+}
+
 void expert_plan_alloc(qw4_plan& plan, int experts, int max_pairs) {
   check(qw4_plan_alloc(&plan, experts, max_pairs), "expert_plan_alloc");
 }
