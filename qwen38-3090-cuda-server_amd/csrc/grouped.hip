@@ -43,7 +43,7 @@ template <int MB, int DD, int OCC, bool GLU, bool GATHER, class Op>
 __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
   // One LDS object for everything: of several, the compiler tells their accesses apart
   // and waits for all loads into one before it reads the next (vmcnt(0) at every k-step;
-  // 32768 rows of 64 experts, 2048 x 2048: 339 us).
+  // 32768 rows of 64 experts, 2048 x 2048: 339 us instead of 258).
   constexpr int kBufs = DD * 32 * MB * 16, kRows = GATHER ? 32 * MB : 0;
   constexpr int kEnds = tile_ends<MB>(), kLists = 1 + kEnds;
   __shared__ u32x4 lds[kBufs + (4 * kRows + kLists * (kMaxExperts + 1 + 4) + 3) / 4];

@@ -383,9 +383,10 @@ void launch_rows(const GroupedArgs& a, int MB, int S, hipStream_t st) {
 //    4, 7808 -> 320          50      18 / - / 108
 //
 // Blocks of 16 in units of four row quads, two items ahead, or of two, three ahead: us (4 / 2),
-// 8 of 64 experts: 2048 -> 2 x 1024 of 1 / 16 / 64 tokens 7.1 / 21.9 / 30.4, 7.6 / 24.5 / 33.4;
-// 4 of 32, 5120 -> 2 x 2176 of 1 token (272 and 544 units on 256 CUs) 15.4, 14.4. Two workgroups
-// a CU were slower throughout (18 to 28 us for 16 tokens).
+// 8 of 64 experts, 2048 -> 2 x 1024, 1 / 16 / 64 tokens 6.1 / 21.2 / 29.3, 6.5 / 23.0 / 30.6; 4 of
+// 32, 5120 -> 2 x 2176, 1 / 8 / 40 tokens (272 and 544 units on 256 CUs at one) 14.6 / 34.6 / 61.6,
+// 13.5 / 33.0 / 62.3; 2 of 8, 8192 -> 1024, 40 tokens 19.7, 24.3. Two workgroups a CU were slower
+// throughout (18 to 28 us for 16 tokens).
 bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s) {
   const int ng = (a.G + kW - 1) / kW;
   if (ng > kMaxGroups || form > 2 || (form == 2 && ng > 5)) return false;
