@@ -104,8 +104,10 @@ __device__ __forceinline__ int expert_of(const int* start, int E, int tiles_n, i
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// Few rows an expert (grouped_rows.hip): launches it and returns true, or returns false
-// where it does not apply or the tiles are faster. form: qw4_tune_grouped's.
+// The kernel for these arguments (qw4_tune_grouped's numbers; 3 for tiles of 128 or 256).
+int grouped_form(const GroupedArgs& a, bool glu, int cus);
+// Forms 1 and 2 (grouped_rows.hip): launches it and returns true, or returns false where it
+// is another or does not apply.
 bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s);
 
 }  // namespace qw4

@@ -179,6 +179,15 @@ void launch_tiles(const GroupedArgs& a, hipStream_t s) {
   a.tokens ? k_grouped_tiles<MB, DD, OCC, GLU, true, Op><<<a.P, 256, 0, s>>>(a)
            : k_grouped_tiles<MB, DD, OCC, GLU, false, Op><<<a.P, 256, 0, s>>>(a);
 }
+template <int MB, int DD>
+void launch_act(const GroupedArgs& a, bool glu, hipStream_t s) {
+  if (!glu)
+    launch_tiles<MB, DD, 2, false, G2Bf16>(a, s);
+  else if (a.cexp)
+    launch_tiles<MB, DD, 2, true, G2F16>(a, s);
+  else
+    launch_tiles<MB, DD, 2, true, G2Bf16>(a, s);
+}
 
 }  // namespace
 }  // namespace qw4
@@ -188,7 +197,7 @@ using namespace qw4;
 extern "C" {
 
 int qw4_tune_grouped(int form) {
-  if (form < 0 || form > 4) return QW4_ERR_SHAPE;
+  if (form < 0 || form > 5) return QW4_ERR_SHAPE;
   g_form.store(form, std::memory_order_relaxed);
   return QW4_OK;
 }
@@ -232,7 +241,8 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   a.ld = glu ? n / 2 : n;
   a.tiles_n = (n + G2_BN - 1) / G2_BN;
   const int cus = device_cus();
-  const int form = g_form.load(std::memory_order_relaxed);
+  const int tuned = g_form.load(std::memory_order_relaxed);
+  const int form = tuned ? tuned : grouped_form(a, glu, cus);
   if (grouped_rows_launch(a, glu, cus, form, (hipStream_t)stream)) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
@@ -244,16 +254,17 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
     a.rexp = h.rexp;
     a.cexp = h.cexp;
   }
-  // 128-row tiles, two workgroups a CU, one's start and end behind the other's products; or
-  // 256-row tiles, one a CU, which cost less a row but waste more where an expert ends, hide
-  // nothing, and need rounds enough not to idle in the last. us (128 / 256), experts, K -> weight
-  // rows, rows an expert: 32, 5120 -> 2048 ungated 768 / 1024 / 1536 511 / 531, 667 / 635, 981 / 915;
-  // 64, 2048 -> 4096 512 / 1024 / 1536 583 / 603, 1106 / 1077, 1636 / 1579; gated 64, 2048 -> 2048
-  // 768 / 1024 / 1536 488 / 525, 569 / 535, 827 / 782; few rounds: 16, 2048 -> 2048 1024 148 / 163, 64,
-  // 2048 -> 1024 768 226 / 253. The gated one has fp16 operands only.
+  // 128-row tiles (64-row ones: grouped_form), two workgroups a CU, one's start and end behind
+  // the other's products; or 256-row tiles, one a CU, which cost less a row but waste more where
+  // an expert ends, hide nothing, and need rounds enough not to idle in the last. us (128 / 256),
+  // experts, K -> weight rows, rows an expert: 32, 5120 -> 2048 ungated 768 / 1024 / 1536
+  // 511 / 531, 667 / 635, 981 / 915; 64, 2048 -> 4096 512 / 1024 / 1536 583 / 603, 1106 / 1077,
+  // 1636 / 1579; gated 64, 2048 -> 2048 768 / 1024 / 1536 488 / 525, 569 / 535, 827 / 782; few
+  // rounds: 16, 2048 -> 2048 1024 148 / 163, 64, 2048 -> 1024 768 226 / 253. The gated one has fp16
+  // operands only.
   const double tiles8 = (pairs / 256. + 0.5 * a.E) * a.tiles_n;
   const bool high = (long long)pairs >= 900LL * a.E && tiles8 >= 4. * cus && (!glu || a.cexp);
-  const int mb = form == 4 || (form != 3 && high) ? (glu && !a.cexp ? 4 : 8) : 4;
+  const int mb = tuned == 4 || (!tuned && high) ? (glu && !a.cexp ? 4 : 8) : form == 5 ? 2 : 4;
   const int occ = mb == 8 ? 1 : 2;
   const long long most = ((long long)pairs / (32 * mb) + std::min(a.E, pairs)) * a.tiles_n;
   if (most > 0x3fffffffLL) return QW4_ERR_SHAPE;
@@ -261,12 +272,10 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   hipStream_t s = (hipStream_t)stream;
   if (mb == 8)
     glu ? launch_tiles<8, 2, 1, true, G2F16>(a, s) : launch_tiles<8, 2, 1, false, G2Bf16>(a, s);
-  else if (!glu)
-    launch_tiles<4, 2, 2, false, G2Bf16>(a, s);
-  else if (a.cexp)
-    launch_tiles<4, 2, 2, true, G2F16>(a, s);
+  else if (mb == 4)
+    launch_act<4, 2>(a, glu, s);
   else
-    launch_tiles<4, 2, 2, true, G2Bf16>(a, s);
+    launch_act<2, 4>(a, glu, s);
   QW4_LAUNCH_CHECK();
   return QW4_OK;
 }

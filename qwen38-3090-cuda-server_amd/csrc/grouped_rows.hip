@@ -364,24 +364,68 @@ void launch_rows(const GroupedArgs& a, int MB, int S, hipStream_t st) {
     launch_ng<GLU, 2, 3>(a, st);
 }
 
+// What the estimates below share: E experts, mean rows of each, experts in use (a token's
+// are different ones; many tokens' as if drawn evenly).
+struct Shares {
+  double E, mean, used;
+  explicit Shares(const GroupedArgs& a) : E(a.E), mean((double)a.R / a.E) {
+    used = 4 * (long long)a.R <= a.E ? a.R : E * (1.0 - std::exp(-mean));
+  }
+  // Blocks of h rows: R rows in random shares make E (R / (E h) + 1/2).
+  double blocks(int h) const { return std::max(used, mean < 1 ? 0. : E * (mean / h + 0.5)); }
+};
+
+// us of blocks of h rows in units of S row quads: a unit of the fullest workgroup costs its
+// groups and its close.
+double rows_us(const GroupedArgs& a, const Shares& sh, bool glu, int cus, int h, int S) {
+  const int ng = (a.G + kW - 1) / kW;
+  const double units = std::max(1., std::ceil(sh.blocks(h) * (a.ld / (16 * (glu ? S / 2 : S))) / cus));
+  return h == 16 ? 6 + units * (0.15 + 0.31 * S * ng) : 24 + units * (0.6 + 0.7 * ng);
+}
+
+// us of tiles of h rows, two a CU at once: a round costs its groups, by the share of the
+// rows in use (ending tiles start at a half), and its start and store; the weights are read
+// before they compute.
+double tiles_us(const GroupedArgs& a, const Shares& sh, int cus, int h) {
+  const double bytes = sh.used * a.n * a.G * (64 + 2.5);
+  const double rounds = std::max(1., sh.blocks(h) * a.tiles_n / (2. * cus));
+  const double share = std::min(1., std::max(0.5, sh.mean / 32));
+  return bytes / 5.4e6 + rounds * (h == 128 ? 15 + 1.7 * share * a.G : 14 + 0.95 * share * a.G);
+}
+
 }  // namespace
 
-// The faster form by the estimated times (us) of this kernel over blocks of 16 rows (in
-// units of two or of four row quads), over blocks of 32 (4 and 5 groups a wave: fewer do
-// not pay, more do not fit the registers) and of the tiles (grouped.hip). R rows in random
-// shares make E (R / (E h) + 1/2) blocks of h rows; a unit costs its groups and its close, a
-// tile its groups by the share of its rows in use (ending ones start at a half) and its
-// start and store, whole rounds of two a CU; the tiles read the weights before they compute.
-// Fitted over 330 shapes (4 to 128 experts, K of 256 to 8192, 192 to 5120 weight rows, 3 to
-// 200 rows an expert); over 400 others it is 1.5% in the geometric mean from the fastest form;
-// by the mean rows of an expert alone (40, or 24 with long K) it was 10%, and up to six times
-// where the tiles are few. E, K -> weight rows, rows an expert: blocks of 16 / of 32 / tiles:
-//   64, 2048 -> 2048 gated   24 rows  63 / 57 / 62,     48 rows  87 / 85 / 76
-//   64, 1024 -> 2048         32      38 / 45 / 45,      48       52 / 58 / 45
-//   32, 5120 -> 4352 gated   16      98 / 101 / 131,    32       152 / 136 / 170,   64  284 / 206 / 183
-//   16, 6144 -> 2048 gated   32      52 / - / 89,       64       83 / - / 91
-//    4, 7808 -> 320          50      18 / - / 108
-//
+// The estimated fastest, as qw4_tune_grouped numbers them (3 for tiles of 256 rows too): blocks
+// of 16 rows, blocks of 32 (4 and 5 groups a wave: fewer do not pay, more do not fit the
+// registers), tiles of 128 rows or of 64. Fitted over 350 shapes (4 to 128 experts, K of 256 to
+// 8192, 192 to 5120 weight rows, 3 to 200 rows an expert); over 400 others 2.0% in the geometric
+// mean from the fastest. By the mean rows of an expert alone (40, or 24 with long K) and without
+// the tiles of 64 rows it was 10%, and up to six times where tiles are few. us, blocks of 16 / of
+// 32 / tiles of 128 / of 64; experts, K -> weight rows, rows an expert:
+//   32, 5120 -> 4352 gated   25 rows  129 / 119 / 165 / 121,    38  169 / 142 / 164 / 126
+//   64, 2048 -> 2048 gated   25       54 / 56 / 50 / 56,        50  90 / 82 / 76 / 59
+//   32, 2176 -> 5120         25       73 / 73 / 74 / 58,        125  287 / 214 / 117 / 134
+//   64, 1024 -> 2048         32       38 / 45 / 45 / -,         48  52 / 58 / 45 / -
+//   16, 6144 -> 2048 gated   32       52 / - / 89 / -
+//    4, 7808 -> 320          50       18 / - / 108 / -
+int grouped_form(const GroupedArgs& a, bool glu, int cus) {
+  const Shares sh(a);
+  const int ng = (a.G + kW - 1) / kW;
+  int form = 3;
+  double best = tiles_us(a, sh, cus, 128);
+  auto consider = [&](int f, double us) {
+    if (us < best) {
+      best = us;
+      form = f;
+    }
+  };
+  consider(5, tiles_us(a, sh, cus, 64));
+  if (ng == 4 || ng == 5) consider(2, rows_us(a, sh, glu, cus, 32, 2));
+  if (ng <= kMaxGroups)
+    consider(1, std::min(rows_us(a, sh, glu, cus, 16, 2), rows_us(a, sh, glu, cus, 16, 4)));
+  return form;
+}
+
 // Blocks of 16 in units of four row quads, two items ahead, or of two, three ahead: us (4 / 2),
 // 8 of 64 experts, 2048 -> 2 x 1024, 1 / 16 / 64 tokens 6.1 / 21.2 / 29.3, 6.5 / 23.0 / 30.6; 4 of
 // 32, 5120 -> 2 x 2176, 1 / 8 / 40 tokens (272 and 544 units on 256 CUs at one) 14.6 / 34.6 / 61.6,
@@ -389,29 +433,14 @@ void launch_rows(const GroupedArgs& a, int MB, int S, hipStream_t st) {
 // throughout (18 to 28 us for 16 tokens).
 bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s) {
   const int ng = (a.G + kW - 1) / kW;
-  if (ng > kMaxGroups || form > 2 || (form == 2 && ng > 5)) return false;
-  const double E = a.E, mean = a.R / E;
-  // experts in use: a token's are different ones; many tokens' as if drawn evenly
-  const double used = 4 * (long long)a.R <= a.E ? a.R : E * (1.0 - std::exp(-mean));
-  auto blocks = [&](int h) { return std::max(used, mean < 1 ? 0. : E * (mean / h + 0.5)); };
-  auto units = [&](int h, int S) {   // of the fullest workgroup
-    return std::ceil(blocks(h) * (a.ld / (16 * (glu ? S / 2 : S))) / cus);
-  };
-  auto sixteen = [&](int S) { return 6 + units(16, S) * (0.26 + 0.3 * S * ng); };
-  const double t32 = ng == 4 || ng == 5 ? 16 + units(32, 2) * (0.4 + 0.7 * ng) : 1e30;
-  const int S = sixteen(4) <= sixteen(2) ? 4 : 2;
-  const bool two = form ? form == 2 : t32 < sixteen(S);
-  if (!form) {
-    const double rounds = std::max(1., blocks(128) * a.tiles_n / (2. * cus));
-    const double bytes = used * a.n * a.G * (64 + 2.5);
-    const double tiles = bytes / 5.2e6 + rounds * (10.7 + 1.6 * std::min(1., std::max(0.5, mean / 32)) * a.G);
-    if (tiles < (two ? t32 : sixteen(S))) return false;
-  }
+  if (form > 2 || ng > (form == 2 ? 5 : kMaxGroups)) return false;
+  const Shares sh(a);
+  const int S = rows_us(a, sh, glu, cus, 16, 4) <= rows_us(a, sh, glu, cus, 16, 2) ? 4 : 2;
   a.P = cus;
   if (glu)
-    launch_rows<true>(a, two ? 2 : 1, S, s);
+    launch_rows<true>(a, form, S, s);
   else
-    launch_rows<false>(a, two ? 2 : 1, S, s);
+    launch_rows<false>(a, form, S, s);
   return true;
 }
 

@@ -530,7 +530,7 @@ def tune_linear(max_t: int = 0) -> None:
 
 def tune_grouped(form: int = 0) -> None:
     """Override of gemm_grouped_w4a16's kernel (qw4_tune_grouped): 0 the estimated
-    fastest, 1 blocks of 16 rows, 2 of 32, 3 tiles of 128 rows, 4 of 256."""
+    fastest, 1 blocks of 16 rows, 2 of 32, 3 tiles of 128 rows, 4 of 256, 5 of 64."""
     _chk(lib().qw4_tune_grouped(form), "tune_grouped")
 
 

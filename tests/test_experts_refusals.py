@@ -153,7 +153,7 @@ def test_gemm_grouped_refusals(hip):
 
 
 def test_tune_grouped(hip):
-    for form in (-1, 5):
+    for form in (-1, 6):
         with pytest.raises(hip.W4A16Error):
             hip.tune_grouped(form)
     hip.tune_grouped(4)

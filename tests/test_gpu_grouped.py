@@ -98,7 +98,7 @@ def test_grouped(hip, orc, case):
     hip.awq_free(w)
 
 
-@pytest.mark.parametrize("form", [1, 2, 3, 4])
+@pytest.mark.parametrize("form", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("case", CASES)
 def test_grouped_forms(hip, orc, case, form):
     """Every kernel of the call (qw4_tune_grouped) on every case; the two that stream the
@@ -149,7 +149,7 @@ def test_grouped_forms(hip, orc, case, form):
     hip.awq_free(w)
 
 
-@pytest.mark.parametrize("form", [1, 2, 3, 4])
+@pytest.mark.parametrize("form", [1, 2, 3, 4, 5])
 def test_grouped_forms_bad_offsets(hip, orc, form):
     """As below, through every kernel."""
     import torch
