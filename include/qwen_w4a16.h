@@ -157,7 +157,8 @@ int qw4_tune_gemm(int schedule, int variant);
 int qw4_tune_linear(int max_t);
 /* qw4_tune_grouped: qw4_gemm_grouped's kernel, 0 the estimated fastest (default); 1
  * blocks of 16 rows with the weights streamed past (in_f up to 8192), 2 blocks of 32 (in_f
- * up to 5120), 3 tiles of 128 rows, 4 of 256 (a gated product: with its workspace), 5 of 64.
+ * up to 5120), 3 tiles of 128 rows, 4 of 256 (a gated product: with its workspace; an ungated
+ * one: weights in bf16), 5 of 64.
  * Where a form does not apply, tiles of 128 rows. */
 int qw4_tune_grouped(int form);
 
@@ -428,11 +429,12 @@ int qw4_route_ids(const qw4_plan* plan, const int32_t* ids, int T, int top_k, vo
  * >= pairs). w holds the experts' weights one after the other (awq_repack_into at row
  * offset e n): out_f = experts n, n % 64 == 0 (QW4_ACT_SWIGLU: n % 128, each expert
  * [gate | up]); width = n, or n / 2. bias [out_f] bf16 may be NULL. fp32 up to the one
- * rounding. Weights are exact where experts have few rows (in_f up to 8192; some tens in the
- * mean, more where experts x n is small); beyond, they are rounded to bf16, or, in a gated
- * product with a 256-byte aligned workspace of qw4_epilogue_workspace(w, rows of x) bytes,
- * to 11 bits.
- * Calls that share a workspace must be stream-ordered. pairs = the T
+ * rounding. Up to as many rows an expert in the mean (pairs / experts) as qw4_linear_max_t
+ * has for a weight of n rows, weights are exact, or, with a 256-byte aligned workspace of
+ * qw4_epilogue_workspace(w, rows of x; pairs without gather) bytes, exact or rounded to 11
+ * bits, whichever is faster (in_f beyond 8192: rounded, to bf16 without that workspace).
+ * Beyond, they are rounded to bf16, as qw4_gemm does, or, in a gated product with that
+ * workspace, to 11 bits. Calls that share a workspace must be stream-ordered. pairs = the T
  * top_k the plan was made for: rows behind offsets[experts] are left as they were,
  * a token outside x counts as zeros. Pointers 16-byte aligned; a gathered x below
  * 4 GiB. ws may be NULL. */

@@ -96,4 +96,8 @@ __device__ __forceinline__ u32x4 add_round8(const float (&v)[8], const u32x4& re
 int gemm_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int M, qw4_workspace* ws,
                   const Epilogue& e, void* stream);
 
+// Rows up to which a product with a weight of out_f rows uses it exactly or, with a
+// workspace, to 11 bits at least (linear.hip; qw4_linear_max_t without its override).
+int exact_rows(int out_f, int in_f);
+
 }  // namespace qw4

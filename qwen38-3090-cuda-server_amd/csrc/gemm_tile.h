@@ -208,7 +208,8 @@ __device__ __forceinline__ bf16x8 g2_deq(uint32_t w, float s, float c) {
 //    value to 2^14 (k_half_rows); exact in fp16 but for what lies 2^-28 (a scale: 2^-20)
 //    below its row's largest. The sums take the exponents back in the epilogue. For gated
 //    products, whose factors each carry the weights' rounding: 0.0027 of the output's
-//    rms in bf16, 0.0017 (the output's own rounding) so.
+//    rms in bf16, 0.0017 (the output's own rounding) so; and for ungated ones by expert
+//    where qw4_linear would use a weight of the expert's size exactly (0.0022, 0.0017).
 struct G2Bf16 {
   static constexpr bool kNorm = false;
   struct Scale {

@@ -104,8 +104,9 @@ __device__ __forceinline__ int expert_of(const int* start, int E, int tiles_n, i
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// The kernel for these arguments (qw4_tune_grouped's numbers; 3 for tiles of 128 or 256).
-int grouped_form(const GroupedArgs& a, bool glu, int cus);
+// The kernel for these arguments (qw4_tune_grouped's numbers; 3 for tiles of 128 or 256),
+// of those alone that use the weights exactly if `exact` is set and they apply.
+int grouped_form(const GroupedArgs& a, bool glu, int cus, bool exact);
 // Forms 1 and 2 (grouped_rows.hip): launches it and returns true, or returns false where it
 // is another or does not apply.
 bool grouped_rows_launch(GroupedArgs& a, bool glu, int cus, int form, hipStream_t s);

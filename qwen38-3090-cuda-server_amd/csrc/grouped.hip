@@ -179,14 +179,13 @@ void launch_tiles(const GroupedArgs& a, hipStream_t s) {
   a.tokens ? k_grouped_tiles<MB, DD, OCC, GLU, true, Op><<<a.P, 256, 0, s>>>(a)
            : k_grouped_tiles<MB, DD, OCC, GLU, false, Op><<<a.P, 256, 0, s>>>(a);
 }
+template <int MB, int DD, class Op>
+void launch_op(const GroupedArgs& a, bool glu, hipStream_t s) {
+  glu ? launch_tiles<MB, DD, 2, true, Op>(a, s) : launch_tiles<MB, DD, 2, false, Op>(a, s);
+}
 template <int MB, int DD>
 void launch_act(const GroupedArgs& a, bool glu, hipStream_t s) {
-  if (!glu)
-    launch_tiles<MB, DD, 2, false, G2Bf16>(a, s);
-  else if (a.cexp)
-    launch_tiles<MB, DD, 2, true, G2F16>(a, s);
-  else
-    launch_tiles<MB, DD, 2, true, G2Bf16>(a, s);
+  a.cexp ? launch_op<MB, DD, G2F16>(a, glu, s) : launch_op<MB, DD, G2Bf16>(a, glu, s);
 }
 
 }  // namespace
@@ -242,13 +241,23 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
   a.tiles_n = (n + G2_BN - 1) / G2_BN;
   const int cus = device_cus();
   const int tuned = g_form.load(std::memory_order_relaxed);
-  const int form = tuned ? tuned : grouped_form(a, glu, cus);
+  // The rounding of the weights follows the sizes and the workspace, not what is faster by
+  // some microseconds: up to the rows an expert where qw4_linear uses a weight of its size
+  // exactly, fp16 operands (11 bits), or without a workspace only the kernels that use it
+  // exactly. Beyond, the ungated tiles take bf16 ones as qw4_gemm does: 0.0022 of the output's
+  // rms from exact against 0.0017, but without k_half_rows (us, fp16 / bf16: 32 experts, 2176 ->
+  // 5120, 125 rows 125 / 116; 64, 1024 -> 2048, 512 rows 182 / 152). Gated, where each factor
+  // carries the rounding (0.0027), they take fp16 ones at any size.
+  const bool few = (long long)pairs <= (long long)a.E * exact_rows(n, w->in_f);
+  const int x_used = gather ? x_rows : pairs;
+  const bool half = (glu || (few && tuned != 4)) && ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 &&
+                    ws->bytes >= half_rows_bytes(x_used, w);
+  const int form = tuned ? tuned : grouped_form(a, glu, cus, few && !half);
   if (grouped_rows_launch(a, glu, cus, form, (hipStream_t)stream)) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
-  const int x_used = gather ? x_rows : pairs;
-  if (glu && ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && ws->bytes >= half_rows_bytes(x_used, w)) {
+  if (half) {
     const HalfRows h = half_rows(ws->buf, x, x_used, w, (hipStream_t)stream);
     a.x = h.x;
     a.rexp = h.rexp;

@@ -408,18 +408,19 @@ double tiles_us(const GroupedArgs& a, const Shares& sh, int cus, int h) {
 //   64, 1024 -> 2048         32       38 / 45 / 45 / -,         48  52 / 58 / 45 / -
 //   16, 6144 -> 2048 gated   32       52 / - / 89 / -
 //    4, 7808 -> 320          50       18 / - / 108 / -
-int grouped_form(const GroupedArgs& a, bool glu, int cus) {
+int grouped_form(const GroupedArgs& a, bool glu, int cus, bool exact) {
   const Shares sh(a);
   const int ng = (a.G + kW - 1) / kW;
+  const bool tiles = !exact || ng > kMaxGroups;
   int form = 3;
-  double best = tiles_us(a, sh, cus, 128);
+  double best = tiles ? tiles_us(a, sh, cus, 128) : HUGE_VAL;
   auto consider = [&](int f, double us) {
     if (us < best) {
       best = us;
       form = f;
     }
   };
-  consider(5, tiles_us(a, sh, cus, 64));
+  if (tiles) consider(5, tiles_us(a, sh, cus, 64));
   if (ng == 4 || ng == 5) consider(2, rows_us(a, sh, glu, cus, 32, 2));
   if (ng <= kMaxGroups)
     consider(1, std::min(rows_us(a, sh, glu, cus, 16, 2), rows_us(a, sh, glu, cus, 16, 4)));

@@ -16,18 +16,9 @@ namespace {
 
 std::atomic<int> g_lin_max_t{0};   // qw4_tune_linear override (0: the rule below)
 
-// Rows up to which skinny passes run instead of the prefill GEMM: they use the
-// weights exactly where the GEMM rounds them to bf16, so this line is not moved
-// with every change of either's speed. 16 whole passes under the ratio that
-// 16-row passes (0.245 us per MB of weights + 5.8 us) and the GEMM (60 us + 0.4
-// us per MB) had on MI355X when it was set: 48 rows for gate|up (93 MB), 64 for
-// down (46 MB), 96 for qkv (19 MB), 112 for o_proj (11 MB).
 int lin_max_t(const qw4_weights* w) {
   const int v = g_lin_max_t.load(std::memory_order_relaxed);
-  if (v > 0) return v;
-  const double mb = (double)w->out_f * w->in_f * (0.5 + 2.5 / 128) / 1e6;
-  const int chunks = (int)((60.0 + 0.4 * mb) / (0.245 * mb + 5.8));
-  return 16 * (chunks < 1 ? 1 : chunks);
+  return v > 0 ? v : qw4::exact_rows(w->out_f, w->in_f);
 }
 
 // T rows of y [T][width] in skinny passes, with the epilogue e or without (null).
@@ -63,6 +54,18 @@ int few_rows(uint16_t* y, int width, const qw4_weights* w, const uint16_t* x, in
 }
 
 }  // namespace
+
+// Rows up to which skinny passes run instead of the prefill GEMM: they use the
+// weights exactly where the GEMM rounds them to bf16, so this line is not moved
+// with every change of either's speed. 16 whole passes under the ratio that
+// 16-row passes (0.245 us per MB of weights + 5.8 us) and the GEMM (60 us + 0.4
+// us per MB) had on MI355X when it was set: 48 rows for gate|up (93 MB), 64 for
+// down (46 MB), 96 for qkv (19 MB), 112 for o_proj (11 MB).
+int qw4::exact_rows(int out_f, int in_f) {
+  const double mb = (double)out_f * in_f * (0.5 + 2.5 / 128) / 1e6;
+  const int chunks = (int)((60.0 + 0.4 * mb) / (0.245 * mb + 5.8));
+  return 16 * (chunks < 1 ? 1 : chunks);
+}
 
 extern "C" {
 
