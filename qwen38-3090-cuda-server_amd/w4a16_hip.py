@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libqwen_w4a16.so")
@@ -236,17 +237,41 @@ def _need(t, nbytes: int, where: str) -> None:
 _torch = None
 
 
-def _buf(t, nbytes: int, where: str) -> int | None:
-    """The address of a buffer of nbytes at least: _need and _ptr in one, 0.1 us less an
-    argument of a call that takes 6 us."""
+# The types that kernels read, once a tensor has come; other types of the same bits.
+_bf16 = _i32 = _f32 = _same = None
+
+
+def _buf(t, dtype, nbytes: int, dev: int, where: str) -> int | None:
+    """The address of a contiguous tensor of this type and at least nbytes on GPU dev, which
+    is what a kernel takes it for; a raw address is trusted."""
     if t is None or type(t) is int:
         return t
     try:
-        if t.nbytes < nbytes:
-            raise ValueError(f"{where}: buffer holds {t.nbytes} bytes, needs {nbytes}")
+        if t.dtype is not dtype or t.nbytes < nbytes or not t.is_contiguous() or t.get_device() != dev:
+            _refuse(t, dtype, nbytes, dev, where)
         return t.data_ptr()
     except AttributeError:
         return int(t)
+
+
+def _types() -> None:
+    global _bf16, _i32, _f32, _same
+    import torch
+
+    _bf16, _i32, _f32 = torch.bfloat16, torch.int32, torch.float32
+    _same = {torch.int16: _bf16, torch.uint16: _bf16, torch.uint32: _i32}
+
+
+def _refuse(t, dtype, nbytes: int, dev: int, where: str) -> None:
+    """Says what is wrong with a tensor, if something is."""
+    if t.dtype is not dtype and _same.get(t.dtype) is not dtype:
+        raise ValueError(f"{where}: type {t.dtype}, needs {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{where}: not contiguous")
+    if t.nbytes < nbytes:
+        raise ValueError(f"{where}: buffer holds {t.nbytes} bytes, needs {nbytes}")
+    if t.get_device() != dev:
+        raise ValueError(f"{where}: not on the current GPU")
 
 
 # torch's calls for the raw handle of a device's current stream and for the current
@@ -267,8 +292,28 @@ def _current_stream() -> int:
     c = _torch._C
     if _torch.cuda.is_initialized() and hasattr(c, "_cuda_getCurrentRawStream"):
         _raw_stream, _device = c._cuda_getCurrentRawStream, c._cuda_getDevice
+        _types()
         return _raw_stream(_device())
     return _torch.cuda.current_stream().cuda_stream
+
+
+def _place(stream) -> tuple:
+    """The current device -- -2, on which no tensor lies, before torch has initialized one --
+    and the raw handle of the stream."""
+    raw = _raw_stream
+    if raw is not None:
+        dev = _device()
+        return dev, raw(dev) if stream is None else _stream(stream)
+    handle = _stream(stream)
+    torch = sys.modules.get("torch")
+    if torch is None:
+        return -2, handle
+    if _same is None:
+        _types()
+    if not torch.cuda.is_initialized():
+        return -2, handle
+    _current_stream()   # keeps torch's calls
+    return torch.cuda.current_device(), handle
 
 
 def _forked() -> None:
@@ -492,14 +537,12 @@ def linear_epilogue_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch | None =
                           ws: GemmWorkspace | None = None, bias=None, act: int = ACT_NONE,
                           residual=None, stream=None) -> None:
     """qw4_linear_epilogue: y = bf16(act(x @ W^T + bias) + residual), one rounding."""
-    width = w.out_f // 2 if act == ACT_SWIGLU else w.out_f
-    _chk(lib().qw4_linear_epilogue(_buf(y, T * width * 2, "linear_epilogue y"), C.byref(w),
-                                   _buf(x, T * w.in_f * 2, "linear_epilogue x"), T,
-                                   _buf(bias, w.out_f * 2, "linear_epilogue bias"), act,
-                                   _buf(residual, T * width * 2, "linear_epilogue residual"),
-                                   C.byref(s) if s is not None else None,
-                                   C.byref(ws) if ws is not None else None, _stream(stream)),
-         "linear_epilogue")
+    width, (dev, to) = w.out_f // 2 if act == ACT_SWIGLU else w.out_f, _place(stream)
+    _chk(lib().qw4_linear_epilogue(_buf(y, _bf16, T * width * 2, dev, "linear_epilogue y"), w,
+                                   _buf(x, _bf16, T * w.in_f * 2, dev, "linear_epilogue x"), T,
+                                   _buf(bias, _bf16, w.out_f * 2, dev, "linear_epilogue bias"), act,
+                                   _buf(residual, _bf16, T * width * 2, dev, "linear_epilogue residual"),
+                                   s, ws, to), "linear_epilogue")
 
 
 def epilogue_workspace(w: W4A16Weights, rows: int) -> int:
@@ -628,12 +671,10 @@ def expert_plan_alloc(experts: int, max_pairs: int) -> ExpertPlan:
 def expert_plan_over(offsets, tokens, pos) -> ExpertPlan:
     """A plan over int32 device tensors of the caller, which keeps them alive:
     offsets [experts + 1], tokens and pos [max_pairs]."""
-    pairs = tokens.numel()
-    _need(pos, pairs * 4, "expert_plan_over pos")
-    for t in (offsets, tokens, pos):
-        if t.element_size() != 4 or not t.is_contiguous():
-            raise ValueError("expert_plan_over: contiguous int32 tensors needed")
-    return ExpertPlan(_ptr(offsets), _ptr(tokens), _ptr(pos), offsets.numel() - 1, pairs)
+    pairs, dev = tokens.numel(), _place(0)[0]
+    return ExpertPlan(_buf(offsets, _i32, 4, dev, "expert_plan_over offsets"),
+                      _buf(tokens, _i32, 0, dev, "expert_plan_over tokens"),
+                      _buf(pos, _i32, pairs * 4, dev, "expert_plan_over pos"), offsets.numel() - 1, pairs)
 
 
 def expert_plan_free(p: ExpertPlan) -> None:
@@ -656,15 +697,17 @@ def route_experts_f32(ids, weights, logits, T: int, experts: int, top_k: int, re
 
 
 def _route(call, size, where, ids, weights, logits, T, experts, top_k, renorm, plan, stream):
-    _chk(call(_buf(ids, T * top_k * 4, where), _buf(weights, T * top_k * 4, where),
-              C.byref(plan) if plan is not None else None, _buf(logits, T * experts * size, where), T,
-              experts, top_k, int(renorm), _stream(stream)), where)
+    pairs, (dev, to) = T * top_k * 4, _place(stream)
+    _chk(call(_buf(ids, _i32, pairs, dev, where), _buf(weights, _f32, pairs, dev, where), plan,
+              _buf(logits, _bf16 if size == 2 else _f32, T * experts * size, dev, where), T, experts, top_k,
+              int(renorm), to), where)
 
 
 def route_expert_ids(plan: ExpertPlan, ids, T: int, top_k: int, stream=None) -> None:
     """qw4_route_ids: the plan of ids [T][top_k] chosen elsewhere."""
-    _chk(lib().qw4_route_ids(C.byref(plan), _buf(ids, T * top_k * 4, "route_expert_ids ids"), T, top_k,
-                             _stream(stream)), "route_expert_ids")
+    dev, to = _place(stream)
+    _chk(lib().qw4_route_ids(plan, _buf(ids, _i32, T * top_k * 4, dev, "route_expert_ids ids"), T, top_k, to),
+         "route_expert_ids")
 
 
 def gemm_grouped_w4a16(y, w: W4A16Weights, x, plan: ExpertPlan, pairs: int, gather: bool,
@@ -675,20 +718,22 @@ def gemm_grouped_w4a16(y, w: W4A16Weights, x, plan: ExpertPlan, pairs: int, gath
     first dimension otherwise)."""
     if x_rows is None:
         x_rows = x.numel() // w.in_f
-    width = w.out_f // max(plan.experts, 1) // (2 if act == ACT_SWIGLU else 1)
-    _chk(lib().qw4_gemm_grouped(_buf(y, pairs * width * 2, "gemm_grouped y"), C.byref(w),
-                                _buf(x, x_rows * w.in_f * 2, "gemm_grouped x"), x_rows, C.byref(plan), pairs,
-                                int(gather), _buf(bias, w.out_f * 2, "gemm_grouped bias"), act,
-                                C.byref(ws) if ws is not None else None, _stream(stream)), "gemm_grouped")
+    width, (dev, to) = w.out_f // max(plan.experts, 1) // (2 if act == ACT_SWIGLU else 1), _place(stream)
+    _chk(lib().qw4_gemm_grouped(_buf(y, _bf16, pairs * width * 2, dev, "gemm_grouped y"), w,
+                                _buf(x, _bf16, x_rows * w.in_f * 2, dev, "gemm_grouped x"), x_rows,
+                                plan, pairs, int(gather),
+                                _buf(bias, _bf16, w.out_f * 2, dev, "gemm_grouped bias"), act,
+                                ws, to), "gemm_grouped")
 
 
 def combine_experts(out, y, weights, T: int, top_k: int, dim: int, plan: ExpertPlan, residual=None,
                     stream=None) -> None:
     """qw4_combine: out = bf16(residual + sum_j weights[t][j] * y[pos of (t, j)])."""
-    _chk(lib().qw4_combine(_buf(out, T * dim * 2, "combine_experts out"),
-                           _buf(y, T * top_k * dim * 2, "combine_experts y"), C.byref(plan),
-                           _buf(weights, T * top_k * 4, "combine_experts weights"), T, top_k, dim,
-                           _buf(residual, T * dim * 2, "combine_experts residual"), _stream(stream)),
+    dev, to = _place(stream)
+    _chk(lib().qw4_combine(_buf(out, _bf16, T * dim * 2, dev, "combine_experts out"),
+                           _buf(y, _bf16, T * top_k * dim * 2, dev, "combine_experts y"), plan,
+                           _buf(weights, _f32, T * top_k * 4, dev, "combine_experts weights"), T, top_k, dim,
+                           _buf(residual, _bf16, T * dim * 2, dev, "combine_experts residual"), to),
          "combine_experts")
 
 
