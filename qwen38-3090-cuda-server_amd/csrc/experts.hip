@@ -444,7 +444,14 @@ void launch_route(const RouteArgs& a, hipStream_t s) {
       k_route_small<T, PER, 16><<<1, 1024, 0, s>>>(a);
     return;
   }
-  if (a.T > 0) k_route<T, PER><<<(a.T + 3) / 4, 256, 0, s>>>(a);
+  launch_rows_of(a.T, 1 << 24, [&](int first, int n) {
+    RouteArgs r = a;
+    r.logits = static_cast<const T*>(a.logits) + (size_t)first * a.E;
+    r.ids += (size_t)first * a.k;
+    r.weights += (size_t)first * a.k;
+    r.T = n;
+    if (n > 0) k_route<T, PER><<<(n + 3) / 4, 256, 0, s>>>(r);
+  });
   if (a.plan.offsets) launch_plan(a.plan, a.ids, a.T * a.k, a.E, a.k, s);
 }
 
@@ -552,8 +559,12 @@ int qw4_combine(uint16_t* out, const uint16_t* y, const qw4_plan* plan, const fl
   if (T == 0) return QW4_OK;
   if (!out || !y || !weights) return QW4_ERR_NULL;
   if (((uintptr_t)out | (uintptr_t)y | (uintptr_t)residual) & 15) return QW4_ERR_ALIGN;
-  k_combine<<<dim3(T, (unsigned)cols), kCombineThreads, 0, (hipStream_t)stream>>>(
-      out, y, plan->pos, weights, residual, (int)pairs, top_k, dim / 8);
+  launch_rows_of(T, 1 << 23, [&](int first, int n) {
+    const size_t at = (size_t)first * dim, pair = (size_t)first * top_k;
+    k_combine<<<dim3(n, (unsigned)cols), kCombineThreads, 0, (hipStream_t)stream>>>(
+        out + at, y, plan->pos + pair, weights + pair, residual ? residual + at : nullptr, (int)pairs, top_k,
+        dim / 8);
+  });
   QW4_LAUNCH_CHECK();
   return QW4_OK;
 }

@@ -1,5 +1,5 @@
 // Operands of the fp16 tile (G2F16, gemm_tile.h): activation rows times a power of two,
-// and the exponents that take it back. One launch: a workgroup a row of x, then
+// and the exponents that take it back. One launch (2^22 rows each): a workgroup a row of x, then
 // workgroups of 256 weight rows, whose largest scale over their groups sets the
 // exponent. Bound by x read and written once (the second reading of a row is cached)
 // and the scales, 1/26 of the weights.
@@ -78,8 +78,12 @@ HalfRows half_rows(void* buf, const uint16_t* x, int T, const qw4_weights* w, hi
   uint16_t* out = reinterpret_cast<uint16_t*>(p);
   int* rexp = reinterpret_cast<int*>(p + align256((size_t)T * w->in_f * 2));
   int* cexp = reinterpret_cast<int*>(reinterpret_cast<char*>(rexp) + align256((size_t)T * 4));
-  k_half_rows<<<T + (w->out_f + kThreads - 1) / kThreads, kThreads, 0, s>>>(
-      out, rexp, cexp, x, T, w->in_f, w->scale, w->out_f, w->num_groups);
+  launch_rows_of(T, 1 << 22, [&](int first, int n) {
+    const size_t at = (size_t)first * w->in_f;
+    const int N = first ? 0 : w->out_f;   // the weight rows once
+    k_half_rows<<<n + (N + kThreads - 1) / kThreads, kThreads, 0, s>>>(
+        out + at, rexp + first, cexp, x + at, n, w->in_f, w->scale, N, w->num_groups);
+  });
   return {out, rexp, cexp};
 }
 

@@ -153,7 +153,19 @@ __device__ __forceinline__ float rmsnorm_f32(uint32_t x, uint32_t w, float inv) 
 // Host-side helpers shared by the C-ABI translation units.
 namespace qw4 {
 void set_hip_error(int e);
+
+// Launches over `rows` rows, f(first, count) for at most `most` at a time: a grid of 2^32
+// threads or more wraps around, and HIP reports no error.
+template <class F>
+void launch_rows_of(int rows, int most, const F& f) {
+  int first = 0;
+  do {
+    const int n = rows - first < most ? rows - first : most;
+    f(first, n);
+    first += n;
+  } while (first < rows);
 }
+}  // namespace qw4
 #define QW4_LAUNCH_CHECK()                                   \
   do {                                                       \
     hipError_t e_ = hipGetLastError();                       \
