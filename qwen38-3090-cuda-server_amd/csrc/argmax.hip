@@ -151,10 +151,14 @@ int qw4_argmax_rows(int32_t* out, const uint16_t* x, int rows, int n, void* stre
   hipStream_t hs = (hipStream_t)stream;
   if (n > 24576 && rows <= 512)
     k_argmax_rows<1024><<<rows, 1024, 0, hs>>>(out, x, n);
-  else if (n > 2048)
-    k_argmax_rows<256><<<rows, 256, 0, hs>>>(out, x, n);
   else
-    k_argmax_rows<64><<<rows, 64, 0, hs>>>(out, x, n);
+    launch_rows_of(rows, 1 << 23, [&](int first, int some) {
+      const uint16_t* const in = x + (size_t)first * n;
+      if (n > 2048)
+        k_argmax_rows<256><<<some, 256, 0, hs>>>(out + first, in, n);
+      else
+        k_argmax_rows<64><<<some, 64, 0, hs>>>(out + first, in, n);
+    });
   QW4_LAUNCH_CHECK();
   return QW4_OK;
 }

@@ -125,14 +125,20 @@ int qw4_rmsnorm(uint16_t* out, const uint16_t* x, const uint16_t* w, int rows, i
   // with four for every row, 16384 rows of 128 / 1024 / 2048 took 25.3 / 28.4 / 30.8 us,
   // 12.0 / 15.7 / 21.7 so.
   hipStream_t hs = (hipStream_t)stream;
-  if (rows <= 512)
+  if (rows <= 512) {
     k_rmsnorm<kNormVThreads, 1><<<rows, kNormVThreads, 0, hs>>>(out, x, w, dim, eps);
-  else if (dim <= 8 * kEwThreads)
-    k_rmsnorm<kEwThreads, 1><<<rows, kEwThreads, 0, hs>>>(out, x, w, dim, eps);
-  else if (dim <= 16 * kEwThreads)
-    k_rmsnorm<kEwThreads, 2><<<rows, kEwThreads, 0, hs>>>(out, x, w, dim, eps);
-  else
-    k_rmsnorm<kEwThreads, 4><<<rows, kEwThreads, 0, hs>>>(out, x, w, dim, eps);
+  } else {
+    launch_rows_of(rows, 1 << 23, [&](int first, int n) {
+      uint16_t* const o = out + (size_t)first * dim;
+      const uint16_t* const in = x + (size_t)first * dim;
+      if (dim <= 8 * kEwThreads)
+        k_rmsnorm<kEwThreads, 1><<<n, kEwThreads, 0, hs>>>(o, in, w, dim, eps);
+      else if (dim <= 16 * kEwThreads)
+        k_rmsnorm<kEwThreads, 2><<<n, kEwThreads, 0, hs>>>(o, in, w, dim, eps);
+      else
+        k_rmsnorm<kEwThreads, 4><<<n, kEwThreads, 0, hs>>>(o, in, w, dim, eps);
+    });
+  }
   QW4_LAUNCH_CHECK();
   return QW4_OK;
 }
