@@ -14,6 +14,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (gfx950) GPU")
 
 
+@pytest.fixture(autouse=True)
+def default_tuning():
+    """The library's tuning overrides are of the process: after each test, also one that
+    failed in between, its own choices hold again."""
+    yield
+    hip = sys.modules.get("w4a16_hip")
+    if hip is not None and hip._lib is not None:
+        hip.tune_decode()
+        hip.tune_gemm()
+        hip.tune_linear()
+        hip.tune_grouped()
+
+
 @pytest.fixture(scope="session")
 def orc():
     import oracle
