@@ -15,9 +15,10 @@ struct Epilogue {
   int up;                 // QW4_ACT_SWIGLU: weight rows from a gate row to its up row
 };
 
-// exp and 1 / x at the hardware's rate, each within about 2^-22: far below the
-// output's rounding, and a third of the code of the exact ones, of which an epilogue
-// holds dozens.
+// exp and 1 / x at the hardware's rate, a third of the code of the exact ones, of which an
+// epilogue holds dozens. exp's argument in powers of two is rounded, so exp is off by
+// |v| 2^-24 (2^-18 at |v| = 80) on top of the instruction's 2^-22: far below the output's
+// rounding, 2^-8.
 __device__ __forceinline__ float fast_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.4426950408889634f); }
 __device__ __forceinline__ float act_silu(float v) {
   return v * __builtin_amdgcn_rcpf(1.f + fast_exp(-v));
@@ -25,7 +26,8 @@ __device__ __forceinline__ float act_silu(float v) {
 
 // v erfc(-v / sqrt 2) / 2: with 1 + erf the terms would cancel for negative v. erfc(z) =
 // t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0, by the Chebyshev fit of Press et al.,
-// Numerical Recipes, section 6.2 (relative error below 1.2e-7).
+// Numerical Recipes, section 6.2 (the fit's relative error is below 1.2e-7; exp adds
+// its argument's rounding, z^2 2^-24).
 __device__ __forceinline__ float act_gelu(float v) {
   const float z = fabsf(v) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.f));

@@ -9,12 +9,13 @@
 #include <type_traits>
 
 #include "../../include/qwen_w4a16.h"
+#include "grouped.h"
 #include "w4a16_common.h"
 
 namespace qw4 {
 namespace {
 
-constexpr int kMaxExperts = 1024;   // 16 logits a lane
+static_assert(kMaxExperts == 1024, "16 logits a lane");
 constexpr int kMaxTopK = 16;        // a row of 16 lanes holds a token's choice
 // Pairs that one workgroup plans: a thread each, whose place among its expert's pairs is
 // counted over all pairs before it (256 pairs: 1.5 us slower than k_plan).

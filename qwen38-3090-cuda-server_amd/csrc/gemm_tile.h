@@ -67,7 +67,7 @@ struct G2Split {
   static constexpr int ACT = 8 * MB / NW;            // 1 KiB (4-row) activation loads per wave and group
   static constexpr int FIXP = (UNITS + 1) / 2;       // fixup blocks per wave region
   // groups buffered: as many 8 MB KiB activation buffers as LDS holds, 4 at most
-  // (MB = 5: three buffers spill 14 VGPRs, 60 bytes a lane, and are still faster
+  // (MB = 5: three buffers spill 17 VGPRs, 72 bytes a lane, and are still faster
   // than two without a spill: whole tiles 3%, split-K 1%, the others equal)
   static constexpr int DEPTH = DD ? DD : MB <= 4 ? 4 : MB == 5 ? 3 : 2;
   // k-step schedule (measured on MI355X at the config-4 shapes): VALU slots

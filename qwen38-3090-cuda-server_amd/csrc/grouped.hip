@@ -160,20 +160,6 @@ __global__ __launch_bounds__(256, OCC) void k_grouped_tiles(GroupedArgs a) {
 
 std::atomic<int> g_form{0};   // qw4_tune_grouped
 
-int device_cus() {
-  static std::atomic<int> cus[kMaxDevices];
-  std::atomic<int>& v = cus[current_device()];
-  int n = v.load(std::memory_order_relaxed);
-  if (!n) {
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-      n = 256;
-    v.store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 template <int MB, int DD, int OCC, bool GLU, class Op>
 void launch_tiles(const GroupedArgs& a, hipStream_t s) {
   a.tokens ? k_grouped_tiles<MB, DD, OCC, GLU, true, Op><<<a.P, 256, 0, s>>>(a)

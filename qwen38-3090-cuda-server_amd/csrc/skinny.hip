@@ -1058,19 +1058,6 @@ __global__ __launch_bounds__(64 * W) void k_dec(SkinnyArgs a) {
 // Per-device caches are filled once per device under std::call_once, or are
 // atomics whose racing writers store the same value; no launch reads the
 // environment.
-int device_cus() {
-  static std::once_flag once[kMaxDevices];
-  static int cus[kMaxDevices];
-  const int dev = current_device();
-  std::call_once(once[dev], [dev] {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        n <= 0)
-      n = 256;
-    cus[dev] = n;
-  });
-  return cus[dev];
-}
 
 // Tuning and test override of the skinny launch (qw4_tune_decode); all zero =
 // the measured policy.
