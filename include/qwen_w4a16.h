@@ -380,8 +380,8 @@ enum {
 int qw4_linear_epilogue(uint16_t* y, const qw4_weights* w, const uint16_t* x, int T,
                         const uint16_t* bias, int act, const uint16_t* residual, qw4_scratch* s,
                         qw4_workspace* ws, void* stream);
-/* Bytes of a workspace that a gated product over `rows` rows of x takes (x in 16 bits
- * and the rows' exponents). qw4_linear_epilogue also splits tiles as qw4_gemm does when
+/* Bytes of a workspace that a gated product, or one by expert, over `rows` rows of x takes
+ * (x in 16 bits and the rows' exponents). qw4_linear_epilogue also splits tiles as qw4_gemm does when
  * the workspace holds that on top. 0 for bad arguments. */
 size_t qw4_epilogue_workspace(const qw4_weights* w, int rows);
 

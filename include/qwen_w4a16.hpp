@@ -167,7 +167,8 @@ void linear_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16
 void linear_epilogue_w4a16(__hip_bfloat16* y, const W4A16Weights& w, const __hip_bfloat16* x, int T,
                            const __hip_bfloat16* bias, int act, const __hip_bfloat16* residual,
                            GemvScratch& s, GemmWorkspace& ws, hipStream_t stream = 0);
-// Workspace bytes of a gated product over `rows` rows of x (qw4_epilogue_workspace).
+// Workspace bytes of a gated product, or one by expert, over `rows` rows of x
+// (qw4_epilogue_workspace).
 size_t epilogue_workspace(const W4A16Weights& w, int rows);
 
 // Layers of experts (no reference counterpart; qwen_w4a16.h describes the plan).

@@ -546,7 +546,8 @@ def linear_epilogue_w4a16(y, w: W4A16Weights, x, T: int, s: GemvScratch | None =
 
 
 def epilogue_workspace(w: W4A16Weights, rows: int) -> int:
-    """qw4_epilogue_workspace: workspace bytes of a gated product over `rows` rows of x."""
+    """qw4_epilogue_workspace: workspace bytes of a gated product, or one by expert, over
+    `rows` rows of x."""
     return lib().qw4_epilogue_workspace(C.byref(w), rows)
 
 
