@@ -271,7 +271,7 @@ def _refuse(t, dtype, nbytes: int, dev: int, where: str) -> None:
     if t.nbytes < nbytes:
         raise ValueError(f"{where}: buffer holds {t.nbytes} bytes, needs {nbytes}")
     if t.get_device() != dev:
-        raise ValueError(f"{where}: not on the current GPU")
+        raise ValueError(f"{where}: not on the call's GPU")
 
 
 # torch's calls for the raw handle of a device's current stream and for the current
@@ -672,7 +672,9 @@ def expert_plan_alloc(experts: int, max_pairs: int) -> ExpertPlan:
 def expert_plan_over(offsets, tokens, pos) -> ExpertPlan:
     """A plan over int32 device tensors of the caller, which keeps them alive:
     offsets [experts + 1], tokens and pos [max_pairs]."""
-    pairs, dev = tokens.numel(), _place(0)[0]
+    if _same is None:
+        _types()
+    pairs, dev = tokens.numel(), max(offsets.get_device(), 0)   # all on one GPU, the current one or not
     return ExpertPlan(_buf(offsets, _i32, 4, dev, "expert_plan_over offsets"),
                       _buf(tokens, _i32, 0, dev, "expert_plan_over tokens"),
                       _buf(pos, _i32, pairs * 4, dev, "expert_plan_over pos"), offsets.numel() - 1, pairs)

@@ -72,7 +72,7 @@ ALL = [(c, a) for c, n in (("linear_epilogue", ("y", "x", "bias", "residual")), 
 def test_refused(hip, name, arg):
     call, args = calls(hip)[name]
     # the other arguments: raw addresses, which are trusted (the plan takes tensors alone)
-    here = hip._place(0)[0]
+    here = hip._place(0)[0] if name != "plan" else 0
     rest = {a: 0x10000 if name != "plan" else On(s, d, here) for a, (s, d) in args.items()}
     shape, dtype = args[arg]
     wrong = {BF: (F32, torch.float16, torch.uint8), F32: (BF, torch.float64, I32), I32: (torch.int64, F32, torch.int16)}
@@ -107,3 +107,13 @@ def test_sixteen_bit_views(hip):
     call, args = calls(hip)["linear_epilogue"]
     with pytest.raises(ValueError, match="GPU"):   # past the type
         call(**{**{a: 0x10000 for a in args}, "x": torch.empty((T, K), dtype=torch.int16)})
+
+
+def test_plan_of_another_gpu(hip):
+    """A plan's arrays lie on one GPU, which need not be the current one yet."""
+    _, args = calls(hip)["plan"]
+    on = {a: On(s, d, 1) for a, (s, d) in args.items()}
+    p = hip.expert_plan_over(**on)
+    assert (p.offsets, p.tokens, p.pos, p.experts, p.max_pairs) == (0x10000, 0x10000, 0x10000, E, T * TOP)
+    with pytest.raises(ValueError, match="GPU"):
+        hip.expert_plan_over(**{**on, "pos": On(*args["pos"], 0)})
