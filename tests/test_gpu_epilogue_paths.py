@@ -77,7 +77,7 @@ def check_columns(y, x, W, cols, up, bias, act, residual):
 
 # weight rows, K, rows of x
 SHAPES = [(9472, 640, (1, 2, 9, 16, 17, 32)), (34816, 5120, (1, 2, 9, 16, 17, 32)), (5120, 17408, (1, 2, 9, 16)),
-          (24576, 8448, (1, 9, 16)), (65536, 128, (1, 3)), (131072, 256, (1, 2)), (524288, 128, (1, 2)), (20480, 2048, (1, 5, 24))]
+          (24576, 8448, (1, 9, 16)), (65536, 128, (1, 3)), (131072, 256, (1, 2)), (524288, 128, (1, 2)), (1024, 65536, (1, 2, 9)), (256, 131072, (1, 16)), (20480, 2048, (1, 5, 24))]
 
 
 @pytest.mark.parametrize("act", ["swiglu", "gelu", "none"])
@@ -89,7 +89,8 @@ def test_paths(hip, N, K, rows, act):
     g = torch.Generator().manual_seed(N)
     cols = torch.randperm(width, generator=g)[:1200]
     edges = torch.arange(0, width, width // 16)
-    cols = torch.unique(torch.cat([cols, edges, edges + 63, torch.tensor([width - 64, width - 1])])).cuda()
+    edges = torch.cat([edges, (edges + 63).clamp(max=width - 1), torch.tensor([width - 64, width - 1])])
+    cols = torch.unique(torch.cat([cols, edges])).cuda()
     for T in rows:
         assert T <= hip.linear_max_t(W.w)
         x = bf(torch.randn(T, K, generator=g) * (8.0 / K ** 0.5))
