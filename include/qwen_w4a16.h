@@ -449,6 +449,75 @@ int qw4_gemm_grouped(uint16_t* y, const qw4_weights* w, const uint16_t* x, int x
 int qw4_combine(uint16_t* out, const uint16_t* y, const qw4_plan* plan, const float* weights, int T,
                 int top_k, int dim, const uint16_t* residual, void* stream);
 
+/* ------------------------------------------------- activations in 8 bits
+ * Rows of activations as int8 codes with a scale for each group of 128 inputs, and the
+ * products that read them (no reference counterpart: its activations stay bf16). A
+ * value is q scale, scale = (largest |value| of the group) / 127, q = its nearest
+ * integer in [-127, 127].
+ *   q      [max_rows][in_f]; input 8 w + e of a chunk of 32 (w, e = 0..3, 0..7) lies at
+ *          byte 4 w + {0, 2, -, -, 1, 3, -, -}[e] or 16 + 4 w + {-, -, 0, 2, -, -, 1, 3}[e]
+ *          of the chunk: the order in which the nibbles of a packed weight word meet it
+ *   scale  [in_f / 128][max_rows] fp32
+ * A group with Inf or NaN gets a NaN scale (and codes 0): its row's products are NaN.
+ * Values whose group's largest is below 2^-100 count as zeros (scale 0). */
+typedef struct qw4_a8 {
+  int8_t* q;
+  float* scale;
+  int32_t max_rows, in_f;
+} qw4_a8;
+
+/* Device arrays for max_rows (>= 1) rows of in_f (% 128 == 0) inputs. A caller may also
+ * fill the struct with arrays of its own (q 16-byte aligned). */
+int qw4_a8_alloc(qw4_a8* a, int max_rows, int in_f);
+int qw4_a8_free(qw4_a8* a);
+/* The first T (0 <= T <= max_rows) rows of a from bf16 rows x[t] at x + t ld (ld >= in_f
+ * elements, % 8 == 0; x 16-byte aligned). */
+int qw4_a8_quantize(const qw4_a8* a, const uint16_t* x, int ld, int T, void* stream);
+/* The residual's addition and the norm before a projection in one pass: h_out [T][in_f] =
+ * bf16(h + residual), and a = h_out rsqrt(mean(h_out^2) + eps) (1 + w) in 8 bits (fp32
+ * up to that rounding; qw4_rmsnorm's sums). residual may be NULL: then h is normed as
+ * it is and h_out is not written (and may be NULL). h_out may be h or residual. Data
+ * 16-byte aligned. */
+int qw4_a8_rmsnorm(const qw4_a8* a, uint16_t* h_out, const uint16_t* h, const uint16_t* residual,
+                   const uint16_t* w, int T, float eps, void* stream);
+/* dst [nrows][in_f] bf16 = RNE(q scale) of rows row0.. (the 8-bit rows' counterpart of
+ * qw4_dequant_rows). dst 16-byte aligned. */
+int qw4_a8_dequant_rows(uint16_t* dst, const qw4_a8* a, int row0, int nrows, void* stream);
+
+/* qw4_linear_epilogue over rows in 8 bits: y [T][width] = bf16(act(x @ W^T + bias) +
+ * residual), x the first T >= 1 rows of a (a->in_f == w->in_f). Integer products, exact
+ * within a group (weights are not rounded); fp32 from there to the one rounding. A
+ * workspace (may be NULL; 256-byte aligned) lets tiles be split along in_f when there are
+ * too few to fill the GPU; calls that share one must be stream-ordered. Scales of a count
+ * to 22 bits. y, bias and residual 16-byte aligned; residual may be y. */
+int qw4_a8_linear(uint16_t* y, const qw4_weights* w, const qw4_a8* a, int T, const uint16_t* bias,
+                  int act, const uint16_t* residual, qw4_workspace* ws, void* stream);
+/* The same without an epilogue, y [T][out_f] in fp32: logits. */
+int qw4_a8_linear_f32(float* y, const qw4_weights* w, const qw4_a8* a, int T, qw4_workspace* ws,
+                      void* stream);
+
+/* ------------------------------------------------------ log probabilities
+ * Of T rows of logits x[t][0..n) (row t at x + t ld elements, ld >= n; any n >= 1 and any
+ * alignment of the type), with L = log(sum_i exp x[t][i]):
+ *   lp [T][asked]       x[t][targets[t][j]] - L; 0 where the target is outside [0, n)
+ *   entropy [T]         -sum p log p, p = exp(x - L); may be NULL
+ *   top_ids, top_lp [T][top_k]   the top_k (0..32) largest, largest first, the lower index
+ *                       among equals, and x - L of each; both NULL with top_k = 0
+ * asked >= 0 targets a row (lp and targets NULL with 0). In fp32. -Inf is a masked token:
+ * never chosen (id -1, -Inf, also behind the last that there is), lp -Inf; a row of
+ * nothing else has entropy 0. NaN or +Inf in a row make its numbers NaN (ids still go by
+ * the other logits; NaN is never chosen). The reference has only argmax over rows
+ * (src/kernels/elementwise.cuh:34-43). ws: at least qw4_logprobs_workspace bytes, 16-byte
+ * aligned (may be NULL when that is 0); calls that share one must be stream-ordered. */
+int qw4_logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const uint16_t* logits,
+                 size_t ld, const int32_t* targets, int T, int n, int asked, int top_k,
+                 qw4_workspace* ws, void* stream);
+int qw4_logprobs_f32(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const float* logits,
+                     size_t ld, const int32_t* targets, int T, int n, int asked, int top_k,
+                     qw4_workspace* ws, void* stream);
+/* Bytes of workspace for such a call; 0 for bad arguments. */
+size_t qw4_logprobs_workspace(int T, int n, int top_k);
+
 /* ------------------------------------------------- synthetic inputs
  * Device-side generator for the benchmark (no reference counterpart). The
  * counter-based spec is documented with the generator kernel:

@@ -1,0 +1,470 @@
+// Log probabilities of given tokens, entropy and top alternatives of rows of logits, in
+// one pass over each row.
+//
+// A wave streams blocks of 512 logits, 8 a lane, and keeps
+//   m       the largest so far (the same in all lanes),
+//   s       per lane, sum of exp(x - m) without the one element that is m (`own`: it was
+//           this lane's),
+//   u       per lane, sum of exp(x - m) (x - m),
+//   a list  the top_k best (value, index) so far, lane j the j-th.
+// With total = 1 + s:  L = m + log1p(s),  H = log1p(s) - u / (1 + s). Without the
+// largest element s keeps its relative precision when that token is all but certain,
+// where 1 + s would lose it and both results are about s.
+// A block whose largest value beats neither m nor the list's last entry, which is nearly
+// every one after the first few, costs one comparison a lane for all of that.
+// Rows split over workgroups, for few rows, write (m, s, u, list) to the workspace and
+// a second kernel joins them in order; nothing depends on which workgroup comes first.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "../../include/qwen_w4a16.h"
+#include "w4a16_common.h"
+
+namespace qw4 {
+namespace {
+
+constexpr int kLpMaxTop = 32;
+constexpr int kLpWaves = 4;
+constexpr int kLpBlock = 512;    // logits of a wave's block
+constexpr int kLpAhead = 4;      // blocks in flight
+constexpr int kLpFew = 12;       // entries put into a list one by one
+
+struct LpArgs {
+  const void* x;
+  size_t ld;
+  const int32_t* targets;
+  float *lp, *entropy, *top_lp;
+  int32_t* top_ids;
+  int n, asked, k, S;
+  uint32_t* part;      // [T][S] records of 4 + 2 k words
+};
+
+struct LpStats {
+  float m, s, u;       // s, u: of the whole wave once joined
+};
+
+__device__ __forceinline__ float lane_value(float v, int l) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return lane_value(v, 0);
+}
+// exp(d), d <= 0; its argument's rounding, |d| 2^-24, is the d's own.
+__device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.4426950408889634f); }
+// A difference to multiply with: e^-10000 is 0, and 0 times it stays 0.
+__device__ __forceinline__ float lp_far(float d) { return fmaxf(d, -10000.f); }
+
+// The sums of reference m (own of them the element m itself, 0 or 1) under reference to >= m.
+__device__ __forceinline__ void lp_rescale(float& s, float& u, float own, float m, float to) {
+  const float d = lp_far(m - to), c = lp_exp(d), all = s + own;
+  u = c * (u + d * all);
+  s = c * all;
+}
+
+// A larger value, then a lower index, comes first; -Inf (no token) last.
+__device__ __forceinline__ bool lp_first(float v, int i, float w, int j) {
+  return v > w || (v == w && (unsigned)i < (unsigned)j);
+}
+
+// The best of what a wave has seen, lane j the j-th of 64.
+struct LpList {
+  float v = -INFINITY;
+  int i = -1;
+
+  // One step of a bitonic network: a lane and its partner `stride` off keep the first
+  // (upper) or the other of their two entries.
+  __device__ __forceinline__ void exchange(int stride, bool upper) {
+    const float w = __shfl_xor(v, stride, 64);
+    const int j = __shfl_xor(i, stride, 64);
+    if (lp_first(v, i, w, j) != upper) {
+      v = w;
+      i = j;
+    }
+  }
+  __device__ __forceinline__ void settle(int lane) {   // sorts a bitonic sequence
+#pragma unroll
+    for (int stride = 32; stride > 0; stride >>= 1) exchange(stride, (lane & stride) == 0);
+  }
+  __device__ __forceinline__ void sort(int lane) {
+#pragma unroll
+    for (int size = 2; size < 64; size <<= 1)
+#pragma unroll
+      for (int stride = size >> 1; stride > 0; stride >>= 1)
+        exchange(stride, ((lane & size) == 0) == ((lane & stride) == 0));
+    settle(lane);
+  }
+  // The best 64 of this sorted list and another.
+  __device__ __forceinline__ void merge(const LpList& o, int lane) {
+    const float w = __shfl(o.v, 63 - lane, 64);
+    const int j = __shfl(o.i, 63 - lane, 64);
+    if (lp_first(w, j, v, i)) {
+      v = w;
+      i = j;
+    }
+    settle(lane);
+  }
+  // One entry (the same in all lanes) into its place.
+  __device__ __forceinline__ void insert(float x, int at, int lane) {
+    const int c = __popcll(__ballot(lp_first(v, i, x, at)));
+    // wave_shr:1, the lane below's
+    const float pv = __uint_as_float(
+        (uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x138, 0xf, 0xf, false));
+    const int pi = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xf, 0xf, false);
+    if (lane >= c) {
+      v = lane == c ? x : pv;
+      i = lane == c ? at : pi;
+    }
+  }
+};
+
+struct LpSlot {
+  float v;
+  int i;
+};
+
+template <bool TOP>
+struct LpWave {
+  float m = -INFINITY;
+  float s = 0.f, u = 0.f, own = 0.f;
+  LpList list;
+  float last = -INFINITY;   // the list's k-th value, which a later element has to beat
+  int last_i = -1;
+
+  // Elements x[e] with indices at(e), rising with e and over a wave's calls; -Inf where
+  // there is none.
+  template <int N, class At>
+  __device__ __forceinline__ void take(const float (&x)[N], const At& at, int k, int lane, LpSlot* slots) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
+    if (__ballot(top > (TOP ? last : m))) {
+      if (TOP) choose(x, at, k, lane, top, slots);
+      if (__ballot(top > m)) {
+        const float to = wave_max(top);
+        lp_rescale(s, u, own, m, to);
+        m = to;
+        bool mine = lane == __builtin_ctzll(__ballot(top == to));
+        own = mine ? 1.f : 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float d = x[e] - m, p = lp_exp(d);
+          if (mine && x[e] == to) {
+            mine = false;   // m itself stays out of s
+          } else {
+            s += p;
+            u = __builtin_fmaf(p, lp_far(d), u);
+          }
+        }
+        return;
+      }
+    }
+    const float ref = m > -INFINITY ? m : 0.f;   // nothing but -Inf so far: they add nothing
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = x[e] - ref, p = lp_exp(d);
+      s += p;
+      u = __builtin_fmaf(p, lp_far(d), u);
+    }
+  }
+
+  // The block's elements into the list. While that is empty, only those from the k-th
+  // largest of the lanes' own largest on: at least k are, and few more. Many at once are
+  // gathered and sorted (27 steps of a network), a few put in one by one.
+  template <int N, class At>
+  __device__ __forceinline__ void choose(const float (&x)[N], const At& at, int k, int lane, float top,
+                                         LpSlot* slots) {
+    float least = -INFINITY;
+    if (lane_value(list.v, 0) == -INFINITY) {
+      int rank = 0;
+      for (int l = 0; l < 64; ++l) {
+        const float o = lane_value(top, l);
+        rank += o > top || (o == top && l < lane);
+      }
+      least = wave_max(rank == k - 1 ? top : -INFINITY);
+    }
+    auto wanted = [&](float v, int i) { return v >= least && v > -INFINITY && lp_first(v, i, last, last_i); };
+    int count = 0, mine[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const unsigned long long some = __ballot(wanted(x[e], at(e)));
+      mine[e] = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+      count += __popcll(some);
+    }
+    if (count > kLpFew && count <= 64) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (wanted(x[e], at(e))) slots[mine[e]] = {x[e], at(e)};
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      LpList more;
+      if (lane < count) {
+        more.v = slots[lane].v;
+        more.i = slots[lane].i;
+      }
+      __builtin_amdgcn_wave_barrier();
+      more.sort(lane);
+      list.merge(more, lane);
+      last = lane_value(list.v, k - 1);
+      last_i = __builtin_amdgcn_readlane(list.i, k - 1);
+      return;
+    }
+    uint32_t done = 0;   // elements of this lane that are in the list
+    for (;;) {
+      float b = -INFINITY;
+      int bi = -1, be = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (!(done >> e & 1) && x[e] > b) {
+          b = x[e];
+          bi = at(e);
+          be = e;
+        }
+      const unsigned long long some = __ballot(wanted(b, bi));
+      if (!some) break;
+      const int from = __builtin_ctzll(some);
+      list.insert(lane_value(b, from), __builtin_amdgcn_readlane(bi, from), lane);
+      last = lane_value(list.v, k - 1);
+      last_i = __builtin_amdgcn_readlane(list.i, k - 1);
+      if (lane == from) done |= 1u << be;
+    }
+  }
+
+  __device__ __forceinline__ LpStats stats() const { return {m, wave_sum(s), wave_sum(u)}; }
+};
+
+// The statistics of two disjoint sets: the largest of both stays out of s once.
+__device__ __forceinline__ LpStats lp_join(LpStats a, LpStats b) {
+  if (b.m > a.m) {
+    const LpStats t = a;
+    a = b;
+    b = t;
+  }
+  lp_rescale(b.s, b.u, b.m > -INFINITY ? 1.f : 0.f, b.m, a.m);
+  return {a.m, a.s + b.s, a.u + b.u};
+}
+
+template <class T>
+__device__ __forceinline__ float lp_logit(const T* p) {
+  if constexpr (std::is_same_v<T, float>)
+    return *p;
+  else
+    return bf16_bits_to_f32(*p);
+}
+
+// A row's results from its statistics and list, by one wave.
+template <class T>
+__device__ __forceinline__ void lp_write(const LpArgs& a, int row, LpStats t, const LpList& list, int lane) {
+  const bool some = t.m > -INFINITY;
+  if (t.m == INFINITY) t.s = __builtin_nanf("");
+  const float log = some ? log1pf(t.s) : t.s;   // of a row without any: 0, or NaN
+  if (lane == 0 && a.entropy) a.entropy[row] = some ? log - t.u / (1.f + t.s) : log;
+  auto lp = [&](float x) { return (some ? x - t.m : -INFINITY) - log; };
+  const T* xr = static_cast<const T*>(a.x) + (size_t)row * a.ld;
+  for (int j = lane; j < a.asked; j += 64) {
+    const size_t at = (size_t)row * a.asked + j;
+    const int i = a.targets[at];
+    a.lp[at] = (unsigned)i < (unsigned)a.n ? lp(lp_logit(xr + i)) : 0.f;
+  }
+  if (lane < a.k) {
+    a.top_ids[(size_t)row * a.k + lane] = list.i;
+    a.top_lp[(size_t)row * a.k + lane] = lp(list.v);
+  }
+}
+
+// Workgroup (row, split): blocks split 4 W + wave, + 4 W S ...
+template <class T, bool TOP>
+__global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
+  constexpr int kVec = 16 / sizeof(T);          // logits of 16 bytes
+  constexpr int kParts = kLpBlock / 64 / kVec;  // 16-byte loads of a block
+  __shared__ LpSlot slots[kLpWaves][64];
+  __shared__ LpStats parts[kLpWaves];
+  const int row = blockIdx.x / a.S, split = blockIdx.x - row * a.S;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const T* xr = static_cast<const T*>(a.x) + (size_t)row * a.ld;
+  // logits before the first 16-byte boundary and behind the last
+  const int head = min(a.n, (int)((0u - (uint32_t)(uintptr_t)xr) % 16u / sizeof(T)));
+  const u32x4* xv = reinterpret_cast<const u32x4*>(xr + head);
+  const int vecs = (a.n - head) / kVec, tail = head + vecs * kVec;
+  const int blocks = (vecs + 64 * kParts - 1) / (64 * kParts);
+  LpWave<TOP> w;
+  auto few = [&](int first, int count) {   // < 8 logits one by one
+    const float x[1] = {lane < count ? lp_logit(xr + first + lane) : -INFINITY};
+    w.take(x, [&](int) { return first + lane; }, a.k, lane, slots[wave]);
+  };
+  const bool ends = split == 0 && wave == 0;
+  if (ends && head) few(0, head);
+  const int step = kLpWaves * a.S;
+  for (int b0 = split * kLpWaves + wave; b0 < blocks; b0 += kLpAhead * step) {
+    u32x4 v[kLpAhead][kParts];
+#pragma unroll
+    for (int d = 0; d < kLpAhead; ++d)
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        const long long i = ((long long)(b0 + d * step) * kParts + p) * 64 + lane;
+        v[d][p] = xv[i < vecs ? i : 0];
+      }
+#pragma unroll
+    for (int d = 0; d < kLpAhead; ++d) {
+      const int b = b0 + d * step;
+      if (b >= blocks) break;
+      float x[8];
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        const bool in = (b * kParts + p) * 64 + lane < vecs;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if constexpr (sizeof(T) == 4) {
+            x[p * 4 + c] = in ? __uint_as_float(v[d][p][c]) : -INFINITY;
+          } else {
+            x[2 * c] = in ? bf16_bits_to_f32(v[d][p][c] & 0xffffu) : -INFINITY;
+            x[2 * c + 1] = in ? bf16_bits_to_f32(v[d][p][c] >> 16) : -INFINITY;
+          }
+      }
+      w.take(x, [&](int e) { return head + ((b * kParts + e / kVec) * 64 + lane) * kVec + e % kVec; }, a.k, lane,
+             slots[wave]);
+    }
+  }
+  if (ends && tail < a.n) few(tail, a.n - tail);
+  const LpStats mine = w.stats();
+  if (lane == 0) parts[wave] = mine;
+  if (TOP) slots[wave][lane] = {w.list.v, w.list.i};
+  __syncthreads();
+  if (wave) return;
+  LpStats t = parts[0];
+#pragma unroll
+  for (int o = 1; o < kLpWaves; ++o) {
+    t = lp_join(t, parts[o]);
+    if (TOP) w.list.merge({slots[o][lane].v, slots[o][lane].i}, lane);
+  }
+  if (a.S == 1) {
+    lp_write<T>(a, row, t, w.list, lane);
+    return;
+  }
+  uint32_t* rec = a.part + (size_t)blockIdx.x * (4 + 2 * a.k);
+  if (lane == 0) *reinterpret_cast<LpStats*>(rec) = t;
+  if (lane < a.k) {
+    rec[4 + lane] = __float_as_uint(w.list.v);
+    rec[4 + a.k + lane] = (uint32_t)w.list.i;
+  }
+}
+
+// A row's splits joined: wave w takes the splits w, w + 16, ..., then pairs of waves.
+constexpr int kLpJoinWaves = 16;
+
+template <class T>
+__global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
+  __shared__ LpSlot slots[kLpJoinWaves][64];
+  __shared__ LpStats parts[kLpJoinWaves];
+  const int row = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  LpStats t{-INFINITY, 0.f, 0.f};
+  LpList list;
+  for (int p = wave; p < a.S; p += kLpJoinWaves) {
+    const uint32_t* rec = a.part + ((size_t)row * a.S + p) * (4 + 2 * a.k);
+    t = lp_join(t, *reinterpret_cast<const LpStats*>(rec));
+    LpList more;
+    if (lane < a.k) {
+      more.v = __uint_as_float(rec[4 + lane]);
+      more.i = (int)rec[4 + a.k + lane];
+    }
+    if (a.k) list.merge(more, lane);
+  }
+  for (int half = kLpJoinWaves / 2; half > 0; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+      if (lane == 0) parts[wave] = t;
+      slots[wave][lane] = {list.v, list.i};
+    }
+    __syncthreads();
+    if (wave < half) {
+      t = lp_join(t, parts[wave + half]);
+      if (a.k) list.merge({slots[wave + half][lane].v, slots[wave + half][lane].i}, lane);
+    }
+  }
+  if (wave == 0) lp_write<T>(a, row, t, list, lane);
+}
+
+// Workgroups a row is split over: none from 512 rows on; else up to about 512 workgroups,
+// of at least two blocks a wave.
+int lp_splits(int T, int n) {
+  const long long blocks = ((long long)n + kLpBlock - 1) / kLpBlock;
+  const long long most = blocks / (2 * kLpWaves);
+  const long long want = T >= 512 ? 1 : 512 / T;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+size_t lp_bytes(int T, int n, int k) {
+  const int S = lp_splits(T, n);
+  return S == 1 ? 0 : (size_t)T * S * (4 + 2 * k) * 4;
+}
+
+template <class T>
+int logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const T* x, size_t ld,
+             const int32_t* targets, int T_, int n, int asked, int k, qw4_workspace* ws, void* stream) {
+  if (T_ < 0) return QW4_ERR_M;
+  if (n < 1 || ld < (size_t)n || asked < 0 || k < 0 || k > kLpMaxTop) return QW4_ERR_SHAPE;
+  if (T_ == 0) return QW4_OK;
+  if (!x || (asked && (!lp || !targets)) || (k && (!top_ids || !top_lp))) return QW4_ERR_NULL;
+  if ((uintptr_t)x % sizeof(T) || ((uintptr_t)lp | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_lp |
+                                   (uintptr_t)targets) & 3)
+    return QW4_ERR_ALIGN;
+  const size_t need = lp_bytes(T_, n, k);
+  LpArgs a{x, ld, targets, lp, entropy, top_lp, top_ids, n, asked, k, lp_splits(T_, n), nullptr};
+  if (need) {
+    if (!ws || !ws->buf || ws->bytes < need) return QW4_ERR_SCRATCH;
+    if ((uintptr_t)ws->buf & 15) return QW4_ERR_ALIGN;
+    a.part = static_cast<uint32_t*>(ws->buf);
+  }
+  hipStream_t s = (hipStream_t)stream;
+  launch_rows_of(T_, 1 << 23, [&](int first, int rows) {
+    LpArgs r = a;   // split rows are few: they go out in one run
+    r.x = x + (size_t)first * ld;
+    if (asked) {
+      r.targets += (size_t)first * asked;
+      r.lp += (size_t)first * asked;
+    }
+    if (entropy) r.entropy += first;
+    if (k) {
+      r.top_ids += (size_t)first * k;
+      r.top_lp += (size_t)first * k;
+    }
+    if (k)
+      k_logprobs<T, true><<<rows * r.S, 64 * kLpWaves, 0, s>>>(r);
+    else
+      k_logprobs<T, false><<<rows * r.S, 64 * kLpWaves, 0, s>>>(r);
+    if (r.S > 1) k_logprobs_join<T><<<rows, 64 * kLpJoinWaves, 0, s>>>(r);
+  });
+  QW4_LAUNCH_CHECK();
+  return QW4_OK;
+}
+
+}  // namespace
+}  // namespace qw4
+
+using namespace qw4;
+
+extern "C" {
+
+int qw4_logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const uint16_t* logits, size_t ld,
+                 const int32_t* targets, int T, int n, int asked, int top_k, qw4_workspace* ws, void* stream) {
+  return logprobs<uint16_t>(lp, entropy, top_ids, top_lp, logits, ld, targets, T, n, asked, top_k, ws, stream);
+}
+
+int qw4_logprobs_f32(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const float* logits, size_t ld,
+                     const int32_t* targets, int T, int n, int asked, int top_k, qw4_workspace* ws, void* stream) {
+  return logprobs<float>(lp, entropy, top_ids, top_lp, logits, ld, targets, T, n, asked, top_k, ws, stream);
+}
+
+size_t qw4_logprobs_workspace(int T, int n, int top_k) {
+  return T < 1 || n < 1 || top_k < 0 || top_k > kLpMaxTop ? 0 : lp_bytes(T, n, top_k);
+}
+
+}  // extern "C"

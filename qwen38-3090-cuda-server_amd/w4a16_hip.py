@@ -56,7 +56,9 @@ EXPORTS = (
     "qw4_tune_gemm", "qw4_tune_linear", "qw4_tune_grouped", "qw4_gemv_argmax_noalloc",
     "qw4_quantize_w4a16", "qw4_plan_alloc", "qw4_plan_free", "qw4_route", "qw4_route_f32",
     "qw4_route_ids", "qw4_combine", "qw4_linear_epilogue", "qw4_gemm_grouped",
-    "qw4_epilogue_workspace",
+    "qw4_epilogue_workspace", "qw4_a8_alloc", "qw4_a8_free", "qw4_a8_quantize", "qw4_a8_rmsnorm",
+    "qw4_a8_dequant_rows", "qw4_a8_linear", "qw4_a8_linear_f32", "qw4_logprobs", "qw4_logprobs_f32",
+    "qw4_logprobs_workspace",
 )
 
 # safetensors dtype order (qw4_st_tensor.dtype)
@@ -116,6 +118,12 @@ class ExpertPlan(C.Structure):
                 ("experts", C.c_int32), ("max_pairs", C.c_int32)]
 
 
+class A8Rows(C.Structure):
+    """qw4_a8: rows of activations in 8 bits with scales."""
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("max_rows", C.c_int32),
+                ("in_f", C.c_int32)]
+
+
 class StTensor(C.Structure):
     """qw4_st_tensor: one tensor of an open safetensors set (host view)."""
     _fields_ = [("dtype", C.c_int32), ("ndim", C.c_int32), ("shape", C.c_int64 * 8),
@@ -136,7 +144,7 @@ def lib():
     vp, i, sz, u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
     W, S, WS = C.POINTER(W4A16Weights), C.POINTER(GemvScratch), C.POINTER(GemmWorkspace)
     W8 = C.POINTER(W8A16Weights)
-    PL = C.POINTER(ExpertPlan)
+    PL, A8 = C.POINTER(ExpertPlan), C.POINTER(A8Rows)
     sig = {
         "qw4_status_string": ([i], C.c_char_p),
         "qw4_last_hip_error": ([], i),
@@ -203,6 +211,16 @@ def lib():
         "qw4_epilogue_workspace": ([W, i], sz),
         "qw4_gemm_grouped": ([vp, W, vp, i, PL, i, i, vp, i, WS, vp], i),
         "qw4_combine": ([vp, vp, PL, vp, i, i, i, vp, vp], i),
+        "qw4_a8_alloc": ([A8, i, i], i),
+        "qw4_a8_free": ([A8], i),
+        "qw4_a8_quantize": ([A8, vp, i, i, vp], i),
+        "qw4_a8_rmsnorm": ([A8, vp, vp, vp, vp, i, C.c_float, vp], i),
+        "qw4_a8_dequant_rows": ([vp, A8, i, i, vp], i),
+        "qw4_a8_linear": ([vp, W, A8, i, vp, i, vp, WS, vp], i),
+        "qw4_a8_linear_f32": ([vp, W, A8, i, WS, vp], i),
+        "qw4_logprobs": ([vp, vp, vp, vp, vp, sz, vp, i, i, i, i, WS, vp], i),
+        "qw4_logprobs_f32": ([vp, vp, vp, vp, vp, sz, vp, i, i, i, i, WS, vp], i),
+        "qw4_logprobs_workspace": ([i, i, i], sz),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -238,7 +256,7 @@ _torch = None
 
 
 # The types that kernels read, once a tensor has come; other types of the same bits.
-_bf16 = _i32 = _f32 = _same = None
+_bf16 = _i32 = _f32 = _i8 = _same = None
 
 
 def _buf(t, dtype, nbytes: int, dev: int, where: str) -> int | None:
@@ -255,10 +273,10 @@ def _buf(t, dtype, nbytes: int, dev: int, where: str) -> int | None:
 
 
 def _types() -> None:
-    global _bf16, _i32, _f32, _same
+    global _bf16, _i32, _f32, _i8, _same
     import torch
 
-    _bf16, _i32, _f32 = torch.bfloat16, torch.int32, torch.float32
+    _bf16, _i32, _f32, _i8 = torch.bfloat16, torch.int32, torch.float32, torch.int8
     _same = {torch.int16: _bf16, torch.uint16: _bf16, torch.uint32: _i32}
 
 
@@ -738,6 +756,113 @@ def combine_experts(out, y, weights, T: int, top_k: int, dim: int, plan: ExpertP
                            _buf(weights, _f32, T * top_k * 4, dev, "combine_experts weights"), T, top_k, dim,
                            _buf(residual, _bf16, T * dim * 2, dev, "combine_experts residual"), to),
          "combine_experts")
+
+
+# --------------------------------------------------- activations in 8 bits
+def a8_alloc(max_rows: int, in_f: int) -> A8Rows:
+    """qw4_a8_alloc: device arrays of the library."""
+    a = A8Rows()
+    _chk(lib().qw4_a8_alloc(C.byref(a), max_rows, in_f), "a8_alloc")
+    return a
+
+
+def a8_over(q, scale) -> A8Rows:
+    """8-bit rows over device tensors of the caller, which keeps them alive: q [max_rows][in_f]
+    int8 (in the order that qw4_a8 describes) and scale [in_f / 128][max_rows] fp32."""
+    if _same is None:
+        _types()
+    (rows, in_f), dev = q.shape, max(q.get_device(), 0)   # both on one GPU, the current one or not
+    return A8Rows(_buf(q, _i8, 0, dev, "a8_over q"),
+                  _buf(scale, _f32, rows * (in_f // 128) * 4, dev, "a8_over scale"), rows, in_f)
+
+
+def a8_free(a: A8Rows) -> None:
+    """qw4_a8_free: for rows of a8_alloc only."""
+    _chk(lib().qw4_a8_free(C.byref(a)), "a8_free")
+
+
+def _rows_of(t, dtype, rows: int, width: int, size: int, dev: int, where: str) -> tuple:
+    """Address and row stride of `rows` rows of `width` elements: a 2-D tensor of that width,
+    which may be columns of a wider one, or any contiguous one; a raw address (rows one
+    behind the other) is trusted."""
+    if getattr(t, "dim", None) is None or t.dim() != 2 or t.shape[1] == width and t.is_contiguous():
+        return _buf(t, dtype, rows * width * size, dev, where), width
+    if t.dtype is not dtype and _same.get(t.dtype) is not dtype:
+        raise ValueError(f"{where}: type {t.dtype}, needs {dtype}")
+    if t.shape[0] < rows or t.shape[1] != width or t.stride(1) != 1 or t.stride(0) < width:
+        raise ValueError(f"{where}: needs {rows} rows of {width} neighbouring elements")
+    if t.get_device() != dev:
+        raise ValueError(f"{where}: not on the call's GPU")
+    return t.data_ptr(), t.stride(0)
+
+
+def quantize_a8(a: A8Rows, x, T: int, stream=None) -> None:
+    """qw4_a8_quantize: the first T rows of a from bf16 rows x, contiguous or the columns of
+    a wider 2-D tensor."""
+    dev, to = _place(stream)
+    x, ld = _rows_of(x, _bf16, max(T, 0), a.in_f, 2, dev, "quantize_a8 x")
+    _chk(lib().qw4_a8_quantize(a, x, ld, T, to), "quantize_a8")
+
+
+def rmsnorm_a8(a: A8Rows, h, w, T: int, eps: float, residual=None, out=None, stream=None) -> None:
+    """qw4_a8_rmsnorm: out = bf16(h + residual) where there is one, and a = rmsnorm of it (of h
+    without a residual) in 8 bits. out may be h."""
+    size, (dev, to) = max(T, 0) * a.in_f * 2, _place(stream)
+    _chk(lib().qw4_a8_rmsnorm(a, _buf(out, _bf16, size, dev, "rmsnorm_a8 out"),
+                              _buf(h, _bf16, size, dev, "rmsnorm_a8 h"),
+                              _buf(residual, _bf16, size, dev, "rmsnorm_a8 residual"),
+                              _buf(w, _bf16, a.in_f * 2, dev, "rmsnorm_a8 w"), T, eps, to), "rmsnorm_a8")
+
+
+def a8_dequant_rows(dst, a: A8Rows, row0: int, nrows: int, stream=None) -> None:
+    """qw4_a8_dequant_rows: dst [nrows][in_f] bf16 = the values of rows row0.."""
+    dev, to = _place(stream)
+    _chk(lib().qw4_a8_dequant_rows(_buf(dst, _bf16, max(nrows, 0) * a.in_f * 2, dev, "a8_dequant_rows dst"),
+                                   a, row0, nrows, to), "a8_dequant_rows")
+
+
+def linear_w4a8(y, w: W4A16Weights, a: A8Rows, T: int, ws: GemmWorkspace | None = None, bias=None,
+                act: int = ACT_NONE, residual=None, stream=None) -> None:
+    """qw4_a8_linear: y = bf16(act(x @ W^T + bias) + residual), x the first T rows of a."""
+    width, (dev, to) = w.out_f // 2 if act == ACT_SWIGLU else w.out_f, _place(stream)
+    _chk(lib().qw4_a8_linear(_buf(y, _bf16, T * width * 2, dev, "linear_w4a8 y"), w, a, T,
+                             _buf(bias, _bf16, w.out_f * 2, dev, "linear_w4a8 bias"), act,
+                             _buf(residual, _bf16, T * width * 2, dev, "linear_w4a8 residual"), ws, to),
+         "linear_w4a8")
+
+
+def linear_w4a8_f32(y, w: W4A16Weights, a: A8Rows, T: int, ws: GemmWorkspace | None = None,
+                    stream=None) -> None:
+    """qw4_a8_linear_f32: y = x @ W^T in fp32 (logits), x the first T rows of a."""
+    dev, to = _place(stream)
+    _chk(lib().qw4_a8_linear_f32(_buf(y, _f32, T * w.out_f * 4, dev, "linear_w4a8_f32 y"), w, a, T, ws, to),
+         "linear_w4a8_f32")
+
+
+# ------------------------------------------------------- log probabilities
+def logprobs_workspace(T: int, n: int, top_k: int) -> int:
+    """qw4_logprobs_workspace: bytes of workspace for such a call."""
+    return lib().qw4_logprobs_workspace(T, n, top_k)
+
+
+def logprobs(lp, logits, targets, T: int, n: int, ws: GemmWorkspace | None = None, entropy=None,
+             top_ids=None, top_logprobs=None, top_k: int = 0, asked: int | None = None,
+             stream=None) -> None:
+    """qw4_logprobs / qw4_logprobs_f32 by the type of logits (bf16 or fp32; [T][n], contiguous
+    or the columns of a wider 2-D tensor; a raw address is of contiguous bf16): lp [T][asked]
+    of targets [T][asked] int32 (asked: targets' elements over T unless given), entropy [T],
+    the top_k best tokens' ids and log probabilities [T][top_k]."""
+    dev, to = _place(stream)
+    if asked is None:
+        asked = targets.numel() // T if targets is not None and T > 0 else 0
+    f32 = _f32 is not None and getattr(logits, "dtype", None) is _f32
+    x, row = _rows_of(logits, _f32 if f32 else _bf16, max(T, 0), n, 4 if f32 else 2, dev, "logprobs logits")
+    rows = max(T, 0) * 4
+    _chk((lib().qw4_logprobs_f32 if f32 else lib().qw4_logprobs)(
+        _buf(lp, _f32, rows * asked, dev, "logprobs lp"), _buf(entropy, _f32, rows, dev, "logprobs entropy"),
+        _buf(top_ids, _i32, rows * top_k, dev, "logprobs top_ids"),
+        _buf(top_logprobs, _f32, rows * top_k, dev, "logprobs top_logprobs"), x, row,
+        _buf(targets, _i32, rows * asked, dev, "logprobs targets"), T, n, asked, top_k, ws, to), "logprobs")
 
 
 # ------------------------------------------------------ synthetic inputs
