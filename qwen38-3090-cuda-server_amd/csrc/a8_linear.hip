@@ -8,6 +8,9 @@
 // are scaled into fp32 accumulators.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <mutex>
+
 #include "../../include/qwen_w4a16.h"
 #include "a8.h"
 #include "epilogue.h"
@@ -37,71 +40,504 @@ __device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
   return ((nib | 0x80808080u) - z) ^ 0x80808080u;
 }
 
-// A wave computes 32 columns (rows of W) x 32 rows of x; gated, the up columns too.
-// MFMA layout (A: weights): lane l holds row l % 32, inputs 16 (l / 32).. of an operand;
-// of the result column l % 32 (a row of x), rows 8 j + 4 (l / 32) + i.
-template <bool GLU, bool F32>
-__global__ __launch_bounds__(64) void k_a8_simple(A8Args a) {
-  const int lane = threadIdx.x, r = lane & 31, h = lane >> 5;
-  const int n0 = blockIdx.x * 32, m = blockIdx.y * 32 + r;
-  const int row = min(m, a.M - 1);
-  constexpr int NP = GLU ? 2 : 1;
-  float acc[NP][16] = {};
-  for (int g = 0; g < a.G; ++g) {
-    const u32x4* xr = reinterpret_cast<const u32x4*>(a.q + (size_t)row * a.K + g * kGroup);
-    const float sx = a.scale[(size_t)g * a.max_rows + row];
+// ---------------------------------------------------------------------------
+// k_a8_tiles: 256 columns (rows of W) x 32 MB rows of x a workgroup of 8 waves, two a
+// SIMD; a wave owns 32 columns against all the tile's rows, in MB blocks of 32 x 32.
+//
+//  * Weights (the MFMA's A operand) come straight into registers, a lane the 32 bytes of
+//    its row and half of a group: every weight is unpacked once per workgroup, 7 vector
+//    instructions for 8.
+//  * Codes (B) go global -> LDS (buffer_load ... lds, whole 128-byte row segments, 1 KiB an
+//    instruction), D groups buffered. Row m holds 16-byte chunk c at c ^ g(m), g = (m % 8) ^
+//    (m / 8 % 2): the 8 rows that 128 bytes of banks serve, and the 16 of 256 bytes, differ.
+//    The scales of the tile's rows lie behind them.
+//  * A block's four MFMAs start from M = 1.5 2^23 as bits, so that the sums, read as
+//    floats, are M + sum: t = fma(f, sx, -M sx) is the scaled sum, rounded once (M sx is
+//    exact for an sx of 22 bits, to which it is cut), and acc = fma(t, sw, acc): two
+//    instructions a sum and group where a conversion, two products and an addition were four.
+//
+// MFMA layout: lane l holds weight row l % 32, inputs of chunks 2 s + l / 32 (s = 0, 1), low
+// nibbles and high nibbles an operand each; of the result column l % 32 (a row of x), rows
+// 8 j + 4 (l / 32) + i.
+constexpr int kTileCols = 256;
+constexpr int kA8Waves = 8;
+constexpr float kMagic = 12582912.f;
+
+// Outputs: bf16 with an epilogue, gate and up joined, fp32.
+enum { A8_EPI = 0, A8_GLU = 1, A8_F32 = 2 };
+
+template <int MB>
+struct A8Split {
+  static constexpr int ACT = MB / 2;               // 1 KiB loads of codes a wave and group
+  static constexpr int DEPTH = MB <= 2 ? 4 : MB <= 4 ? 3 : 2;
+  static constexpr int LOADS = ACT + 1 + 7;        // codes, scales, weights (2 + 4 + 1)
+  static constexpr int CODES = 32 * MB * 8;        // 16-byte units of a buffer's codes
+  static constexpr int UNITS = CODES + kA8Waves * 16;   // and of its scales, 64 a wave's load
+  static_assert(MB % 2 == 0 && MB <= 8, "whole loads a wave");
+};
+
+struct A8Tiles {
+  A8Args a;
+  float* slots;              // [P][2] partial tiles
+  int tiles_n, tiles_m, map;
+  int P, full, U;            // as in the bf16 product: whole tiles [0, full), then U units over P
+};
+
+struct A8Weights {
+  u32x4 q[2];                // chunks h, 2 + h of the lane's row
+  u32x2 s[4];                // scales of rows 8 j + 4 h .. + 3
+  uint32_t z;                // zero points of rows r & ~3 .. + 3
+};
+struct A8Src {               // of a wave's weight tile: blocks and (scale, zero-point) records
+  const uint32_t* qw;
+  const uint16_t* sc;
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t a8_rsrc(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+
+// Part 0: the words and zero points of group g, part 1: the scales. A group of which there
+// is not `some` is read from a resource of no length: no memory, no branch.
+__device__ __forceinline__ void a8_load_weights(A8Weights& w, const A8Src& src, int b, int g, bool some, int lane,
+                                                int part) {
+  const int r = lane & 31, h = lane >> 5;
+  const int pos = tile_pos_of_row(32 * b + r);
+  const __amdgpu_buffer_rsrc_t rec = a8_rsrc(src.sc + (size_t)g * kMetaU16, some ? (uint32_t)kMetaBytes : 0u);
+  if (part == 0) {
+    const __amdgpu_buffer_rsrc_t qw = a8_rsrc(src.qw + (size_t)g * kWordsPerBlock, some ? 4096u : 0u);
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int n = n0 + p * a.epi.up, tile = n / kTileN, b = (n % kTileN) / 32;
-      const size_t blk = (size_t)tile * a.G + g;
-      const int pos = tile_pos_of_row(32 * b + r);
-      const uint32_t z = (a.zr[blk * 16 + (32 * b + r) / 4] >> (4 * (r & 3))) & 15u;
-      i32x16 c = {};
+    for (int s = 0; s < 2; ++s)
+      w.q[s] = __builtin_amdgcn_raw_buffer_load_b128(qw, ((2 * s + h) * 64 + pos) * 16, 0, 0);
+    w.z = __builtin_amdgcn_raw_buffer_load_b16(rec, 128 + (8 * b + (r >> 2)) * 2, 0, 0);
+  } else {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 w = reinterpret_cast<const u32x4*>(a.qw + blk * kWordsPerBlock)[(2 * s + h) * 64 + pos];
-        u32x4 lo, hi;
+    for (int j = 0; j < 4; ++j)
+      w.s[j] = __builtin_amdgcn_raw_buffer_load_b64(rec, (32 * b + 8 * j + 4 * h) * 2, 0, 0);
+  }
+}
+
+// The rows of x that a tile reads.
+struct A8Rows {
+  const int8_t* q;           // of the tile's first row
+  const float* scale;
+  uint32_t rows;             // of the tile that there are
+};
+
+template <int MB>
+__device__ __forceinline__ void a8_load_rows(const A8Args& a, const A8Rows& x, uint32_t voff, u32x4* buf, int g,
+                                             bool some, int wave, int lane, int part) {
+  using Sp = A8Split<MB>;
+  if (part < Sp::ACT) {
+    const int rb = part * kA8Waves + wave;   // 8 rows
+    const __amdgpu_buffer_rsrc_t rs = a8_rsrc(x.q, some ? x.rows * (uint32_t)a.K : 0u);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, buf + rb * 64, 16, voff + (uint32_t)(8 * rb) * (uint32_t)a.K,
+                                             (uint32_t)g * kGroup, 0, 0);
+  } else {   // 64 scales a wave; those past the tile's rows from a resource of no length
+    const __amdgpu_buffer_rsrc_t rs =
+        a8_rsrc(x.scale + (size_t)g * a.max_rows, some && wave < MB / 2 ? x.rows * 4u : 0u);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, buf + Sp::CODES + wave * 16, 4, (uint32_t)(wave * 64 + lane) * 4u, 0, 0, 0);
+  }
+}
+
+// One group: the MFMAs over buf with the weights w, while the loads of group gn go out. A
+// block's operands are read while the block before it is scaled; the fence between blocks
+// keeps the compiler from reading them all at the start, into registers that there aren't.
+template <int MB>
+__device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], const A8Weights& w, A8Weights& wn,
+                                         const u32x4* buf, u32x4* nbuf, const A8Rows& x, const A8Src& src, bool more,
+                                         uint32_t voff, int b, int gn, int wave, int lane) {
+  using Sp = A8Split<MB>;
+  const int r = lane & 31, h = lane >> 5;
+  const int swz = (r & 7) ^ ((r >> 3) & 1);
+  const uint32_t z = ((w.z >> (4 * (r & 3))) & 15u) * 0x01010101u;
+  const float* scales = reinterpret_cast<const float*>(buf + Sp::CODES);
+  u32x4 v[4];
+  float sx;
+  auto read = [&](int mb) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[i] = a8_less(w[i] & 0x0F0F0F0Fu, z * 0x01010101u);
-          hi[i] = a8_less((w[i] >> 4) & 0x0F0F0F0Fu, z * 0x01010101u);
-        }
-        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, lo),
-                                                  __builtin_bit_cast(i32x4, xr[2 * (2 * s + h)]), c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, hi),
-                                                  __builtin_bit_cast(i32x4, xr[2 * (2 * s + h) + 1]), c, 0, 0, 0);
-      }
+    for (int o = 0; o < 4; ++o) v[o] = buf[(32 * mb + r) * 8 + ((4 * (o >> 1) + 2 * h + (o & 1)) ^ swz)];
+    sx = scales[32 * mb + r];
+  };
+  read(0);
+  i32x4 op[4];               // chunk s = 0 low, high nibbles, s = 1 low, high
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      op[2 * s][i] = (int)a8_less(w.q[s][i] & 0x0F0F0F0Fu, z);
+      op[2 * s + 1][i] = (int)a8_less((w.q[s][i] >> 4) & 0x0F0F0F0Fu, z);
+    }
+  float sw[16];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sw[4 * j + i] = bf16_bits_to_f32((w.s[j][i >> 1] >> (16 * (i & 1))) & 0xffffu);
+  i32x16 start;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) start[i] = 0x4B400000;
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    i32x16 c = start;
+#pragma unroll
+    for (int o = 0; o < 4; ++o)
+      c = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[o], __builtin_bit_cast(i32x4, v[o]), c, 0, 0, 0);
+    const float f = __uint_as_float(__float_as_uint(sx) & ~3u), less = -kMagic * f;
+    if (mb + 1 < MB) read(mb + 1);
+    if (mb < Sp::ACT + 1) a8_load_rows<MB>(a, x, voff, nbuf, gn, more, wave, lane, mb);
+    if (mb == MB - 2) a8_load_weights(wn, src, b, gn, more, lane, 0);
+    if (mb == MB - 1) a8_load_weights(wn, src, b, gn, more, lane, 1);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      acc[mb][i] = __builtin_fmaf(__builtin_fmaf(__int_as_float(c[i]), f, less), sw[i], acc[mb][i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <int MB>
+__device__ __forceinline__ void a8_segment(const A8Args& a, float (&acc)[MB][16], u32x4* lds, const A8Rows& x,
+                                           int tile, int b, int g0, int g1, int wave, int lane) {
+  using Sp = A8Split<MB>;
+  constexpr int D = Sp::DEPTH;
+  const A8Src src{a.qw + (size_t)tile * a.G * kWordsPerBlock, a.sc + (size_t)tile * a.G * kMetaU16};
+  // lane i of a load writes slot i % 8 of row i / 8: it fetches the chunk that belongs there
+  const uint32_t voff = (uint32_t)(lane >> 3) * (uint32_t)a.K + (uint32_t)((lane & 7) ^ (lane >> 3) ^ (wave & 1)) * 16u;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
+  __syncthreads();   // the previous segment's last LDS reads are done
+  A8Weights w[D];
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) {
+    const bool in = g0 + d < g1;
+#pragma unroll
+    for (int p = 0; p <= Sp::ACT; ++p) a8_load_rows<MB>(a, x, voff, lds + d * Sp::UNITS, g0 + d, in, wave, lane, p);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) a8_load_weights(w[d], src, b, g0 + d, in, lane, p);
+  }
+  for (int gb = g0; gb < g1; gb += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int g = gb + d;
+      if (g >= g1) break;
+      // group g has landed (the D - 2 behind it may be in flight) for every wave, and
+      // every wave is done with group g - 1's buffer
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 2) * Sp::LOADS) : "memory");
+      constexpr int kBack = D - 1;
+      a8_group<MB>(a, acc, w[d], w[(d + kBack) % D], lds + d * Sp::UNITS, lds + (d + kBack) % D * Sp::UNITS, x, src,
+                   g + kBack < g1, voff, b, g + kBack, wave, lane);
+    }
+  }
+}
+
+__device__ __forceinline__ void a8_tile_coords(const A8Tiles& t, int i, int& tn, int& tm) {
+  if (t.map == 2) {   // slices along K: row-major, so an XCD's run shares rows of x
+    tm = i / t.tiles_n;
+    tn = i - tm * t.tiles_n;
+    return;
+  }
+  const int band = 4 * t.tiles_n;   // bands of 4 row tiles, as in the bf16 product
+  const int bd = i / band, w = i % band;
+  const int rows = min(4, t.tiles_m - 4 * bd);
+  tm = 4 * bd + w % rows;
+  tn = w / rows;
+}
+
+// Weight tile, half and first output column of wave w in column tile tn. Gated, waves 4..7
+// take the up rows of waves 0..3.
+struct A8Wave {
+  int tile, b, col;
+  bool valid;
+};
+template <int OUT>
+__device__ __forceinline__ A8Wave a8_wave(const A8Args& a, int tn, int w) {
+  if (OUT == A8_GLU) {
+    const int t = 2 * tn + ((w & 3) >> 1);
+    const bool ok = t * kTileN < a.ld;
+    const int gate = ok ? t : a.ld / kTileN - 1;
+    return {gate + (w >> 2) * (a.epi.up / kTileN), w & 1, t * kTileN + 32 * (w & 1), ok};
+  }
+  const int t = 4 * tn + (w >> 1);
+  const bool ok = t * kTileN < a.N;
+  return {ok ? t : a.N / kTileN - 1, w & 1, t * kTileN + 32 * (w & 1), ok};
+}
+
+constexpr uint32_t kA8SlotBytes = 256u * kTileCols * 4;
+
+__device__ __forceinline__ uint32_t a8_slot_off(int vp, int which, int wave, int mb, int lane) {
+  return (uint32_t)(vp * 2 + which) * kA8SlotBytes + (uint32_t)((wave * 8 + mb) * 4096 + lane * 16);
+}
+__device__ __forceinline__ int a8_range_start(const A8Tiles& t, int vp) { return (int)((long long)vp * t.U / t.P); }
+__device__ __forceinline__ int a8_owner_of(const A8Tiles& t, int u) { return (int)(((long long)(u + 1) * t.P - 1) / t.U); }
+
+// Tile store: the sums pass through LDS, 32 rows x 256 columns of fp32 a block (16-byte
+// chunk c of a row at c ^ (row % 16)), and come back as whole row segments, 8 output
+// columns a lane, where gate and up meet, bias and residual are added and the result is
+// rounded once.
+template <int MB, int OUT>
+__device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB][16], u32x4* lds, int m0, int tn,
+                                         int wave, int lane) {
+  constexpr bool GLU = OUT == A8_GLU;
+  constexpr int kFits = A8Split<MB>::DEPTH * A8Split<MB>::UNITS / 2048;
+  constexpr int kPass = kFits < MB ? kFits : MB;   // blocks of 32 KiB at a time
+  static_assert(kPass >= 1, "a block fits the buffers");
+  constexpr int kCols = GLU ? 128 : 256, kLanes = kCols / 8, kRows = 64 * kA8Waves / kLanes;
+  const int r = lane & 31, h = lane >> 5;
+  const int t = wave * 64 + lane, cl = t % kLanes, rl = t / kLanes;
+  const int col = tn * kCols + 8 * cl;
+  const bool in = col < a.ld;
+  float bias[GLU ? 2 : 1][8];
+  if (OUT != A8_F32 && in) load_bias<GLU>(bias, a.epi, col);
+#pragma unroll
+  for (int p0 = 0; p0 < MB; p0 += kPass) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPass; ++k) {
+      if (p0 + k >= MB) break;
+      const float(&v)[16] = acc[p0 + k < MB ? p0 + k : 0];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
+        lds[(32 * k + r) * 64 + ((8 * wave + 2 * j + h) ^ (r & 15))] =
+            u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                  __float_as_uint(v[4 * j + 3])};
+    }
+    __syncthreads();
+    const int rows = 32 * (p0 + kPass <= MB ? kPass : MB - p0);
+    for (int row = rl; row < rows; row += kRows) {
+      const int m = m0 + 32 * p0 + row;
+      if (!in || m >= a.M) continue;
+      const size_t at = (size_t)m * a.ld + col;
+      if constexpr (OUT == A8_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sw = bf16_bits_to_f32(a.sc[blk * kMetaU16 + 32 * b + 8 * j + 4 * h + i]);
-          acc[p][4 * j + i] = __builtin_fmaf((float)c[4 * j + i] * sx, sw, acc[p][4 * j + i]);
-        }
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<u32x4*>(static_cast<float*>(a.y) + at + 4 * c) = lds[row * 64 + ((2 * cl + c) ^ (row & 15))];
+      } else {
+        u32x4 res = {0u, 0u, 0u, 0u};
+        if (a.epi.res) res = *reinterpret_cast<const u32x4*>(a.epi.res + at);
+        float v[GLU ? 2 : 1][8];
+#pragma unroll
+        for (int j = 0; j < (GLU ? 2 : 1); ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const u32x4 w = lds[row * 64 + ((32 * j + 2 * cl + c) ^ (row & 15))];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][4 * c + i] = __uint_as_float(w[i]) + bias[j][4 * c + i];
+          }
+        epilogue_act<GLU>(v, a.epi.act);
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + at) = add_round8(v[0], res);
+      }
+    }
+  }
+}
+
+template <int MB, int OUT>
+__global__ __launch_bounds__(64 * kA8Waves, 2) void k_a8_tiles(A8Tiles t) {
+  using Sp = A8Split<MB>;
+  __shared__ u32x4 lds[Sp::DEPTH * Sp::UNITS];
+  const A8Args& a = t.a;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  float acc[MB][16];
+  int vp = blockIdx.x;
+  if (t.map) vp = (vp & 7) * (t.P >> 3) + (vp >> 3);   // each XCD a contiguous run (P % 8 == 0)
+  if (t.map == 2) {   // the runs go over slices, then tiles
+    const int nt = t.tiles_n * t.tiles_m, sl = vp / nt;
+    vp = (vp - sl * nt) * (t.P / nt) + sl;
+  }
+  const int u1 = a8_range_start(t, vp + 1);
+  int u = a8_range_start(t, vp), i = vp, which = 0;
+  for (;;) {   // whole tiles, then the units of this workgroup's range
+    int tile = i, g0 = 0, g1 = a.G;
+    if (i < t.full) {
+      i += t.P;
+    } else if (u < u1) {
+      const int ts = u / a.G;
+      g0 = u - ts * a.G;
+      g1 = min(a.G, u1 - ts * a.G);
+      tile = t.full + ts;
+      u = ts * a.G + g1;
+    } else {
+      break;
+    }
+    int tn, tm;
+    a8_tile_coords(t, tile, tn, tm);
+    const int m0 = tm * 32 * MB;
+    const A8Wave w = a8_wave<OUT>(a, tn, wave);
+    const A8Rows x{a.q + (size_t)m0 * a.K, a.scale + m0, (uint32_t)min(a.M - m0, 32 * MB)};
+    a8_segment<MB>(a, acc, lds, x, w.tile, w.b, g0, g1, wave, lane);
+    if (g0 == 0 && g1 == a.G) {
+      a8_store<MB, OUT>(a, acc, lds, m0, tn, wave, lane);
+    } else {   // the range's first tile to the first slot, its last to the second
+      const __amdgpu_buffer_rsrc_t rs = a8_rsrc(t.slots, 2u * t.P * kA8SlotBytes);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              u32x4{__float_as_uint(acc[mb][4 * k]), __float_as_uint(acc[mb][4 * k + 1]),
+                    __float_as_uint(acc[mb][4 * k + 2]), __float_as_uint(acc[mb][4 * k + 3])},
+              rs, a8_slot_off(vp, which, wave, mb, lane) + 1024 * k, 0, 0);
+    }
+    if (tile >= t.full) which = 1;
+  }
+}
+
+// The cut tiles: a wave sums one block (wave w, m-block mb; gated: gate and up) over its
+// pieces, in order, kAhead of them loaded at a time, and stores it.
+template <int MB, int OUT>
+__global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
+  constexpr bool GLU = OUT == A8_GLU;
+  constexpr int kPer = (GLU ? 4 : 8) * MB, NP = GLU ? 2 : 1, kAhead = 4;
+  const A8Args& a = t.a;
+  const int ts = blockIdx.x / kPer, w = blockIdx.x % kPer / MB, mb = blockIdx.x % MB;
+  const int p0 = a8_owner_of(t, ts * a.G), p1 = a8_owner_of(t, ts * a.G + a.G - 1);
+  if (p0 == p1) return;   // stored whole
+  int tn, tm;
+  a8_tile_coords(t, t.full + ts, tn, tm);
+  const A8Wave wv = a8_wave<OUT>(a, tn, w);
+  const int lane = threadIdx.x, r = lane & 31, h = lane >> 5, m = tm * 32 * MB + 32 * mb + r;
+  if (!wv.valid || tm * 32 * MB + 32 * mb >= a.M) return;
+  const __amdgpu_buffer_rsrc_t rs = a8_rsrc(t.slots, 2u * t.P * kA8SlotBytes);
+  float acc[NP][16] = {};
+  for (int pp = p0; pp <= p1; pp += kAhead) {
+    u32x4 v[kAhead][NP][4];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int q = pp + k;
+      const bool live = q <= p1;   // others read out of range, without memory
+      const int which = live && a8_range_start(t, q) / a.G == ts ? 0 : 1;
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[k][j][i] = __builtin_amdgcn_raw_buffer_load_b128(
+              rs, live ? a8_slot_off(q, which, w + 4 * j, mb, lane) + 1024 * i : 0xfffffff0u, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (pp + k > p1) break;
+#pragma unroll
+      for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[j][i] += __uint_as_float(v[k][j][i >> 2][i & 3]);
     }
   }
   if (m >= a.M) return;
+  if constexpr (OUT == A8_F32) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int col = n0 + 8 * j + 4 * h;
-    const size_t at = (size_t)m * a.ld + col;
-    if constexpr (F32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) =
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + (size_t)m * a.ld + wv.col + 8 * j + 4 * h) =
           f32x4{acc[0][4 * j], acc[0][4 * j + 1], acc[0][4 * j + 2], acc[0][4 * j + 3]};
-    } else {
-      float v[NP][4];
+  } else {
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[p][i] = acc[p][4 * j + i] + (a.epi.bias ? bf16_bits_to_f32(a.epi.bias[p * a.epi.up + col + i]) : 0.f);
-      epilogue_act<GLU>(v, a.epi.act);
+      for (int j = 0; j < 4; ++j) {
+        u32x2 bv = {0u, 0u};
+        if (a.epi.bias) bv = *reinterpret_cast<const u32x2*>(a.epi.bias + p * a.epi.up + wv.col + 8 * j + 4 * h);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[0][i] += a.epi.res ? bf16_bits_to_f32(a.epi.res[at + i]) : 0.f;
+        for (int i = 0; i < 4; ++i) acc[p][4 * j + i] += bf16_bits_to_f32((bv[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+      }
+    epilogue_act<GLU>(acc, a.epi.act);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const size_t at = (size_t)m * a.ld + wv.col + 8 * j + 4 * h;
+      u32x2 q = {0u, 0u};
+      if (a.epi.res) q = *reinterpret_cast<const u32x2*>(a.epi.res + at);
+      const float* f = &acc[0][4 * j];
       *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + at) =
-          u32x2{pack_bf16x2(v[0][0], v[0][1]), pack_bf16x2(v[0][2], v[0][3])};
+          u32x2{pack_bf16x2(f[0] + bf16_bits_to_f32(q[0] & 0xffffu), f[1] + bf16_bits_to_f32(q[0] >> 16)),
+                pack_bf16x2(f[2] + bf16_bits_to_f32(q[1] & 0xffffu), f[3] + bf16_bits_to_f32(q[1] >> 16))};
     }
   }
+}
+
+// How a call is cut: tiles of 32 mb rows, schedule (0 whole tiles, 1 all units over one
+// workgroup a CU, 2 whole rounds and the rest split, 3 every tile in S slices) and its
+// cost in group steps of 256 rows.
+struct A8Plan {
+  int mb, tiles_n, tiles_m, pick, S;
+  double cost;
+};
+
+double a8_step(int mb) { return 0.2 + 0.1 * mb; }
+
+A8Plan a8_plan(int M, int cols, long long G, int mb, int cus, bool ws_ok) {
+  A8Plan p{mb, (cols + kTileCols - 1) / kTileCols, (M + 32 * mb - 1) / (32 * mb), 0, 0, 0.};
+  const long long nt = (long long)p.tiles_n * p.tiles_m, rem = nt % cus;
+  const double t_dp = (double)((nt + cus - 1) / cus) * G, work = (double)nt * G / cus;
+  p.cost = t_dp;
+  ws_ok = ws_ok && rem != 0 && nt * G < (1LL << 31);
+  if (ws_ok) {
+    double best = 0.95 * t_dp;
+    auto take = [&](bool ok, int pick, double c) {
+      if (ok && c < best) {
+        p.pick = pick;
+        p.cost = best = c;
+      }
+    };
+    take(nt * G >= 2LL * cus, 1, work + 16.0 + 0.1 * ((cus + nt - 1) / nt + 1));
+    take(nt > cus && rem * G >= cus, 2, work + 8.0 + 0.1 * ((cus + rem - 1) / rem + 1));
+    int S = 2 * nt <= cus ? (int)std::min<long long>(cus / nt, G >= 8 ? G / 4 : G / 2) : 0;
+    while (S >= 2 && (nt * S) % 8) --S;
+    take(S >= 2, 3, (double)G / (S > 0 ? S : 1) + 8.0 + 0.1 * S);
+    p.S = S;
+  }
+  p.cost *= a8_step(mb);
+  return p;
+}
+
+int device_cus() {
+  static std::once_flag once[64];
+  static int cus[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  std::call_once(once[dev], [dev] {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cus[dev] = n;
+  });
+  return cus[dev];
+}
+
+template <int OUT, int MB>
+void launch_tiles(const A8Tiles& t, int grid, int nt, hipStream_t s) {
+  k_a8_tiles<MB, OUT><<<grid, 64 * kA8Waves, 0, s>>>(t);
+  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? 4 : 8) * MB, 64, 0, s>>>(t);
+}
+
+template <int OUT>
+int run_tiles(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
+  const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
+  const bool ws_ok = ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && cus % 8 == 0 &&
+                     ws->bytes >= 2ull * cus * kA8SlotBytes;
+  A8Plan p = a8_plan(a.M, cols, a.G, 8, cus, ws_ok);
+  for (int mb = 6; mb >= 2; mb -= 2) {
+    const A8Plan q = a8_plan(a.M, cols, a.G, mb, cus, ws_ok);
+    if (q.cost < 0.97 * p.cost) p = q;
+  }
+  const long long tiles = (long long)p.tiles_n * p.tiles_m;
+  if (tiles > 0x7fffffffLL / 64) return QW4_ERR_SHAPE;
+  const int nt = (int)tiles;
+  A8Tiles t{a, nullptr, p.tiles_n, p.tiles_m, nt % 8 == 0, nt, nt, 0};
+  int grid = nt;
+  if (p.pick) {
+    t.slots = static_cast<float*>(ws->buf);
+    t.P = grid = p.pick == 3 ? nt * p.S : cus;
+    t.full = p.pick == 2 ? nt - nt % cus : 0;
+    t.U = (nt - t.full) * a.G;
+    t.map = p.pick == 3 ? 2 : 1;
+  }
+  switch (p.mb) {
+    case 2: launch_tiles<OUT, 2>(t, grid, nt, s); break;
+    case 4: launch_tiles<OUT, 4>(t, grid, nt, s); break;
+    case 6: launch_tiles<OUT, 6>(t, grid, nt, s); break;
+    default: launch_tiles<OUT, 8>(t, grid, nt, s);
+  }
+  QW4_LAUNCH_CHECK();
+  return QW4_OK;
 }
 
 int check_call(const void* y, const qw4_weights* w, const qw4_a8* a, int T) {
@@ -136,25 +572,14 @@ int qw4_a8_linear(uint16_t* y, const qw4_weights* w, const qw4_a8* a, int T, con
   const bool glu = act == QW4_ACT_SWIGLU;
   if (glu && w->out_f % (2 * kTileN)) return QW4_ERR_SHAPE;
   if (((uintptr_t)bias | (uintptr_t)residual) & 15) return QW4_ERR_ALIGN;
-  (void)ws;
   const A8Args g = args_of(y, w, a, T, Epilogue{bias, residual, act, glu ? w->out_f / 2 : 0});
-  const dim3 grid(g.ld / 32, (T + 31) / 32);
-  if (glu)
-    k_a8_simple<true, false><<<grid, 64, 0, (hipStream_t)stream>>>(g);
-  else
-    k_a8_simple<false, false><<<grid, 64, 0, (hipStream_t)stream>>>(g);
-  QW4_LAUNCH_CHECK();
-  return QW4_OK;
+  return glu ? run_tiles<A8_GLU>(g, ws, (hipStream_t)stream) : run_tiles<A8_EPI>(g, ws, (hipStream_t)stream);
 }
 
 int qw4_a8_linear_f32(float* y, const qw4_weights* w, const qw4_a8* a, int T, qw4_workspace* ws, void* stream) {
   const int st = check_call(y, w, a, T);
   if (st) return st;
-  (void)ws;
-  const A8Args g = args_of(y, w, a, T, Epilogue{});
-  k_a8_simple<false, true><<<dim3(g.ld / 32, (T + 31) / 32), 64, 0, (hipStream_t)stream>>>(g);
-  QW4_LAUNCH_CHECK();
-  return QW4_OK;
+  return run_tiles<A8_F32>(args_of(y, w, a, T, Epilogue{}), ws, (hipStream_t)stream);
 }
 
 }  // extern "C"
