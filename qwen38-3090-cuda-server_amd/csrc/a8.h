@@ -4,9 +4,35 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/qwen_w4a16.h"
+#include "epilogue.h"
 #include "w4a16_common.h"
 
 namespace qw4 {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// Outputs of a product: bf16 with an epilogue, gate and up joined, fp32.
+enum { A8_EPI = 0, A8_GLU = 1, A8_F32 = 2 };
+
+struct A8Args {
+  const uint32_t* qw;
+  const uint16_t* sc;    // (scale, zero-point) records
+  const int8_t* q;
+  const float* scale;
+  void* y;               // bf16, or fp32 (A8_F32)
+  int M, N, K, G, max_rows, ld;
+  Epilogue epi;
+};
+
+// Four weights q - z of each byte's low nibble: 128 + q - z borrows from no other byte.
+__device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
+  return ((nib | 0x80808080u) - z) ^ 0x80808080u;
+}
+
+// The kernel for few rows (a8_few.hip): launches it and returns true, or returns false
+// where it does not apply.
+bool a8_few(int out, const A8Args& a, int cus, hipStream_t st);
 
 // The arrays of `a` are there, and it holds rows [row0, row0 + T).
 inline int check_a8(const qw4_a8* a, int row0, int T) {

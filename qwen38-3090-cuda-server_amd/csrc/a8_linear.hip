@@ -21,25 +21,6 @@ int check_weights_public(const qw4_weights* w);
 
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
-
-struct A8Args {
-  const uint32_t* qw;
-  const uint16_t* sc;
-  const uint16_t* zr;
-  const int8_t* q;
-  const float* scale;
-  void* y;               // bf16, or fp32 (F32)
-  int M, N, K, G, max_rows, ld;
-  Epilogue epi;
-};
-
-// Four weights q - z of each byte's low nibble: 128 + q - z borrows from no other byte.
-__device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
-  return ((nib | 0x80808080u) - z) ^ 0x80808080u;
-}
-
 // ---------------------------------------------------------------------------
 // k_a8_tiles: 256 columns (rows of W) x 32 MB rows of x a workgroup of 8 waves, two a
 // SIMD; a wave owns 32 columns against all the tile's rows, in MB blocks of 32 x 32.
@@ -59,16 +40,14 @@ __device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
 // MFMA layout: lane l holds weight row l % 32, inputs of chunks 2 s + l / 32 (s = 0, 1), low
 // nibbles and high nibbles an operand each; of the result column l % 32 (a row of x), rows
 // 8 j + 4 (l / 32) + i.
-constexpr int kTileCols = 256;
-constexpr int kA8Waves = 8;
+constexpr int kA8Waves = 4;
+constexpr int kTileCols = 32 * kA8Waves;
+constexpr int kPerCu = 2;   // workgroups
 constexpr float kMagic = 12582912.f;
-
-// Outputs: bf16 with an epilogue, gate and up joined, fp32.
-enum { A8_EPI = 0, A8_GLU = 1, A8_F32 = 2 };
 
 template <int MB>
 struct A8Split {
-  static constexpr int ACT = MB / 2;               // 1 KiB loads of codes a wave and group
+  static constexpr int ACT = 4 * MB / kA8Waves;               // 1 KiB loads of codes a wave and group
   static constexpr int DEPTH = MB <= 2 ? 4 : MB <= 4 ? 3 : 2;
   static constexpr int LOADS = ACT + 1 + 7;        // codes, scales, weights (2 + 4 + 1)
   static constexpr int CODES = 32 * MB * 8;        // 16-byte units of a buffer's codes
@@ -85,7 +64,7 @@ struct A8Tiles {
 
 struct A8Weights {
   u32x4 q[2];                // chunks h, 2 + h of the lane's row
-  u32x2 s[4];                // scales of rows 8 j + 4 h .. + 3
+  uint32_t s[4];             // scale of row 8 j + 4 h + lane % 4
   uint32_t z;                // zero points of rows r & ~3 .. + 3
 };
 struct A8Src {               // of a wave's weight tile: blocks and (scale, zero-point) records
@@ -113,7 +92,7 @@ __device__ __forceinline__ void a8_load_weights(A8Weights& w, const A8Src& src, 
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      w.s[j] = __builtin_amdgcn_raw_buffer_load_b64(rec, (32 * b + 8 * j + 4 * h) * 2, 0, 0);
+      w.s[j] = __builtin_amdgcn_raw_buffer_load_b16(rec, (32 * b + 8 * j + 4 * h + (lane & 3)) * 2, 0, 0);
   }
 }
 
@@ -131,8 +110,8 @@ __device__ __forceinline__ void a8_load_rows(const A8Args& a, const A8Rows& x, u
   if (part < Sp::ACT) {
     const int rb = part * kA8Waves + wave;   // 8 rows
     const __amdgpu_buffer_rsrc_t rs = a8_rsrc(x.q, some ? x.rows * (uint32_t)a.K : 0u);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, buf + rb * 64, 16, voff + (uint32_t)(8 * rb) * (uint32_t)a.K,
-                                             (uint32_t)g * kGroup, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, buf + rb * 64, 16, voff,
+                                             (uint32_t)(8 * rb) * (uint32_t)a.K + (uint32_t)g * kGroup, 0, 0);
   } else {   // 64 scales a wave; those past the tile's rows from a resource of no length
     const __amdgpu_buffer_rsrc_t rs =
         a8_rsrc(x.scale + (size_t)g * a.max_rows, some && wave < MB / 2 ? x.rows * 4u : 0u);
@@ -140,9 +119,24 @@ __device__ __forceinline__ void a8_load_rows(const A8Args& a, const A8Rows& x, u
   }
 }
 
-// One group: the MFMAs over buf with the weights w, while the loads of group gn go out. A
-// block's operands are read while the block before it is scaled; the fence between blocks
-// keeps the compiler from reading them all at the start, into registers that there aren't.
+// y += f times lane I's s of each lane's four. I = 0 waits as a register that a vector
+// instruction has written needs before it is read across lanes.
+template <int I>
+__device__ __forceinline__ void a8_fmac_quad(float& y, float s, float f) {
+  if constexpr (I == 0)
+    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
+  else if constexpr (I == 1)
+    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
+  else if constexpr (I == 2)
+    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
+  else
+    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
+}
+
+// One group: the MFMAs over buf with the weights w, while the loads of group gn go out. Four
+// sums of the block before are scaled behind each MFMA, and the operand that it has taken is
+// read for the block after; the fences keep that order. sw: in each four lanes the scales of
+// four neighbouring rows, for a v_fmac that takes its factor from one of them.
 template <int MB>
 __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], const A8Weights& w, A8Weights& wn,
                                          const u32x4* buf, u32x4* nbuf, const A8Rows& x, const A8Src& src, bool more,
@@ -153,13 +147,10 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
   const uint32_t z = ((w.z >> (4 * (r & 3))) & 15u) * 0x01010101u;
   const float* scales = reinterpret_cast<const float*>(buf + Sp::CODES);
   u32x4 v[4];
-  float sx;
-  auto read = [&](int mb) __attribute__((always_inline)) {
+  auto code = [&](int mb, int o) { return buf[(32 * mb + r) * 8 + ((4 * (o >> 1) + 2 * h + (o & 1)) ^ swz)]; };
 #pragma unroll
-    for (int o = 0; o < 4; ++o) v[o] = buf[(32 * mb + r) * 8 + ((4 * (o >> 1) + 2 * h + (o & 1)) ^ swz)];
-    sx = scales[32 * mb + r];
-  };
-  read(0);
+  for (int o = 0; o < 4; ++o) v[o] = code(0, o);
+  float sx = scales[r];
   i32x4 op[4];               // chunk s = 0 low, high nibbles, s = 1 low, high
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -168,11 +159,9 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
       op[2 * s][i] = (int)a8_less(w.q[s][i] & 0x0F0F0F0Fu, z);
       op[2 * s + 1][i] = (int)a8_less((w.q[s][i] >> 4) & 0x0F0F0F0Fu, z);
     }
-  float sw[16];
+  float sw[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sw[4 * j + i] = bf16_bits_to_f32((w.s[j][i >> 1] >> (16 * (i & 1))) & 0xffffu);
+  for (int j = 0; j < 4; ++j) sw[j] = bf16_bits_to_f32(w.s[j]);
   i32x16 start;
 #pragma unroll
   for (int i = 0; i < 16; ++i) start[i] = 0x4B400000;
@@ -180,17 +169,34 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     i32x16 c = start;
+    const float fx = __uint_as_float(__float_as_uint(sx) & ~3u), less = -kMagic * fx;
 #pragma unroll
-    for (int o = 0; o < 4; ++o)
+    for (int o = 0; o < 4; ++o) {
       c = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[o], __builtin_bit_cast(i32x4, v[o]), c, 0, 0, 0);
-    const float f = __uint_as_float(__float_as_uint(sx) & ~3u), less = -kMagic * f;
-    if (mb + 1 < MB) read(mb + 1);
-    if (mb < Sp::ACT + 1) a8_load_rows<MB>(a, x, voff, nbuf, gn, more, wave, lane, mb);
-    if (mb == MB - 2) a8_load_weights(wn, src, b, gn, more, lane, 0);
-    if (mb == MB - 1) a8_load_weights(wn, src, b, gn, more, lane, 1);
+      if (mb + 1 < MB) {
+        v[o] = code(mb + 1, o);
+        if (o == 0) sx = scales[32 * (mb + 1) + r];
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      acc[mb][i] = __builtin_fmaf(__builtin_fmaf(__int_as_float(c[i]), f, less), sw[i], acc[mb][i]);
+    for (int p = 0; p < Sp::ACT + 3; ++p)
+      if (p * MB / 2 / (Sp::ACT + 3) == mb) {
+        if (p < 2)
+          a8_load_weights(wn, src, b, gn, more, lane, p);
+        else
+          a8_load_rows<MB>(a, x, voff, nbuf, gn, more, wave, lane, p - 2);
+      }
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __builtin_fmaf(__int_as_float(c[4 * o + i]), fx, less);
+      float* y = acc[mb] + 4 * o;
+      a8_fmac_quad<0>(y[0], sw[o], f[0]);
+      a8_fmac_quad<1>(y[1], sw[o], f[1]);
+      a8_fmac_quad<2>(y[2], sw[o], f[2]);
+      a8_fmac_quad<3>(y[3], sw[o], f[3]);
+    }
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -245,8 +251,8 @@ __device__ __forceinline__ void a8_tile_coords(const A8Tiles& t, int i, int& tn,
   tn = w / rows;
 }
 
-// Weight tile, half and first output column of wave w in column tile tn. Gated, waves 4..7
-// take the up rows of waves 0..3.
+// Weight tile, half and first output column of wave w in column tile tn. Gated, the second
+// half of the waves takes the up rows of the first.
 struct A8Wave {
   int tile, b, col;
   bool valid;
@@ -254,12 +260,13 @@ struct A8Wave {
 template <int OUT>
 __device__ __forceinline__ A8Wave a8_wave(const A8Args& a, int tn, int w) {
   if (OUT == A8_GLU) {
-    const int t = 2 * tn + ((w & 3) >> 1);
+    constexpr int kHalf = kA8Waves / 2;
+    const int t = kHalf / 2 * tn + ((w % kHalf) >> 1);
     const bool ok = t * kTileN < a.ld;
     const int gate = ok ? t : a.ld / kTileN - 1;
-    return {gate + (w >> 2) * (a.epi.up / kTileN), w & 1, t * kTileN + 32 * (w & 1), ok};
+    return {gate + (w / kHalf) * (a.epi.up / kTileN), w & 1, t * kTileN + 32 * (w & 1), ok};
   }
-  const int t = 4 * tn + (w >> 1);
+  const int t = kA8Waves / 2 * tn + (w >> 1);
   const bool ok = t * kTileN < a.N;
   return {ok ? t : a.N / kTileN - 1, w & 1, t * kTileN + 32 * (w & 1), ok};
 }
@@ -280,10 +287,10 @@ template <int MB, int OUT>
 __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB][16], u32x4* lds, int m0, int tn,
                                          int wave, int lane) {
   constexpr bool GLU = OUT == A8_GLU;
-  constexpr int kFits = A8Split<MB>::DEPTH * A8Split<MB>::UNITS / 2048;
+  constexpr int kFits = A8Split<MB>::DEPTH * A8Split<MB>::UNITS / (8 * kTileCols);
   constexpr int kPass = kFits < MB ? kFits : MB;   // blocks of 32 KiB at a time
   static_assert(kPass >= 1, "a block fits the buffers");
-  constexpr int kCols = GLU ? 128 : 256, kLanes = kCols / 8, kRows = 64 * kA8Waves / kLanes;
+  constexpr int kCols = GLU ? kTileCols / 2 : kTileCols, kChunks = kTileCols / 4, kLanes = kCols / 8, kRows = 64 * kA8Waves / kLanes;
   const int r = lane & 31, h = lane >> 5;
   const int t = wave * 64 + lane, cl = t % kLanes, rl = t / kLanes;
   const int col = tn * kCols + 8 * cl;
@@ -300,7 +307,7 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
       const float(&v)[16] = acc[p0 + k < MB ? p0 + k : 0];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        lds[(32 * k + r) * 64 + ((8 * wave + 2 * j + h) ^ (r & 15))] =
+        lds[(32 * k + r) * kChunks + ((8 * wave + 2 * j + h) ^ (r & 15))] =
             u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
                   __float_as_uint(v[4 * j + 3])};
     }
@@ -313,7 +320,7 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
       if constexpr (OUT == A8_F32) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          *reinterpret_cast<u32x4*>(static_cast<float*>(a.y) + at + 4 * c) = lds[row * 64 + ((2 * cl + c) ^ (row & 15))];
+          *reinterpret_cast<u32x4*>(static_cast<float*>(a.y) + at + 4 * c) = lds[row * kChunks + ((2 * cl + c) ^ (row & 15))];
       } else {
         u32x4 res = {0u, 0u, 0u, 0u};
         if (a.epi.res) res = *reinterpret_cast<const u32x4*>(a.epi.res + at);
@@ -322,7 +329,7 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
         for (int j = 0; j < (GLU ? 2 : 1); ++j)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const u32x4 w = lds[row * 64 + ((32 * j + 2 * cl + c) ^ (row & 15))];
+            const u32x4 w = lds[row * kChunks + ((kChunks / 2 * j + 2 * cl + c) ^ (row & 15))];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[j][4 * c + i] = __uint_as_float(w[i]) + bias[j][4 * c + i];
           }
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(64 * kA8Waves, 2) void k_a8_tiles(A8Tiles t) {
 template <int MB, int OUT>
 __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   constexpr bool GLU = OUT == A8_GLU;
-  constexpr int kPer = (GLU ? 4 : 8) * MB, NP = GLU ? 2 : 1, kAhead = 4;
+  constexpr int kPer = (GLU ? kA8Waves / 2 : kA8Waves) * MB, NP = GLU ? 2 : 1, kAhead = 4;
   const A8Args& a = t.a;
   const int ts = blockIdx.x / kPer, w = blockIdx.x % kPer / MB, mb = blockIdx.x % MB;
   const int p0 = a8_owner_of(t, ts * a.G), p1 = a8_owner_of(t, ts * a.G + a.G - 1);
@@ -413,7 +420,7 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           v[k][j][i] = __builtin_amdgcn_raw_buffer_load_b128(
-              rs, live ? a8_slot_off(q, which, w + 4 * j, mb, lane) + 1024 * i : 0xfffffff0u, 0, 0);
+              rs, live ? a8_slot_off(q, which, w + kA8Waves / 2 * j, mb, lane) + 1024 * i : 0xfffffff0u, 0, 0);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -505,12 +512,16 @@ int device_cus() {
 template <int OUT, int MB>
 void launch_tiles(const A8Tiles& t, int grid, int nt, hipStream_t s) {
   k_a8_tiles<MB, OUT><<<grid, 64 * kA8Waves, 0, s>>>(t);
-  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? 4 : 8) * MB, 64, 0, s>>>(t);
+  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? kA8Waves / 2 : kA8Waves) * MB, 64, 0, s>>>(t);
 }
 
 template <int OUT>
-int run_tiles(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
-  const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
+int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
+  if (a.M <= 64 && a8_few(OUT, a, device_cus(), s)) {
+    QW4_LAUNCH_CHECK();
+    return QW4_OK;
+  }
+  const int cus = kPerCu * device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
   const bool ws_ok = ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && cus % 8 == 0 &&
                      ws->bytes >= 2ull * cus * kA8SlotBytes;
   A8Plan p = a8_plan(a.M, cols, a.G, 8, cus, ws_ok);
@@ -553,7 +564,7 @@ int check_call(const void* y, const qw4_weights* w, const qw4_a8* a, int T) {
 }
 
 A8Args args_of(void* y, const qw4_weights* w, const qw4_a8* a, int T, const Epilogue& e) {
-  return {w->qweight, w->scale, w->zeros, a->q, a->scale, y, T, w->out_f, w->in_f, w->num_groups,
+  return {w->qweight, w->scale, a->q, a->scale, y, T, w->out_f, w->in_f, w->num_groups,
           a->max_rows, w->out_f - e.up, e};
 }
 
@@ -573,13 +584,13 @@ int qw4_a8_linear(uint16_t* y, const qw4_weights* w, const qw4_a8* a, int T, con
   if (glu && w->out_f % (2 * kTileN)) return QW4_ERR_SHAPE;
   if (((uintptr_t)bias | (uintptr_t)residual) & 15) return QW4_ERR_ALIGN;
   const A8Args g = args_of(y, w, a, T, Epilogue{bias, residual, act, glu ? w->out_f / 2 : 0});
-  return glu ? run_tiles<A8_GLU>(g, ws, (hipStream_t)stream) : run_tiles<A8_EPI>(g, ws, (hipStream_t)stream);
+  return glu ? run<A8_GLU>(g, ws, (hipStream_t)stream) : run<A8_EPI>(g, ws, (hipStream_t)stream);
 }
 
 int qw4_a8_linear_f32(float* y, const qw4_weights* w, const qw4_a8* a, int T, qw4_workspace* ws, void* stream) {
   const int st = check_call(y, w, a, T);
   if (st) return st;
-  return run_tiles<A8_F32>(args_of(y, w, a, T, Epilogue{}), ws, (hipStream_t)stream);
+  return run<A8_F32>(args_of(y, w, a, T, Epilogue{}), ws, (hipStream_t)stream);
 }
 
 }  // extern "C"
