@@ -517,7 +517,7 @@ void launch_tiles(const A8Tiles& t, int grid, int nt, hipStream_t s) {
 
 template <int OUT>
 int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
-  if (a.M <= 64 && a8_few(OUT, a, device_cus(), s)) {
+  if (a8_few(OUT, a, device_cus(), s)) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
