@@ -52,7 +52,7 @@ struct A8Split {
   static constexpr int LOADS = ACT + 1 + 7;        // codes, scales, weights (2 + 4 + 1)
   static constexpr int CODES = 32 * MB * 8;        // 16-byte units of a buffer's codes
   static constexpr int UNITS = CODES + kA8Waves * 16;   // and of its scales, 64 a wave's load
-  static_assert(MB % 2 == 0 && MB <= 8, "whole loads a wave");
+  static_assert(4 * MB % kA8Waves == 0 && 32 * MB <= 64 * kA8Waves, "whole loads a wave");
 };
 
 struct A8Tiles {
@@ -114,7 +114,7 @@ __device__ __forceinline__ void a8_load_rows(const A8Args& a, const A8Rows& x, u
                                              (uint32_t)(8 * rb) * (uint32_t)a.K + (uint32_t)g * kGroup, 0, 0);
   } else {   // 64 scales a wave; those past the tile's rows from a resource of no length
     const __amdgpu_buffer_rsrc_t rs =
-        a8_rsrc(x.scale + (size_t)g * a.max_rows, some && wave < MB / 2 ? x.rows * 4u : 0u);
+        a8_rsrc(x.scale + (size_t)g * a.max_rows, some && wave < (MB + 1) / 2 ? x.rows * 4u : 0u);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, buf + Sp::CODES + wave * 16, 4, (uint32_t)(wave * 64 + lane) * 4u, 0, 0, 0);
   }
 }
@@ -461,38 +461,44 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   }
 }
 
-// How a call is cut: tiles of 32 mb rows, schedule (0 whole tiles, 1 all units over one
-// workgroup a CU, 2 whole rounds and the rest split, 3 every tile in S slices) and its
-// cost in group steps of 256 rows.
+// How a call is cut: tiles of 32 mb rows; schedule 0 whole tiles, 2 whole rounds and the
+// rest's units spread over all workgroups, 3 every tile in S slices; estimated us.
 struct A8Plan {
   int mb, tiles_n, tiles_m, pick, S;
   double cost;
 };
 
-double a8_step(int mb) { return 0.2 + 0.1 * mb; }
-
-A8Plan a8_plan(int M, int cols, long long G, int mb, int cus, bool ws_ok) {
-  A8Plan p{mb, (cols + kTileCols - 1) / kTileCols, (M + 32 * mb - 1) / (32 * mb), 0, 0, 0.};
-  const long long nt = (long long)p.tiles_n * p.tiles_m, rem = nt % cus;
-  const double t_dp = (double)((nt + cus - 1) / cus) * G, work = (double)nt * G / cus;
-  p.cost = t_dp;
-  ws_ok = ws_ok && rem != 0 && nt * G < (1LL << 31);
-  if (ws_ok) {
-    double best = 0.95 * t_dp;
-    auto take = [&](bool ok, int pick, double c) {
-      if (ok && c < best) {
-        p.pick = pick;
-        p.cost = best = c;
-      }
-    };
-    take(nt * G >= 2LL * cus, 1, work + 16.0 + 0.1 * ((cus + nt - 1) / nt + 1));
-    take(nt > cus && rem * G >= cus, 2, work + 8.0 + 0.1 * ((cus + rem - 1) / rem + 1));
-    int S = 2 * nt <= cus ? (int)std::min<long long>(cus / nt, G >= 8 ? G / 4 : G / 2) : 0;
-    while (S >= 2 && (nt * S) % 8) --S;
-    take(S >= 2, 3, (double)G / (S > 0 ? S : 1) + 8.0 + 0.1 * S);
-    p.S = S;
+// The best cut of tiles of mb rows. The estimate's figures are fitted to 3000 timed calls on
+// MI355X (7 projections from 5120x2176 to 34816x5120, 33 to 4096 rows, every mb, schedule and
+// S): the pick is 1.1% (geometric mean) from the fastest of all, 27% at worst (128 rows and
+// fewer of 5120x4096). A (tile, group) step takes 0.27 + 0.14 mb us with one workgroup on a
+// CU and 0.29 + 0.23 mb with two; storing a tile 0.66 mb; slices 4.6 for the second kernel,
+// their partial tiles' traffic and 0.45 for each piece of a sum. All units over all workgroups
+// (ranges that begin and end anywhere) was the fastest by 0.3% in the mean and is not kept.
+A8Plan a8_plan(int M, int cols, int G, int mb, int cus, bool ws_ok) {
+  A8Plan p{mb, (cols + kTileCols - 1) / kTileCols, (M + 32 * mb - 1) / (32 * mb), 0, 1, 0.};
+  const long long nt = (long long)p.tiles_n * p.tiles_m, most = kPerCu * cus, rem = nt % most;
+  const double one = 0.27 + 0.14 * mb, two = 0.29 + 0.23 * mb, store = 0.66 * mb;
+  auto whole = [&](long long tiles) {   // of the CU with most tiles, two at a time
+    const long long n = (tiles + cus - 1) / cus;
+    return (double)(n / 2) * (G * two + store) + (double)(n % 2) * (G * one + store);
+  };
+  p.cost = whole(nt);
+  if (!ws_ok || nt * G >= (1LL << 31)) return p;
+  auto take = [&](int pick, int S, double c) {
+    if (c < p.cost) {
+      p.pick = pick;
+      p.S = S;
+      p.cost = c;
+    }
+  };
+  if (nt > most && rem && rem * G >= most) take(2, 1, whole(nt - rem) + (double)rem * G / most * two + 7.0 + 3.3 * mb);
+  for (int S = 2; S <= 64 && nt * S <= most && 2 * S <= G; ++S) {
+    const long long P = nt * S;
+    if (P % 8) continue;   // runs of workgroups on each XCD
+    const int steps = (G + S - 1) / S;
+    take(3, S, steps * (P <= cus ? one : two) + 4.6 + 1.63 * (double)P / most * mb + 0.45 * S);
   }
-  p.cost *= a8_step(mb);
   return p;
 }
 
@@ -521,13 +527,13 @@ int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
-  const int cus = kPerCu * device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
+  const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
   const bool ws_ok = ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && cus % 8 == 0 &&
-                     ws->bytes >= 2ull * cus * kA8SlotBytes;
+                     ws->bytes >= 2ull * kPerCu * cus * kA8SlotBytes;
   A8Plan p = a8_plan(a.M, cols, a.G, 8, cus, ws_ok);
-  for (int mb = 6; mb >= 2; mb -= 2) {
+  for (int mb = 6; mb >= 1; --mb) {
     const A8Plan q = a8_plan(a.M, cols, a.G, mb, cus, ws_ok);
-    if (q.cost < 0.97 * p.cost) p = q;
+    if (q.cost < p.cost) p = q;
   }
   const long long tiles = (long long)p.tiles_n * p.tiles_m;
   if (tiles > 0x7fffffffLL / 64) return QW4_ERR_SHAPE;
@@ -536,14 +542,17 @@ int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
   int grid = nt;
   if (p.pick) {
     t.slots = static_cast<float*>(ws->buf);
-    t.P = grid = p.pick == 3 ? nt * p.S : cus;
-    t.full = p.pick == 2 ? nt - nt % cus : 0;
+    t.P = grid = p.pick == 3 ? nt * p.S : kPerCu * cus;
+    t.full = p.pick == 2 ? nt - nt % (kPerCu * cus) : 0;
     t.U = (nt - t.full) * a.G;
     t.map = p.pick == 3 ? 2 : 1;
   }
   switch (p.mb) {
+    case 1: launch_tiles<OUT, 1>(t, grid, nt, s); break;
     case 2: launch_tiles<OUT, 2>(t, grid, nt, s); break;
+    case 3: launch_tiles<OUT, 3>(t, grid, nt, s); break;
     case 4: launch_tiles<OUT, 4>(t, grid, nt, s); break;
+    case 5: launch_tiles<OUT, 5>(t, grid, nt, s); break;
     case 6: launch_tiles<OUT, 6>(t, grid, nt, s); break;
     default: launch_tiles<OUT, 8>(t, grid, nt, s);
   }
