@@ -5,13 +5,21 @@
 //   m       the largest so far (the same in all lanes),
 //   s       per lane, sum of exp(x - m) without the one element that is m (`own`: it was
 //           this lane's),
-//   u       per lane, sum of exp(x - m) (x - m),
-//   a list  the top_k best (value, index) so far, lane j the j-th.
+//   u       per lane, sum of exp(x - m) (x - m).
 // With total = 1 + s:  L = m + log1p(s),  H = log1p(s) - u / (1 + s). Without the
 // largest element s keeps its relative precision when that token is all but certain,
 // where 1 + s would lose it and both results are about s.
-// A block whose largest value beats neither m nor the list's last entry, which is nearly
-// every one after the first few, costs one comparison a lane for all of that.
+//
+// Alternatives: a lane keeps the six largest maxima of its eights as keys (the upper 16
+// bits of the value, ordered, over the block's number): 2 vector instructions a logit,
+// no branch. At the end the k-th largest of the lanes' first keys bounds the k-th largest
+// logit from below, and one wave reads the eights whose key reaches it again, some k of them.
+// Where a lane's sixth key reaches it, there may have been a seventh: then the waves go over
+// their blocks once more and keep lists (sorted or constant rows). 1000 x 248320 bf16 logits
+// take 103 us at k = 5, 20 and 32, and 92 without alternatives; with lists kept from the start
+// they took 138 / 207 / 245; with four keys one row of some 500 went over its blocks again at
+// k = 32, and its workgroup alone lengthened the launch to 212 us (five: 149).
+//
 // Rows split over workgroups, for few rows, write (m, s, u, list) to the workspace and
 // a second kernel joins them in order; nothing depends on which workgroup comes first.
 #include <hip/hip_runtime.h>
@@ -37,6 +45,7 @@ struct LpArgs {
   float *lp, *entropy, *top_lp;
   int32_t* top_ids;
   int n, asked, k, S;
+  int few;             // a wave's blocks are fewer than 2^16, the row's than 2^24
   uint32_t* part;      // [T][S] records of 4 + 2 k words
 };
 
@@ -47,15 +56,46 @@ struct LpStats {
 __device__ __forceinline__ float lane_value(float v, int l) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return lane_value(v, 0);
+// v of lane (lane ^ X), in registers (through LDS, as shuffles go, a step of the networks
+// below waits 5 times as long).
+template <int X>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
+  if constexpr (X == 1) return dpp<0xB1>(v);                // quad_perm [1, 0, 3, 2]
+  if constexpr (X == 2) return dpp<0x4E>(v);                // quad_perm [2, 3, 0, 1]
+  if constexpr (X == 4) return dpp<0x1B>(dpp<0x141>(v));    // half rows mirrored, fours mirrored
+  if constexpr (X == 8) return dpp<0x128>(v);               // rows rotated by 8
+  if constexpr (X == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? p[0] : p[1];
+  }
+  if constexpr (X == 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? p[0] : p[1];
+  }
+}
+template <int X>
+__device__ __forceinline__ float lane_xor(float v, int lane) {
+  return __uint_as_float(lane_xor<X>(__float_as_uint(v), lane));
+}
+__device__ __forceinline__ float wave_sum(float v, int lane) {
+  v += lane_xor<1>(v, lane);
+  v += lane_xor<2>(v, lane);
+  v += lane_xor<4>(v, lane);
+  v += lane_xor<8>(v, lane);
+  v += lane_xor<16>(v, lane);
+  return v + lane_xor<32>(v, lane);
+}
+__device__ __forceinline__ float wave_max(float v, int lane) {
+  v = fmaxf(v, lane_xor<1>(v, lane));
+  v = fmaxf(v, lane_xor<2>(v, lane));
+  v = fmaxf(v, lane_xor<4>(v, lane));
+  v = fmaxf(v, lane_xor<8>(v, lane));
+  v = fmaxf(v, lane_xor<16>(v, lane));
+  return lane_value(fmaxf(v, lane_xor<32>(v, lane)), 0);
 }
 // exp(d), d <= 0; its argument's rounding, |d| 2^-24, is the d's own.
 __device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.4426950408889634f); }
@@ -79,31 +119,36 @@ struct LpList {
   float v = -INFINITY;
   int i = -1;
 
-  // One step of a bitonic network: a lane and its partner `stride` off keep the first
+  // One step of a bitonic network: a lane and its partner STRIDE off keep the first
   // (upper) or the other of their two entries.
-  __device__ __forceinline__ void exchange(int stride, bool upper) {
-    const float w = __shfl_xor(v, stride, 64);
-    const int j = __shfl_xor(i, stride, 64);
+  template <int STRIDE>
+  __device__ __forceinline__ void exchange(bool upper, int lane) {
+    const float w = lane_xor<STRIDE>(v, lane);
+    const int j = (int)lane_xor<STRIDE>((uint32_t)i, lane);
     if (lp_first(v, i, w, j) != upper) {
       v = w;
       i = j;
     }
   }
-  __device__ __forceinline__ void settle(int lane) {   // sorts a bitonic sequence
-#pragma unroll
-    for (int stride = 32; stride > 0; stride >>= 1) exchange(stride, (lane & stride) == 0);
+  // Steps of strides STRIDE, STRIDE / 2, ... 1 within runs of SIZE entries, every other run
+  // the other way round.
+  template <int SIZE, int STRIDE>
+  __device__ __forceinline__ void runs(int lane) {
+    exchange<STRIDE>((SIZE == 64 || (lane & SIZE) == 0) == ((lane & STRIDE) == 0), lane);
+    if constexpr (STRIDE > 1) runs<SIZE, STRIDE / 2>(lane);
   }
+  __device__ __forceinline__ void settle(int lane) { runs<64, 32>(lane); }   // sorts a bitonic sequence
   __device__ __forceinline__ void sort(int lane) {
-#pragma unroll
-    for (int size = 2; size < 64; size <<= 1)
-#pragma unroll
-      for (int stride = size >> 1; stride > 0; stride >>= 1)
-        exchange(stride, ((lane & size) == 0) == ((lane & stride) == 0));
+    runs<2, 1>(lane);
+    runs<4, 2>(lane);
+    runs<8, 4>(lane);
+    runs<16, 8>(lane);
+    runs<32, 16>(lane);
     settle(lane);
   }
   // The best 64 of this sorted list and another.
   __device__ __forceinline__ void merge(const LpList& o, int lane) {
-    const float w = __shfl(o.v, 63 - lane, 64);
+    const float w = __shfl(o.v, 63 - lane, 64);   // reversed
     const int j = __shfl(o.i, 63 - lane, 64);
     if (lp_first(w, j, v, i)) {
       v = w;
@@ -130,41 +175,53 @@ struct LpSlot {
   int i;
 };
 
+constexpr int kLpKeys = 6;   // eights that a lane remembers
+
+// A maximum's order in 16 bits (larger: larger, or equal up to the bits cut off; -Inf and
+// below: at most kLpNone), and the least value of that order.
+constexpr uint32_t kLpNone = 0x7f;
+__device__ __forceinline__ uint32_t lp_order(float v) {
+  const int b = __float_as_int(v + 0.f);   // -0 as 0
+  return (uint32_t)(b ^ ((b >> 31) | (int)0x80000000)) >> 16;
+}
+__device__ __forceinline__ float lp_least(uint32_t order) {
+  const uint32_t u = order << 16;
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+
 template <bool TOP>
 struct LpWave {
   float m = -INFINITY;
   float s = 0.f, u = 0.f, own = 0.f;
+  uint32_t key[kLpKeys] = {};   // descending
   LpList list;
-  float last = -INFINITY;   // the list's k-th value, which a later element has to beat
+  float last = -INFINITY;       // the list's k-th entry, which another has to beat
   int last_i = -1;
 
-  // Elements x[e] with indices at(e), rising with e and over a wave's calls; -Inf where
-  // there is none.
-  template <int N, class At>
-  __device__ __forceinline__ void take(const float (&x)[N], const At& at, int k, int lane, LpSlot* slots) {
-    float top = x[0];
+  // Elements x[e] of the lane (-Inf where there is none): their share of the sums, and their
+  // maximum.
+  template <int N>
+  __device__ __forceinline__ float add(const float (&x)[N], int lane) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-    if (__ballot(top > (TOP ? last : m))) {
-      if (TOP) choose(x, at, k, lane, top, slots);
-      if (__ballot(top > m)) {
-        const float to = wave_max(top);
-        lp_rescale(s, u, own, m, to);
-        m = to;
-        bool mine = lane == __builtin_ctzll(__ballot(top == to));
-        own = mine ? 1.f : 0.f;
+    for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
+    if (__ballot(top > m)) {
+      const float to = wave_max(top, lane);
+      lp_rescale(s, u, own, m, to);
+      m = to;
+      bool mine = lane == __builtin_ctzll(__ballot(top == to));
+      own = mine ? 1.f : 0.f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float d = x[e] - m, p = lp_exp(d);
-          if (mine && x[e] == to) {
-            mine = false;   // m itself stays out of s
-          } else {
-            s += p;
-            u = __builtin_fmaf(p, lp_far(d), u);
-          }
+      for (int e = 0; e < N; ++e) {
+        const float d = x[e] - m, p = lp_exp(d);
+        if (mine && x[e] == to) {
+          mine = false;   // m itself stays out of s
+        } else {
+          s += p;
+          u = __builtin_fmaf(p, lp_far(d), u);
         }
-        return;
       }
+      return top;
     }
     const float ref = m > -INFINITY ? m : 0.f;   // nothing but -Inf so far: they add nothing
 #pragma unroll
@@ -173,23 +230,31 @@ struct LpWave {
       s += p;
       u = __builtin_fmaf(p, lp_far(d), u);
     }
+    return top;
   }
 
-  // The block's elements into the list. While that is empty, only those from the k-th
-  // largest of the lanes' own largest on: at least k are, and few more. Many at once are
-  // gathered and sorted (27 steps of a network), a few put in one by one.
+  __device__ __forceinline__ void remember(float top, uint32_t number) {
+    const uint32_t k = (lp_order(top) << 16) | number;
+#pragma unroll
+    for (int l = kLpKeys - 1; l > 0; --l) key[l] = max(key[l], min(key[l - 1], k));
+    key[0] = max(key[0], k);
+  }
+
+  __device__ __forceinline__ void close(int k) {
+    last = lane_value(list.v, k - 1);
+    last_i = __builtin_amdgcn_readlane(list.i, k - 1);
+  }
+
+  // Elements x[e] with indices at(e), rising with e, into the list: while that is empty,
+  // only those from `least` on, which k are at least. Many at once are gathered and sorted, a
+  // few put in one by one.
   template <int N, class At>
-  __device__ __forceinline__ void choose(const float (&x)[N], const At& at, int k, int lane, float top,
+  __device__ __forceinline__ void choose(const float (&x)[N], const At& at, int k, int lane, float least,
                                          LpSlot* slots) {
-    float least = -INFINITY;
-    if (lane_value(list.v, 0) == -INFINITY) {
-      int rank = 0;
-      for (int l = 0; l < 64; ++l) {
-        const float o = lane_value(top, l);
-        rank += o > top || (o == top && l < lane);
-      }
-      least = wave_max(rank == k - 1 ? top : -INFINITY);
-    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
+    if (!__ballot(top >= last && top > -INFINITY)) return;
     auto wanted = [&](float v, int i) { return v >= least && v > -INFINITY && lp_first(v, i, last, last_i); };
     int count = 0, mine[N];
 #pragma unroll
@@ -209,11 +274,11 @@ struct LpWave {
         more.v = slots[lane].v;
         more.i = slots[lane].i;
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
       more.sort(lane);
       list.merge(more, lane);
-      last = lane_value(list.v, k - 1);
-      last_i = __builtin_amdgcn_readlane(list.i, k - 1);
+      close(k);
       return;
     }
     uint32_t done = 0;   // elements of this lane that are in the list
@@ -231,13 +296,23 @@ struct LpWave {
       if (!some) break;
       const int from = __builtin_ctzll(some);
       list.insert(lane_value(b, from), __builtin_amdgcn_readlane(bi, from), lane);
-      last = lane_value(list.v, k - 1);
-      last_i = __builtin_amdgcn_readlane(list.i, k - 1);
+      close(k);
       if (lane == from) done |= 1u << be;
     }
   }
 
-  __device__ __forceinline__ LpStats stats() const { return {m, wave_sum(s), wave_sum(u)}; }
+  // The k-th largest of the lanes' `top` while the list is empty.
+  __device__ __forceinline__ float first_least(float top, int k, int lane) const {
+    if (lane_value(list.v, 0) > -INFINITY) return -INFINITY;
+    int rank = 0;
+    for (int l = 0; l < 64; ++l) {
+      const float o = lane_value(top, l);
+      rank += o > top || (o == top && l < lane);
+    }
+    return wave_max(rank == k - 1 ? top : -INFINITY, lane);
+  }
+
+  __device__ __forceinline__ LpStats stats(int lane) const { return {m, wave_sum(s, lane), wave_sum(u, lane)}; }
 };
 
 // The statistics of two disjoint sets: the largest of both stays out of s once.
@@ -286,6 +361,8 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
   constexpr int kParts = kLpBlock / 64 / kVec;  // 16-byte loads of a block
   __shared__ LpSlot slots[kLpWaves][64];
   __shared__ LpStats parts[kLpWaves];
+  __shared__ uint32_t keys[TOP ? kLpKeys : 1][64 * kLpWaves];
+  __shared__ int again;   // the keys do not tell
   const int row = blockIdx.x / a.S, split = blockIdx.x - row * a.S;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const T* xr = static_cast<const T*>(a.x) + (size_t)row * a.ld;
@@ -294,55 +371,145 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
   const u32x4* xv = reinterpret_cast<const u32x4*>(xr + head);
   const int vecs = (a.n - head) / kVec, tail = head + vecs * kVec;
   const int blocks = (vecs + 64 * kParts - 1) / (64 * kParts);
+  const int b0 = split * kLpWaves + wave, step = kLpWaves * a.S;
   LpWave<TOP> w;
-  auto few = [&](int first, int count) {   // < 8 logits one by one
-    const float x[1] = {lane < count ? lp_logit(xr + first + lane) : -INFINITY};
-    w.take(x, [&](int) { return first + lane; }, a.k, lane, slots[wave]);
-  };
-  const bool ends = split == 0 && wave == 0;
-  if (ends && head) few(0, head);
-  const int step = kLpWaves * a.S;
-  for (int b0 = split * kLpWaves + wave; b0 < blocks; b0 += kLpAhead * step) {
-    u32x4 v[kLpAhead][kParts];
+  // the eight that lane `of` has in block b: its 16-byte parts (past the row's, some other),
+  // its logits, and their indices
+  auto load = [&](u32x4 (&v)[kParts], int b, int of) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < kLpAhead; ++d)
-#pragma unroll
-      for (int p = 0; p < kParts; ++p) {
-        const long long i = ((long long)(b0 + d * step) * kParts + p) * 64 + lane;
-        v[d][p] = xv[i < vecs ? i : 0];
-      }
-#pragma unroll
-    for (int d = 0; d < kLpAhead; ++d) {
-      const int b = b0 + d * step;
-      if (b >= blocks) break;
-      float x[8];
-#pragma unroll
-      for (int p = 0; p < kParts; ++p) {
-        const bool in = (b * kParts + p) * 64 + lane < vecs;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if constexpr (sizeof(T) == 4) {
-            x[p * 4 + c] = in ? __uint_as_float(v[d][p][c]) : -INFINITY;
-          } else {
-            x[2 * c] = in ? bf16_bits_to_f32(v[d][p][c] & 0xffffu) : -INFINITY;
-            x[2 * c + 1] = in ? bf16_bits_to_f32(v[d][p][c] >> 16) : -INFINITY;
-          }
-      }
-      w.take(x, [&](int e) { return head + ((b * kParts + e / kVec) * 64 + lane) * kVec + e % kVec; }, a.k, lane,
-             slots[wave]);
+    for (int p = 0; p < kParts; ++p) {
+      const long long i = ((long long)b * kParts + p) * 64 + of;
+      v[p] = xv[i < vecs ? i : 0];
     }
-  }
-  if (ends && tail < a.n) few(tail, a.n - tail);
-  const LpStats mine = w.stats();
+  };
+  auto values = [&](float (&x)[8], const u32x4 (&v)[kParts], int b, int of) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const bool in = ((long long)b * kParts + p) * 64 + of < vecs;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if constexpr (sizeof(T) == 4) {
+          x[p * 4 + c] = in ? __uint_as_float(v[p][c]) : -INFINITY;
+        } else {
+          x[2 * c] = in ? bf16_bits_to_f32(v[p][c] & 0xffffu) : -INFINITY;
+          x[2 * c + 1] = in ? bf16_bits_to_f32(v[p][c] >> 16) : -INFINITY;
+        }
+    }
+  };
+  auto index = [&](int b, int of, int e) { return head + ((b * kParts + e / kVec) * 64 + of) * kVec + e % kVec; };
+  // use(x, block, number) for the wave's blocks, kLpAhead of them read at a time
+  auto scan = [&](const auto& use) __attribute__((always_inline)) {
+    for (int b = b0, number = 0; b < blocks; b += kLpAhead * step, number += kLpAhead) {
+      u32x4 v[kLpAhead][kParts];
+#pragma unroll
+      for (int d = 0; d < kLpAhead; ++d) load(v[d], min(b + d * step, blocks - 1), lane);
+#pragma unroll
+      for (int d = 0; d < kLpAhead; ++d) {
+        if (b + d * step >= blocks) break;
+        float x[8];
+        values(x, v[d], b + d * step, lane);
+        use(x, b + d * step, (uint32_t)(number + d));
+      }
+    }
+  };
+  scan([&](const float (&x)[8], int, uint32_t number) __attribute__((always_inline)) {
+    const float top = w.add(x, lane);
+    if (TOP) w.remember(top, number);
+  });
+  const LpStats mine = w.stats(lane);
   if (lane == 0) parts[wave] = mine;
-  if (TOP) slots[wave][lane] = {w.list.v, w.list.i};
+  if constexpr (TOP) {
+#pragma unroll
+    for (int l = 0; l < kLpKeys; ++l) keys[l][threadIdx.x] = w.key[l];
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t key[kLpKeys][kLpWaves], t = 0;
+#pragma unroll
+      for (int l = 0; l < kLpKeys; ++l)
+#pragma unroll
+        for (int o = 0; o < kLpWaves; ++o) key[l][o] = keys[l][64 * o + lane];
+      // the order that the first keys of k lanes reach; at least that of a number
+#pragma unroll
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        int count = 0;
+#pragma unroll
+        for (int o = 0; o < kLpWaves; ++o) count += __popcll(__ballot(key[0][o] >= c << 16));
+        if (count >= a.k) t = c;
+      }
+      t = max(t, kLpNone + 1) << 16;
+      // the eights whose key reaches it, a lane each
+      bool fits = a.few;
+      int count = 0;
+#pragma unroll
+      for (int l = 0; l < kLpKeys; ++l)
+#pragma unroll
+        for (int o = 0; o < kLpWaves; ++o) {
+          const unsigned long long some = __ballot(key[l][o] >= t);
+          if (l == kLpKeys - 1 && some) fits = false;
+          if (some) {
+            const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+            if (key[l][o] >= t && at < 64)
+              slots[0][at].i = (int)(((key[l][o] & 0xffffu) * (uint32_t)step + (uint32_t)(split * kLpWaves + o)) * 64u) + lane;
+            count += __popcll(some);
+          }
+        }
+      if (fits && count <= 64) {
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const bool has = lane < count;
+        const int place = has ? slots[0][lane].i : 0, b = place >> 6, of = place & 63;   // block, its lane
+        __builtin_amdgcn_wave_barrier();
+        u32x4 v[kParts];
+        float x[8];
+        load(v, b, of);
+        values(x, v, b, of);
+        const float least = lp_least(t >> 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = has && x[e] >= least ? x[e] : -INFINITY;
+        w.choose(x, [&](int e) { return index(b, of, e); }, a.k, lane, least, slots[0]);
+      } else {
+        fits = false;
+      }
+      if (lane == 0) again = !fits || count > 64;
+    }
+    __syncthreads();
+    if (again)
+      scan([&](const float (&x)[8], int b, uint32_t) __attribute__((always_inline)) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+        if (__ballot(top > w.last))
+          w.choose(x, [&](int e) { return index(b, lane, e); }, a.k, lane, w.first_least(top, a.k, lane), slots[wave]);
+      });
+    if (again) slots[wave][lane] = {w.list.v, w.list.i};
+  }
   __syncthreads();
   if (wave) return;
   LpStats t = parts[0];
 #pragma unroll
-  for (int o = 1; o < kLpWaves; ++o) {
-    t = lp_join(t, parts[o]);
-    if (TOP) w.list.merge({slots[o][lane].v, slots[o][lane].i}, lane);
+  for (int o = 1; o < kLpWaves; ++o) t = lp_join(t, parts[o]);
+  if constexpr (TOP) {
+    if (again) {
+#pragma unroll
+      for (int o = 1; o < kLpWaves; ++o) w.list.merge({slots[o][lane].v, slots[o][lane].i}, lane);
+      w.close(a.k);
+    }
+  }
+  if (split == 0) {   // the ends, less than 8 logits each
+    w.m = t.m;
+    w.s = lane == 0 ? t.s : 0.f;
+    w.u = lane == 0 ? t.u : 0.f;
+    w.own = lane == 0 && t.m > -INFINITY ? 1.f : 0.f;
+#pragma unroll
+    for (int end = 0; end < 2; ++end) {
+      const int first = end ? tail : 0, count = end ? a.n - tail : head;
+      if (count <= 0) continue;
+      const float x[1] = {lane < count ? lp_logit(xr + first + lane) : -INFINITY};
+      w.add(x, lane);
+      if (TOP) w.choose(x, [&](int) { return first + lane; }, a.k, lane, -INFINITY, slots[0]);
+    }
+    t = w.stats(lane);
   }
   if (a.S == 1) {
     lp_write<T>(a, row, t, w.list, lane);
@@ -391,12 +558,13 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
   if (wave == 0) lp_write<T>(a, row, t, list, lane);
 }
 
-// Workgroups a row is split over: none from 512 rows on; else up to about 512 workgroups,
-// of at least two blocks a wave.
+// Workgroups a row is split over: one from 640 rows on; else some 1024 workgroups, of at least
+// two blocks a wave. 256 / 400 rows of 248320 bf16 logits: 40 / 54 us, with some 512 workgroups
+// 46 / 68, with 2048 42 / 54; 64 rows 22, 22 and 25; 1000 rows 103 whole, 112 in two.
 int lp_splits(int T, int n) {
   const long long blocks = ((long long)n + kLpBlock - 1) / kLpBlock;
   const long long most = blocks / (2 * kLpWaves);
-  const long long want = T >= 512 ? 1 : 512 / T;
+  const long long want = T >= 640 ? 1 : (1024 + T - 1) / T;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
@@ -417,7 +585,8 @@ int logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const T
                                    (uintptr_t)targets) & 3)
     return QW4_ERR_ALIGN;
   const size_t need = lp_bytes(T_, n, k);
-  LpArgs a{x, ld, targets, lp, entropy, top_lp, top_ids, n, asked, k, lp_splits(T_, n), nullptr};
+  LpArgs a{x, ld, targets, lp, entropy, top_lp, top_ids, n, asked, k, lp_splits(T_, n), 0, nullptr};
+  a.few = (long long)n / kLpBlock < (1 << 24) && (long long)n / kLpBlock / (kLpWaves * a.S) < 65500;
   if (need) {
     if (!ws || !ws->buf || ws->bytes < need) return QW4_ERR_SCRATCH;
     if ((uintptr_t)ws->buf & 15) return QW4_ERR_ALIGN;
