@@ -391,14 +391,18 @@ __global__ __launch_bounds__(64 * kA8Waves, 2) void k_a8_tiles(A8Tiles t) {
   }
 }
 
-// The cut tiles: a wave sums one block (wave w, m-block mb; gated: gate and up) over its
-// pieces, in order, kAhead of them loaded at a time, and stores it.
+// The cut tiles: a wave sums a quarter of a block (wave w, m-block mb, 8 j .. 8 j + 7 of its
+// columns; gated: of gate and up) over its pieces, in order, kAhead of them loaded at a time,
+// and stores it.
+constexpr int kA8Quarters = 4;
+
 template <int MB, int OUT>
 __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   constexpr bool GLU = OUT == A8_GLU;
-  constexpr int kPer = (GLU ? kA8Waves / 2 : kA8Waves) * MB, NP = GLU ? 2 : 1, kAhead = 4;
+  constexpr int kPer = (GLU ? kA8Waves / 2 : kA8Waves) * MB * kA8Quarters, NP = GLU ? 2 : 1, kAhead = 12;
   const A8Args& a = t.a;
-  const int ts = blockIdx.x / kPer, w = blockIdx.x % kPer / MB, mb = blockIdx.x % MB;
+  const int ts = blockIdx.x / kPer, part = blockIdx.x % kPer;
+  const int j = part % kA8Quarters, mb = part / kA8Quarters % MB, w = part / (kA8Quarters * MB);
   const int p0 = a8_owner_of(t, ts * a.G), p1 = a8_owner_of(t, ts * a.G + a.G - 1);
   if (p0 == p1) return;   // stored whole
   int tn, tm;
@@ -407,57 +411,46 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   const int lane = threadIdx.x, r = lane & 31, h = lane >> 5, m = tm * 32 * MB + 32 * mb + r;
   if (!wv.valid || tm * 32 * MB + 32 * mb >= a.M) return;
   const __amdgpu_buffer_rsrc_t rs = a8_rsrc(t.slots, 2u * t.P * kA8SlotBytes);
-  float acc[NP][16] = {};
+  float acc[NP][4] = {};
   for (int pp = p0; pp <= p1; pp += kAhead) {
-    u32x4 v[kAhead][NP][4];
+    u32x4 v[kAhead][NP];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int q = pp + k;
-      const bool live = q <= p1;   // others read out of range, without memory
+      const bool live = q <= p1;   // others read out of range: zeros, without memory
       const int which = live && a8_range_start(t, q) / a.G == ts ? 0 : 1;
 #pragma unroll
-      for (int j = 0; j < NP; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[k][j][i] = __builtin_amdgcn_raw_buffer_load_b128(
-              rs, live ? a8_slot_off(q, which, w + kA8Waves / 2 * j, mb, lane) + 1024 * i : 0xfffffff0u, 0, 0);
+      for (int p = 0; p < NP; ++p)
+        v[k][p] = __builtin_amdgcn_raw_buffer_load_b128(
+            rs, live ? a8_slot_off(q, which, w + kA8Waves / 2 * p, mb, lane) + 1024 * j : 0xfffffff0u, 0, 0);
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (pp + k > p1) break;
+    for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-      for (int j = 0; j < NP; ++j)
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[j][i] += __uint_as_float(v[k][j][i >> 2][i & 3]);
-    }
+        for (int i = 0; i < 4; ++i) acc[p][i] += __uint_as_float(v[k][p][i]);
   }
   if (m >= a.M) return;
+  const int col = wv.col + 8 * j + 4 * h;
+  const size_t at = (size_t)m * a.ld + col;
   if constexpr (OUT == A8_F32) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + (size_t)m * a.ld + wv.col + 8 * j + 4 * h) =
-          f32x4{acc[0][4 * j], acc[0][4 * j + 1], acc[0][4 * j + 2], acc[0][4 * j + 3]};
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = f32x4{acc[0][0], acc[0][1], acc[0][2], acc[0][3]};
   } else {
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+    for (int p = 0; p < NP; ++p) {
+      u32x2 bv = {0u, 0u};
+      if (a.epi.bias) bv = *reinterpret_cast<const u32x2*>(a.epi.bias + p * a.epi.up + col);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x2 bv = {0u, 0u};
-        if (a.epi.bias) bv = *reinterpret_cast<const u32x2*>(a.epi.bias + p * a.epi.up + wv.col + 8 * j + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[p][4 * j + i] += bf16_bits_to_f32((bv[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-      }
-    epilogue_act<GLU>(acc, a.epi.act);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const size_t at = (size_t)m * a.ld + wv.col + 8 * j + 4 * h;
-      u32x2 q = {0u, 0u};
-      if (a.epi.res) q = *reinterpret_cast<const u32x2*>(a.epi.res + at);
-      const float* f = &acc[0][4 * j];
-      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + at) =
-          u32x2{pack_bf16x2(f[0] + bf16_bits_to_f32(q[0] & 0xffffu), f[1] + bf16_bits_to_f32(q[0] >> 16)),
-                pack_bf16x2(f[2] + bf16_bits_to_f32(q[1] & 0xffffu), f[3] + bf16_bits_to_f32(q[1] >> 16))};
+      for (int i = 0; i < 4; ++i) acc[p][i] += bf16_bits_to_f32((bv[i >> 1] >> (16 * (i & 1))) & 0xffffu);
     }
+    epilogue_act<GLU>(acc, a.epi.act);
+    u32x2 q = {0u, 0u};
+    if (a.epi.res) q = *reinterpret_cast<const u32x2*>(a.epi.res + at);
+    const float* f = acc[0];
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + at) =
+        u32x2{pack_bf16x2(f[0] + bf16_bits_to_f32(q[0] & 0xffffu), f[1] + bf16_bits_to_f32(q[0] >> 16)),
+              pack_bf16x2(f[2] + bf16_bits_to_f32(q[1] & 0xffffu), f[3] + bf16_bits_to_f32(q[1] >> 16))};
   }
 }
 
@@ -518,7 +511,7 @@ int device_cus() {
 template <int OUT, int MB>
 void launch_tiles(const A8Tiles& t, int grid, int nt, hipStream_t s) {
   k_a8_tiles<MB, OUT><<<grid, 64 * kA8Waves, 0, s>>>(t);
-  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? kA8Waves / 2 : kA8Waves) * MB, 64, 0, s>>>(t);
+  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? kA8Waves / 2 : kA8Waves) * MB * kA8Quarters, 64, 0, s>>>(t);
 }
 
 template <int OUT>
