@@ -22,8 +22,16 @@ int check_weights_public(const qw4_weights* w);
 namespace {
 
 // ---------------------------------------------------------------------------
-// k_a8_tiles: 256 columns (rows of W) x 32 MB rows of x a workgroup of 8 waves, two a
-// SIMD; a wave owns 32 columns against all the tile's rows, in MB blocks of 32 x 32.
+// k_a8_tiles: 128 columns (rows of W) x 32 MB rows of x a workgroup of 4 waves; a wave owns
+// 32 columns against all the tile's rows, in MB blocks of 32 x 32. Two workgroups fit a CU, so
+// that one's vector instructions run beside the other's MFMAs: 4096 rows of 34816 x 5120 take
+// 0.96 ms (1.52 POP/s; the clock falls to 1.5 GHz under its power), in a first form with one
+// workgroup of 8 waves and 256 columns a CU 1.04.
+//
+// In halves (KS = 2, tiles of up to 4 blocks) a workgroup has 8 waves, the second four take the
+// second half of the groups, and the sums meet in LDS: half as many slices for as many waves.
+// 77 rows of 5120 x 17408 26 us (29.6 in whole workgroups), 96 of 34816 x 5120 44 (50), 512 of
+// 5120 x 4096 25 (31). Other sizes lose: 256 of 5120 x 17408 50.5 against 49.
 //
 //  * Weights (the MFMA's A operand) come straight into registers, a lane the 32 bytes of
 //    its row and half of a group: every weight is unpacked once per workgroup, 7 vector
@@ -42,13 +50,14 @@ namespace {
 // 8 j + 4 (l / 32) + i.
 constexpr int kA8Waves = 4;
 constexpr int kTileCols = 32 * kA8Waves;
-constexpr int kPerCu = 2;   // workgroups
+constexpr int kPerCu = 2;   // workgroups; in halves, 1
+constexpr int kHalvesMb = 4;   // blocks of a tile in halves at most
 constexpr float kMagic = 12582912.f;
 
 template <int MB>
 struct A8Split {
   static constexpr int ACT = 4 * MB / kA8Waves;               // 1 KiB loads of codes a wave and group
-  static constexpr int DEPTH = MB <= 2 ? 4 : MB <= 4 ? 3 : 2;
+  static constexpr int DEPTH = MB <= 2 ? 4 : MB <= 4 ? 3 : 2;   // one or two more: 0 .. 9% slower
   static constexpr int LOADS = ACT + 1 + 7;        // codes, scales, weights (2 + 4 + 1)
   static constexpr int CODES = 32 * MB * 8;        // 16-byte units of a buffer's codes
   static constexpr int UNITS = CODES + kA8Waves * 16;   // and of its scales, 64 a wave's load
@@ -201,11 +210,12 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
   }
 }
 
-template <int MB>
+template <int MB, int KS>
 __device__ __forceinline__ void a8_segment(const A8Args& a, float (&acc)[MB][16], u32x4* lds, const A8Rows& x,
-                                           int tile, int b, int g0, int g1, int wave, int lane) {
+                                           int tile, int b, int g0, int g1, int half, int wave, int lane) {
   using Sp = A8Split<MB>;
   constexpr int D = Sp::DEPTH;
+  const int first = g0;
   const A8Src src{a.qw + (size_t)tile * a.G * kWordsPerBlock, a.sc + (size_t)tile * a.G * kMetaU16};
   // lane i of a load writes slot i % 8 of row i / 8: it fetches the chunk that belongs there
   const uint32_t voff = (uint32_t)(lane >> 3) * (uint32_t)a.K + (uint32_t)((lane & 7) ^ (lane >> 3) ^ (wave & 1)) * 16u;
@@ -214,6 +224,12 @@ __device__ __forceinline__ void a8_segment(const A8Args& a, float (&acc)[MB][16]
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mb][i] = 0.f;
   __syncthreads();   // the previous segment's last LDS reads are done
+  if (KS == 2) {     // a half of the waves takes a half of the groups
+    const int mid = (g0 + g1 + 1) / 2;
+    (half ? g0 : g1) = mid;
+    lds += half * D * Sp::UNITS;
+  }
+  const int end = KS == 2 && half ? 2 * g0 - first : g1;   // as many steps for both
   A8Weights w[D];
 #pragma unroll
   for (int d = 0; d < D - 1; ++d) {
@@ -223,14 +239,15 @@ __device__ __forceinline__ void a8_segment(const A8Args& a, float (&acc)[MB][16]
 #pragma unroll
     for (int p = 0; p < 2; ++p) a8_load_weights(w[d], src, b, g0 + d, in, lane, p);
   }
-  for (int gb = g0; gb < g1; gb += D) {
+  for (int gb = g0; gb < end; gb += D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int g = gb + d;
-      if (g >= g1) break;
+      if (g >= end) break;
       // group g has landed (the D - 2 behind it may be in flight) for every wave, and
       // every wave is done with group g - 1's buffer
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 2) * Sp::LOADS) : "memory");
+      if (KS == 2 && g >= g1) break;   // the other half's last
       constexpr int kBack = D - 1;
       a8_group<MB>(a, acc, w[d], w[(d + kBack) % D], lds + d * Sp::UNITS, lds + (d + kBack) % D * Sp::UNITS, x, src,
                    g + kBack < g1, voff, b, g + kBack, wave, lane);
@@ -279,20 +296,20 @@ __device__ __forceinline__ uint32_t a8_slot_off(int vp, int which, int wave, int
 __device__ __forceinline__ int a8_range_start(const A8Tiles& t, int vp) { return (int)((long long)vp * t.U / t.P); }
 __device__ __forceinline__ int a8_owner_of(const A8Tiles& t, int u) { return (int)(((long long)(u + 1) * t.P - 1) / t.U); }
 
-// Tile store: the sums pass through LDS, 32 rows x 256 columns of fp32 a block (16-byte
+// Tile store: the sums pass through LDS, 32 rows x 128 columns of fp32 a block (16-byte
 // chunk c of a row at c ^ (row % 16)), and come back as whole row segments, 8 output
 // columns a lane, where gate and up meet, bias and residual are added and the result is
 // rounded once.
-template <int MB, int OUT>
+template <int MB, int OUT, int KS>
 __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB][16], u32x4* lds, int m0, int tn,
-                                         int wave, int lane) {
+                                         int half, int wave, int lane) {
   constexpr bool GLU = OUT == A8_GLU;
-  constexpr int kFits = A8Split<MB>::DEPTH * A8Split<MB>::UNITS / (8 * kTileCols);
-  constexpr int kPass = kFits < MB ? kFits : MB;   // blocks of 32 KiB at a time
+  constexpr int kFits = KS * A8Split<MB>::DEPTH * A8Split<MB>::UNITS / (8 * kTileCols);
+  constexpr int kPass = kFits < MB ? kFits : MB;   // blocks of 16 KiB at a time
   static_assert(kPass >= 1, "a block fits the buffers");
-  constexpr int kCols = GLU ? kTileCols / 2 : kTileCols, kChunks = kTileCols / 4, kLanes = kCols / 8, kRows = 64 * kA8Waves / kLanes;
+  constexpr int kCols = GLU ? kTileCols / 2 : kTileCols, kChunks = kTileCols / 4, kLanes = kCols / 8, kRows = 64 * kA8Waves * KS / kLanes;
   const int r = lane & 31, h = lane >> 5;
-  const int t = wave * 64 + lane, cl = t % kLanes, rl = t / kLanes;
+  const int t = (KS == 2 ? half * kA8Waves + wave : wave) * 64 + lane, cl = t % kLanes, rl = t / kLanes;
   const int col = tn * kCols + 8 * cl;
   const bool in = col < a.ld;
   float bias[GLU ? 2 : 1][8];
@@ -303,7 +320,7 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kPass; ++k) {
-      if (p0 + k >= MB) break;
+      if (p0 + k >= MB || (KS == 2 && half)) break;
       const float(&v)[16] = acc[p0 + k < MB ? p0 + k : 0];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -340,12 +357,40 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
   }
 }
 
-template <int MB, int OUT>
-__global__ __launch_bounds__(64 * kA8Waves, 2) void k_a8_tiles(A8Tiles t) {
+// The second half's sums to the first's.
+template <int MB>
+__device__ __forceinline__ void a8_join(float (&acc)[MB][16], u32x4* lds, int half, int wave, int lane) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      u32x4& at = lds[((wave * MB + mb) * 4 + k) * 64 + lane];
+      if (half)
+        at = u32x4{__float_as_uint(acc[mb][4 * k]), __float_as_uint(acc[mb][4 * k + 1]),
+                   __float_as_uint(acc[mb][4 * k + 2]), __float_as_uint(acc[mb][4 * k + 3])};
+    }
+  __syncthreads();
+  if (half) return;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const u32x4 v = lds[((wave * MB + mb) * 4 + k) * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[mb][4 * k + i] += __uint_as_float(v[i]);
+    }
+}
+
+template <int MB, int OUT, int KS>
+__global__ __launch_bounds__(64 * kA8Waves * KS, 2) void k_a8_tiles(A8Tiles t) {
   using Sp = A8Split<MB>;
-  __shared__ u32x4 lds[Sp::DEPTH * Sp::UNITS];
+  __shared__ u32x4 lds[KS * Sp::DEPTH * Sp::UNITS];
+  static_assert(KS == 1 || 1024 * MB <= KS * Sp::DEPTH * Sp::UNITS, "the join's sums fit the buffers");
   const A8Args& a = t.a;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = KS == 2 ? waves % kA8Waves : waves, half = KS == 2 ? waves / kA8Waves : 0;
   float acc[MB][16];
   int vp = blockIdx.x;
   if (t.map) vp = (vp & 7) * (t.P >> 3) + (vp >> 3);   // each XCD a contiguous run (P % 8 == 0)
@@ -373,10 +418,11 @@ __global__ __launch_bounds__(64 * kA8Waves, 2) void k_a8_tiles(A8Tiles t) {
     const int m0 = tm * 32 * MB;
     const A8Wave w = a8_wave<OUT>(a, tn, wave);
     const A8Rows x{a.q + (size_t)m0 * a.K, a.scale + m0, (uint32_t)min(a.M - m0, 32 * MB)};
-    a8_segment<MB>(a, acc, lds, x, w.tile, w.b, g0, g1, wave, lane);
+    a8_segment<MB, KS>(a, acc, lds, x, w.tile, w.b, g0, g1, half, wave, lane);
+    if constexpr (KS == 2) a8_join<MB>(acc, lds, half, wave, lane);
     if (g0 == 0 && g1 == a.G) {
-      a8_store<MB, OUT>(a, acc, lds, m0, tn, wave, lane);
-    } else {   // the range's first tile to the first slot, its last to the second
+      a8_store<MB, OUT, KS>(a, acc, lds, m0, tn, half, wave, lane);
+    } else if (half == 0) {   // the range's first tile to the first slot, its last to the second
       const __amdgpu_buffer_rsrc_t rs = a8_rsrc(t.slots, 2u * t.P * kA8SlotBytes);
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
@@ -454,27 +500,31 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   }
 }
 
-// How a call is cut: tiles of 32 mb rows; schedule 0 whole tiles, 2 whole rounds and the
-// rest's units spread over all workgroups, 3 every tile in S slices; estimated us.
+// How a call is cut: ks 1 or, in halves, 2; tiles of 32 mb rows; schedule 0 whole tiles, 2
+// whole rounds and the rest's units spread over all workgroups, 3 every tile in S slices;
+// estimated us.
 struct A8Plan {
-  int mb, tiles_n, tiles_m, pick, S;
+  int ks, mb, tiles_n, tiles_m, pick, S;
   double cost;
 };
 
-// The best cut of tiles of mb rows. The estimate's figures are fitted to 3000 timed calls on
-// MI355X (7 projections from 5120x2176 to 34816x5120, 33 to 4096 rows, every mb, schedule and
-// S): the pick is 1.1% (geometric mean) from the fastest of all, 27% at worst (128 rows and
-// fewer of 5120x4096). A (tile, group) step takes 0.27 + 0.14 mb us with one workgroup on a
-// CU and 0.29 + 0.23 mb with two; storing a tile 0.66 mb; slices 4.6 for the second kernel,
-// their partial tiles' traffic and 0.45 for each piece of a sum. All units over all workgroups
-// (ranges that begin and end anywhere) was the fastest by 0.3% in the mean and is not kept.
-A8Plan a8_plan(int M, int cols, int G, int mb, int cus, bool ws_ok) {
-  A8Plan p{mb, (cols + kTileCols - 1) / kTileCols, (M + 32 * mb - 1) / (32 * mb), 0, 1, 0.};
-  const long long nt = (long long)p.tiles_n * p.tiles_m, most = kPerCu * cus, rem = nt % most;
-  const double one = 0.27 + 0.14 * mb, two = 0.29 + 0.23 * mb, store = 0.66 * mb;
-  auto whole = [&](long long tiles) {   // of the CU with most tiles, two at a time
+// The best cut of tiles of mb rows. The estimate's figures are fitted to 2100 timed calls on
+// MI355X (15 projections from 2048x2048 to 248320x5120, 24 to 4096 rows, every ks, mb,
+// schedule and S): over its 110 sizes the pick is 1.2% (geometric mean) from the fastest of
+// all, 11% at worst (64 rows and fewer of 2048x2048). A (tile, group) step takes `one` us with
+// one workgroup on a CU and `two` with two, or with one in halves; then come storing a tile, the
+// second kernel that joins slices, and their partial tiles' traffic. All units over all
+// workgroups (ranges that begin and end anywhere) was the fastest by 0.3% in the mean and is
+// not kept.
+A8Plan a8_plan(int M, int cols, int G, int ks, int mb, int cus, bool ws_ok) {
+  A8Plan p{ks, mb, (cols + kTileCols - 1) / kTileCols, (M + 32 * mb - 1) / (32 * mb), 0, 1, 0.};
+  const int at_once = ks == 2 ? 1 : kPerCu, half = (G + ks - 1) / ks;
+  const long long nt = (long long)p.tiles_n * p.tiles_m, most = at_once * cus, rem = nt % most;
+  const double one = 0.23 + 0.21 * mb, two = ks == 2 ? 0.57 + 0.27 * mb : 0.54 + 0.23 * mb;
+  const double store = (ks == 2 ? 0.08 : 0.86) * mb;
+  auto whole = [&](long long tiles) {   // of the CU with most tiles, as many at once as it holds
     const long long n = (tiles + cus - 1) / cus;
-    return (double)(n / 2) * (G * two + store) + (double)(n % 2) * (G * one + store);
+    return (double)(n / at_once) * (half * two + store) + (double)(n % at_once) * (half * one + store);
   };
   p.cost = whole(nt);
   if (!ws_ok || nt * G >= (1LL << 31)) return p;
@@ -485,12 +535,13 @@ A8Plan a8_plan(int M, int cols, int G, int mb, int cus, bool ws_ok) {
       p.cost = c;
     }
   };
-  if (nt > most && rem && rem * G >= most) take(2, 1, whole(nt - rem) + (double)rem * G / most * two + 7.0 + 3.3 * mb);
+  if (nt > most && rem && rem * G >= most)
+    take(2, 1, whole(nt - rem) + (double)rem * half / most * two + 3.1 + 4.45 * mb);
   for (int S = 2; S <= 64 && nt * S <= most && 2 * S <= G; ++S) {
     const long long P = nt * S;
     if (P % 8) continue;   // runs of workgroups on each XCD
-    const int steps = (G + S - 1) / S;
-    take(3, S, steps * (P <= cus ? one : two) + 4.6 + 1.63 * (double)P / most * mb + 0.45 * S);
+    const int steps = ((G + S - 1) / S + ks - 1) / ks;
+    take(3, S, steps * (P <= cus && ks == 1 ? one : two) + 3.9 + 4.71 * (double)P / (kPerCu * cus) * mb);
   }
   return p;
 }
@@ -509,9 +560,15 @@ int device_cus() {
 }
 
 template <int OUT, int MB>
-void launch_tiles(const A8Tiles& t, int grid, int nt, hipStream_t s) {
-  k_a8_tiles<MB, OUT><<<grid, 64 * kA8Waves, 0, s>>>(t);
-  if (t.full != nt) k_a8_fixup<MB, OUT><<<(nt - t.full) * (OUT == A8_GLU ? kA8Waves / 2 : kA8Waves) * MB * kA8Quarters, 64, 0, s>>>(t);
+void launch_tiles(const A8Tiles& t, int ks, int grid, int nt, hipStream_t s) {
+  if (ks == 1) {
+    k_a8_tiles<MB, OUT, 1><<<grid, 64 * kA8Waves, 0, s>>>(t);
+  } else if constexpr (MB <= kHalvesMb) {
+    k_a8_tiles<MB, OUT, 2><<<grid, 128 * kA8Waves, 0, s>>>(t);
+  }
+  if (t.full != nt)
+    k_a8_fixup<MB, OUT>
+        <<<(nt - t.full) * (OUT == A8_GLU ? kA8Waves / 2 : kA8Waves) * MB * kA8Quarters, 64, 0, s>>>(t);
 }
 
 template <int OUT>
@@ -523,11 +580,12 @@ int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
   const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
   const bool ws_ok = ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && cus % 8 == 0 &&
                      ws->bytes >= 2ull * kPerCu * cus * kA8SlotBytes;
-  A8Plan p = a8_plan(a.M, cols, a.G, 8, cus, ws_ok);
-  for (int mb = 6; mb >= 1; --mb) {
-    const A8Plan q = a8_plan(a.M, cols, a.G, mb, cus, ws_ok);
-    if (q.cost < p.cost) p = q;
-  }
+  A8Plan p = a8_plan(a.M, cols, a.G, 1, 8, cus, ws_ok);
+  for (int ks = 1; ks <= 2; ++ks)
+    for (int mb = ks == 2 ? kHalvesMb : 6; mb >= 1; --mb) {
+      const A8Plan q = a8_plan(a.M, cols, a.G, ks, mb, cus, ws_ok);
+      if (q.cost < p.cost) p = q;
+    }
   const long long tiles = (long long)p.tiles_n * p.tiles_m;
   if (tiles > 0x7fffffffLL / 64) return QW4_ERR_SHAPE;
   const int nt = (int)tiles;
@@ -535,19 +593,20 @@ int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
   int grid = nt;
   if (p.pick) {
     t.slots = static_cast<float*>(ws->buf);
-    t.P = grid = p.pick == 3 ? nt * p.S : kPerCu * cus;
-    t.full = p.pick == 2 ? nt - nt % (kPerCu * cus) : 0;
+    const int most = (p.ks == 2 ? 1 : kPerCu) * cus;
+    t.P = grid = p.pick == 3 ? nt * p.S : most;
+    t.full = p.pick == 2 ? nt - nt % most : 0;
     t.U = (nt - t.full) * a.G;
     t.map = p.pick == 3 ? 2 : 1;
   }
   switch (p.mb) {
-    case 1: launch_tiles<OUT, 1>(t, grid, nt, s); break;
-    case 2: launch_tiles<OUT, 2>(t, grid, nt, s); break;
-    case 3: launch_tiles<OUT, 3>(t, grid, nt, s); break;
-    case 4: launch_tiles<OUT, 4>(t, grid, nt, s); break;
-    case 5: launch_tiles<OUT, 5>(t, grid, nt, s); break;
-    case 6: launch_tiles<OUT, 6>(t, grid, nt, s); break;
-    default: launch_tiles<OUT, 8>(t, grid, nt, s);
+    case 1: launch_tiles<OUT, 1>(t, p.ks, grid, nt, s); break;
+    case 2: launch_tiles<OUT, 2>(t, p.ks, grid, nt, s); break;
+    case 3: launch_tiles<OUT, 3>(t, p.ks, grid, nt, s); break;
+    case 4: launch_tiles<OUT, 4>(t, p.ks, grid, nt, s); break;
+    case 5: launch_tiles<OUT, 5>(t, p.ks, grid, nt, s); break;
+    case 6: launch_tiles<OUT, 6>(t, p.ks, grid, nt, s); break;
+    default: launch_tiles<OUT, 8>(t, p.ks, grid, nt, s);
   }
   QW4_LAUNCH_CHECK();
   return QW4_OK;
