@@ -850,11 +850,14 @@ def logprobs(lp, logits, targets, T: int, n: int, ws: GemmWorkspace | None = Non
              stream=None) -> None:
     """qw4_logprobs / qw4_logprobs_f32 by the type of logits (bf16 or fp32; [T][n], contiguous
     or the columns of a wider 2-D tensor; a raw address is of contiguous bf16): lp [T][asked]
-    of targets [T][asked] int32 (asked: targets' elements over T unless given), entropy [T],
+    of targets int32 [T][asked] (or [T], one a row; an address comes with `asked`), entropy [T],
     the top_k best tokens' ids and log probabilities [T][top_k]."""
     dev, to = _place(stream)
     if asked is None:
-        asked = targets.numel() // T if targets is not None and T > 0 else 0
+        shape = (T, 0) if targets is None else getattr(targets, "shape", ())
+        if not 1 <= len(shape) <= 2:
+            raise ValueError("logprobs: targets of neither [T][asked] nor [T] need `asked`")
+        asked = shape[1] if len(shape) == 2 else 1
     f32 = _f32 is not None and getattr(logits, "dtype", None) is _f32
     x, row = _rows_of(logits, _f32 if f32 else _bf16, max(T, 0), n, 4 if f32 else 2, dev, "logprobs logits")
     rows = max(T, 0) * 4

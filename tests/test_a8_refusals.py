@@ -191,6 +191,11 @@ def test_binding_checks(hip):
         hip.logprobs(torch.zeros(4), torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64), 4, 100, stream=0)
     with pytest.raises(ValueError):
         hip.logprobs(torch.zeros(4), torch.zeros(4, 99), torch.zeros(4, dtype=torch.int32), 4, 100, stream=0)
+    for targets in (0x3000, torch.zeros(4, 1, 1, dtype=torch.int32), torch.zeros((), dtype=torch.int32)):
+        with pytest.raises(ValueError):   # how many a row?
+            hip.logprobs(torch.zeros(4), torch.zeros(4, 100), targets, 4, 100, stream=0)
+    with pytest.raises(ValueError):   # rows of two targets, values of one
+        hip.logprobs(torch.zeros(4), torch.zeros(4, 100), torch.zeros(8, 2, dtype=torch.int32), 4, 100, stream=0)
     with pytest.raises(hip.W4A16Error) as e:
         hip.logprobs(0x1000, 0x2000, 0x3000, 4, 100, top_k=40, top_ids=0x4000, top_logprobs=0x5000, asked=1, stream=0)
     assert e.value.status == hip.QW4_ERR_SHAPE
