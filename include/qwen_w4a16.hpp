@@ -187,4 +187,30 @@ void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_pla
                      const float* weights, int T, int top_k, int dim, const __hip_bfloat16* residual,
                      hipStream_t stream = 0);
 
+// Activations in 8 bits and the products that read them (no reference counterpart;
+// qwen_w4a16.h describes the rows).
+void a8_alloc(qw4_a8& a, int max_rows, int in_f);
+void a8_free(qw4_a8& a);
+void quantize_a8(const qw4_a8& a, const __hip_bfloat16* x, int ld, int T, hipStream_t stream = 0);
+void rmsnorm_a8(const qw4_a8& a, __hip_bfloat16* h_out, const __hip_bfloat16* h,
+                const __hip_bfloat16* residual, const __hip_bfloat16* w, int T, float eps,
+                hipStream_t stream = 0);
+void a8_dequant_rows(__hip_bfloat16* dst, const qw4_a8& a, int row0, int nrows,
+                     hipStream_t stream = 0);
+void linear_w4a8(__hip_bfloat16* y, const W4A16Weights& w, const qw4_a8& a, int T,
+                 const __hip_bfloat16* bias, int act, const __hip_bfloat16* residual,
+                 GemmWorkspace& ws, hipStream_t stream = 0);
+void linear_w4a8_f32(float* y, const W4A16Weights& w, const qw4_a8& a, int T, GemmWorkspace& ws,
+                     hipStream_t stream = 0);
+
+// Log probabilities, entropy and top alternatives of rows of logits (no reference
+// counterpart; argmax_rows is its nearest).
+void logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp,
+              const __hip_bfloat16* logits, size_t ld, const int32_t* targets, int T, int n,
+              int asked, int top_k, GemmWorkspace& ws, hipStream_t stream = 0);
+void logprobs_f32(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const float* logits,
+                  size_t ld, const int32_t* targets, int T, int n, int asked, int top_k,
+                  GemmWorkspace& ws, hipStream_t stream = 0);
+size_t logprobs_workspace(int T, int n, int top_k);
+
 }  // namespace qwen

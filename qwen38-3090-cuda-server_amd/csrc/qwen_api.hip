@@ -334,4 +334,52 @@ void combine_experts(__hip_bfloat16* out, const __hip_bfloat16* y, const qw4_pla
         "combine_experts");
 }
 
+void a8_alloc(qw4_a8& a, int max_rows, int in_f) { check(qw4_a8_alloc(&a, max_rows, in_f), "a8_alloc"); }
+
+void a8_free(qw4_a8& a) { check(qw4_a8_free(&a), "a8_free"); }
+
+void quantize_a8(const qw4_a8& a, const __hip_bfloat16* x, int ld, int T, hipStream_t stream) {
+  check(qw4_a8_quantize(&a, u16(x), ld, T, stream), "quantize_a8");
+}
+
+void rmsnorm_a8(const qw4_a8& a, __hip_bfloat16* h_out, const __hip_bfloat16* h, const __hip_bfloat16* residual,
+                const __hip_bfloat16* w, int T, float eps, hipStream_t stream) {
+  check(qw4_a8_rmsnorm(&a, u16(h_out), u16(h), u16(residual), u16(w), T, eps, stream), "rmsnorm_a8");
+}
+
+void a8_dequant_rows(__hip_bfloat16* dst, const qw4_a8& a, int row0, int nrows, hipStream_t stream) {
+  check(qw4_a8_dequant_rows(u16(dst), &a, row0, nrows, stream), "a8_dequant_rows");
+}
+
+void linear_w4a8(__hip_bfloat16* y, const W4A16Weights& w, const qw4_a8& a, int T, const __hip_bfloat16* bias,
+                 int act, const __hip_bfloat16* residual, GemmWorkspace& ws, hipStream_t stream) {
+  const qw4_weights v = view(w);
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_a8_linear(u16(y), &v, &a, T, u16(bias), act, u16(residual), &q, stream), "linear_w4a8");
+}
+
+void linear_w4a8_f32(float* y, const W4A16Weights& w, const qw4_a8& a, int T, GemmWorkspace& ws,
+                     hipStream_t stream) {
+  const qw4_weights v = view(w);
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_a8_linear_f32(y, &v, &a, T, &q, stream), "linear_w4a8_f32");
+}
+
+void logprobs(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const __hip_bfloat16* logits, size_t ld,
+              const int32_t* targets, int T, int n, int asked, int top_k, GemmWorkspace& ws, hipStream_t stream) {
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_logprobs(lp, entropy, top_ids, top_lp, u16(logits), ld, targets, T, n, asked, top_k, &q, stream),
+        "logprobs");
+}
+
+void logprobs_f32(float* lp, float* entropy, int32_t* top_ids, float* top_lp, const float* logits, size_t ld,
+                  const int32_t* targets, int T, int n, int asked, int top_k, GemmWorkspace& ws,
+                  hipStream_t stream) {
+  qw4_workspace q{ws.wbuf, ws.bytes};
+  check(qw4_logprobs_f32(lp, entropy, top_ids, top_lp, logits, ld, targets, T, n, asked, top_k, &q, stream),
+        "logprobs_f32");
+}
+
+size_t logprobs_workspace(int T, int n, int top_k) { return qw4_logprobs_workspace(T, n, top_k); }
+
 }  // namespace qwen
