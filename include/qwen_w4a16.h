@@ -485,7 +485,7 @@ int qw4_a8_rmsnorm(const qw4_a8* a, uint16_t* h_out, const uint16_t* h, const ui
 int qw4_a8_dequant_rows(uint16_t* dst, const qw4_a8* a, int row0, int nrows, void* stream);
 
 /* qw4_linear_epilogue over rows in 8 bits: y [T][width] = bf16(act(x @ W^T + bias) +
- * residual), x the first T >= 1 rows of a (a->in_f == w->in_f). Integer products, exact
+ * residual), x the first T >= 1 rows of a (a->in_f == w->in_f <= 2^23). Integer products, exact
  * within a group (weights are not rounded); fp32 from there to the one rounding. A
  * workspace (may be NULL; 256-byte aligned) of >= 2 x CUs x 256 KiB, as qw4_gemm's, lets
  * tiles be split along in_f when there are too few to fill the GPU; calls that share one

@@ -119,6 +119,8 @@ def test_linear_refusals(hip):
         assert f(y=0x10008) == hip.QW4_ERR_ALIGN
         assert f(a=_a8(hip, in_f=640)) == hip.QW4_ERR_SHAPE      # of another product
         assert f(w=_weights(hip, out_f=200)) == hip.QW4_ERR_SHAPE
+        wide = (1 << 23) + 128
+        assert f(w=_weights(hip, in_f=wide), a=_a8(hip, in_f=wide)) == hip.QW4_ERR_SHAPE
         for a, st in _bad_rows(hip):
             assert f(a=a) == st
     assert call(act=5) == hip.QW4_ERR_ACT
