@@ -277,7 +277,10 @@ struct LpWave {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
       more.sort(lane);
-      list.merge(more, lane);
+      if (last > -INFINITY || lane_value(list.v, 0) > -INFINITY)
+        list.merge(more, lane);
+      else
+        list = more;
       close(k);
       return;
     }
@@ -334,19 +337,31 @@ __device__ __forceinline__ float lp_logit(const T* p) {
     return bf16_bits_to_f32(*p);
 }
 
-// A row's results from its statistics and list, by one wave.
+// Target j of a row and its logit, where there is one.
+struct LpAsked {
+  bool in;
+  float x;
+};
 template <class T>
-__device__ __forceinline__ void lp_write(const LpArgs& a, int row, LpStats t, const LpList& list, int lane) {
+__device__ __forceinline__ LpAsked lp_asked(const LpArgs& a, int row, int j) {
+  if (j >= a.asked) return {false, 0.f};
+  const int i = a.targets[(size_t)row * a.asked + j];
+  const bool in = (unsigned)i < (unsigned)a.n;
+  return {in, in ? lp_logit(static_cast<const T*>(a.x) + (size_t)row * a.ld + i) : 0.f};
+}
+
+// A row's results from its statistics and list, by one wave; `first` is target `lane`.
+template <class T>
+__device__ __forceinline__ void lp_write(const LpArgs& a, int row, LpStats t, const LpList& list, LpAsked first,
+                                         int lane) {
   const bool some = t.m > -INFINITY;
   if (t.m == INFINITY) t.s = __builtin_nanf("");
   const float log = some ? log1pf(t.s) : t.s;   // of a row without any: 0, or NaN
   if (lane == 0 && a.entropy) a.entropy[row] = some ? log - t.u / (1.f + t.s) : log;
   auto lp = [&](float x) { return (some ? x - t.m : -INFINITY) - log; };
-  const T* xr = static_cast<const T*>(a.x) + (size_t)row * a.ld;
   for (int j = lane; j < a.asked; j += 64) {
-    const size_t at = (size_t)row * a.asked + j;
-    const int i = a.targets[at];
-    a.lp[at] = (unsigned)i < (unsigned)a.n ? lp(lp_logit(xr + i)) : 0.f;
+    const LpAsked at = j == lane ? first : lp_asked<T>(a, row, j);
+    a.lp[(size_t)row * a.asked + j] = at.in ? lp(at.x) : 0.f;
   }
   if (lane < a.k) {
     a.top_ids[(size_t)row * a.k + lane] = list.i;
@@ -512,7 +527,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
     t = w.stats(lane);
   }
   if (a.S == 1) {
-    lp_write<T>(a, row, t, w.list, lane);
+    lp_write<T>(a, row, t, w.list, lp_asked<T>(a, row, lane), lane);
     return;
   }
   uint32_t* rec = a.part + (size_t)blockIdx.x * (4 + 2 * a.k);
@@ -524,7 +539,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
 }
 
 // A row's splits joined: wave w takes the splits w, w + 16, ..., then pairs of waves.
-constexpr int kLpJoinWaves = 16;
+constexpr int kLpJoinWaves = 16, kLpMostSplits = 64;
 
 template <class T>
 __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
@@ -532,17 +547,31 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
   __shared__ LpStats parts[kLpJoinWaves];
   const int row = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int kPer = kLpMostSplits / kLpJoinWaves;
+  // all that the row needs is under way at once
+  LpAsked first{};
+  if (wave == 0) first = lp_asked<T>(a, row, lane);
+  LpStats part[kPer];
+  LpSlot slot[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int p = wave + kLpJoinWaves * j;
+    const uint32_t* rec = a.part + ((size_t)row * a.S + min(p, a.S - 1)) * (4 + 2 * a.k);
+    part[j] = *reinterpret_cast<const LpStats*>(rec);
+    slot[j] = {-INFINITY, -1};
+    if (lane < a.k) slot[j] = {__uint_as_float(rec[4 + lane]), (int)rec[4 + a.k + lane]};
+  }
   LpStats t{-INFINITY, 0.f, 0.f};
   LpList list;
-  for (int p = wave; p < a.S; p += kLpJoinWaves) {
-    const uint32_t* rec = a.part + ((size_t)row * a.S + p) * (4 + 2 * a.k);
-    t = lp_join(t, *reinterpret_cast<const LpStats*>(rec));
-    LpList more;
-    if (lane < a.k) {
-      more.v = __uint_as_float(rec[4 + lane]);
-      more.i = (int)rec[4 + a.k + lane];
-    }
-    if (a.k) list.merge(more, lane);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (wave + kLpJoinWaves * j >= a.S) break;
+    t = lp_join(t, part[j]);
+    if (a.k == 0) continue;
+    if (j)
+      list.merge({slot[j].v, slot[j].i}, lane);
+    else
+      list = {slot[j].v, slot[j].i};
   }
   for (int half = kLpJoinWaves / 2; half > 0; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
@@ -555,7 +584,7 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
       if (a.k) list.merge({slots[wave + half][lane].v, slots[wave + half][lane].i}, lane);
     }
   }
-  if (wave == 0) lp_write<T>(a, row, t, list, lane);
+  if (wave == 0) lp_write<T>(a, row, t, list, first, lane);
 }
 
 // Workgroups a row is split over: one from 640 rows on; else some 1024 workgroups, of at least
@@ -566,7 +595,7 @@ int lp_splits(int T, int n) {
   const long long most = blocks / (2 * kLpWaves);
   const long long want = T >= 640 ? 1 : (1024 + T - 1) / T;
   const long long s = want < most ? want : most;
-  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  return s < 1 ? 1 : s > kLpMostSplits ? kLpMostSplits : (int)s;
 }
 
 size_t lp_bytes(int T, int n, int k) {
