@@ -2,6 +2,7 @@
 the other, captured and replayed, on two streams, beside the rows of others."""
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -264,6 +265,40 @@ def test_two_streams(hip, model, T):
     for s, w in zip(kept, want):
         for one, two in zip(w, s.outputs()):
             assert torch.equal(one, two)
+        s.free()
+
+
+def test_two_threads(hip, model):
+    """Host threads that launch at once, on their own streams and buffers, other row counts."""
+    sizes = (9, 40, 24, 1)
+    kept = [Buffers(hip, T) for T in sizes]
+    inputs = [rows(T, 300 + T) for T in sizes]
+    want = []
+    for T, s, (x, t) in zip(sizes, kept, inputs):
+        s.targets[:] = t
+        run(hip, model, s, x, T)
+        want.append(s.outputs())
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(T, s, x, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    run(hip, model, s, x, T)
+                torch.cuda.current_stream().synchronize()
+                for one, two in zip(w, s.outputs()):
+                    assert torch.equal(one, two)
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(T, s, x, w)) for T, s, (x, _), w in zip(sizes, kept, inputs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for s in kept:
         s.free()
 
 
