@@ -30,9 +30,11 @@ __device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
   return ((nib | 0x80808080u) - z) ^ 0x80808080u;
 }
 
-// The kernel for few rows (a8_few.hip): launches it and returns true, or returns false
+// The kernel for few rows (a8_few.h): launches it and returns true, or returns false
 // where it does not apply.
 bool a8_few(int out, const A8Args& a, int cus, hipStream_t st);
+bool a8_few_epi(const A8Args& a, int P, int U, bool small, hipStream_t st);
+bool a8_few_f32(const A8Args& a, int P, int U, bool small, hipStream_t st);
 
 // The arrays of `a` are there, and it holds rows [row0, row0 + T).
 inline int check_a8(const qw4_a8* a, int row0, int T) {
