@@ -30,6 +30,13 @@ __device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
   return ((nib | 0x80808080u) - z) ^ 0x80808080u;
 }
 
+// A group's integer sum starts as the bits of M = 1.5 2^23, so that, read as a float, it is M +
+// sum: t = fma(f, sx, -M sx) is the scaled sum, rounded once, for M sx is exact for an sx of 22
+// bits, to which it is cut.
+constexpr float kA8Magic = 12582912.f;
+constexpr int kA8Start = 0x4B400000;
+__device__ __forceinline__ float a8_scale(float sx) { return __uint_as_float(__float_as_uint(sx) & ~3u); }
+
 // The kernel for few rows (a8_few.h): launches it and returns true, or returns false
 // where it does not apply.
 bool a8_few(int out, const A8Args& a, int cus, hipStream_t st);

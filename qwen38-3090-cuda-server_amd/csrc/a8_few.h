@@ -33,6 +33,12 @@ namespace {
 // Buffers of the waves' sums of a part.
 template <int MB, int S>
 constexpr int few_buffers(int W) { return MB * S * W <= 16 ? 2 : 1; }
+// 16-byte units that they take for a wave, and its codes of 16 rows and a group.
+template <int MB, int S, int JJ>
+constexpr int few_red(int W) {
+  const int sums = few_buffers<MB, S>(W) * MB * S * 16 * JJ;
+  return JJ > 1 && sums < 128 ? 128 : sums;
+}
 
 // Row m, columns n0 + i: the sums (gate, up) of a unit.
 template <int OUT, int S>
@@ -78,8 +84,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
   constexpr int kL = PT * L::kLoads, kLX = kL + 2 * MB, kSlot = PT * L::kUnits, kBuf = few_buffers<MB, S>(W);
   constexpr int kPer = 4 / S;
   const A8Args& a = f.a;
-  __shared__ fJ red[W][kBuf * MB * S * 64];
-  __shared__ u32x4 area[JJ == 1 ? 1 : W][MB * 128];   // a group's codes on their way into MFMA rows
+  // A wave's sums of a part; before it has any, its codes of a group on their way into MFMA rows.
+  constexpr int kRed = few_red<MB, S, JJ>(W);
+  __shared__ u32x4 room[W][kRed];
   extern __shared__ u32x4 few_lds[];   // the waves' slots; scales and code sums [G][2][16 MB]
   float* const sxl = reinterpret_cast<float*>(few_lds + W * D * kSlot);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -98,7 +105,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
   // Scales: of MFMA row m of block b, at 16 b + m.
   for (int i = threadIdx.x; i < a.G * 16 * MB; i += 64 * W) {
     const int g = i / (16 * MB), m = i - g * (16 * MB), row = (m & ~15) + 4 * (m & 3) + ((m & 15) >> 2);
-    sxl[(2 * g) * 16 * MB + m] = row < a.M ? a.scale[(size_t)g * a.max_rows + row] : 0.f;
+    sxl[(2 * g) * 16 * MB + m] = row < a.M ? a8_scale(a.scale[(size_t)g * a.max_rows + row]) : 0.f;
   }
 
   u32x4 x[NG][MB][2];
@@ -146,6 +153,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
   }
   lds_barrier<true>();   // the scales are there
 
+  const i32x4 start = {kA8Start, kA8Start, kA8Start, kA8Start};
   fJ acc[PT][MB][S];
 #pragma unroll
   for (int t = 0; t < PT; ++t)
@@ -175,25 +183,24 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
       for (int t = 0; t < PT; ++t) dma_read<4, S, true>(d[t], ring + j * kSlot + t * L::kUnits, lane, st0);
       if constexpr (kFirst && !kDirect) {   // through LDS: chunk k of row m at k ^ g(m), as in the tiles
         auto at = [](int m, int k) { return m * 8 + (k ^ (m & 7) ^ ((m >> 3) & 1)); };
-        u32x4* const own = area[JJ == 1 ? 0 : wave];
+        u32x4* const own = room[wave];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) own[mb * 128 + at(8 * h + (lane >> 3), lane & 7)] = x[gi][mb][h];
-        }
-        __builtin_amdgcn_wave_barrier();
+          for (int h = 0; h < 2; ++h) own[at(8 * h + (lane >> 3), lane & 7)] = x[gi][mb][h];
+          __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) x[gi][mb][h] = own[mb * 128 + at(4 * (c & 3) + (c >> 2), 2 * q + h)];
+          for (int h = 0; h < 2; ++h) x[gi][mb][h] = own[at(4 * (c & 3) + (c >> 2), 2 * q + h)];
+          __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_wave_barrier();
       }
       float* const sg = sxl + 2 * (wave + W * gi) * 16 * MB + 4 * q;
-      fJ sx[MB], xs[MB];   // scales and minus the sums of the rows' codes
+      fJ sx[MB], xs[MB], less[MB];   // scales, minus the sums of the rows' codes, -M sx
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         sx[mb] = *reinterpret_cast<const fJ*>(sg + 16 * mb);
+#pragma unroll
+        for (int k = 0; k < JJ; ++k) less[mb][k] = -kA8Magic * sx[mb][k];
         if constexpr (kFirst) {   // the same in all columns
           const i32x4 minus = {-1, -1, -1, -1};
           i32x4 C = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x[gi][mb][0]), minus, i32x4{0, 0, 0, 0}, 0, 0, 0);
@@ -220,13 +227,14 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) {
             i32x4 C = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x[gi][mb][0]),
-                                                            __builtin_bit_cast(i32x4, lo), i32x4{0, 0, 0, 0}, 0, 0, 0);
+                                                            __builtin_bit_cast(i32x4, lo), start, 0, 0, 0);
             C = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x[gi][mb][1]),
                                                       __builtin_bit_cast(i32x4, hi), C, 0, 0, 0);
 #pragma unroll
             for (int k = 0; k < JJ; ++k) {
               const int v = __mul24(z, __float_as_int(xs[mb][k])) + C[k];
-              acc[t][mb][i][k] = __builtin_fmaf((float)v * sw, sx[mb][k], acc[t][mb][i][k]);
+              const float p = __builtin_fmaf(__int_as_float(v), sx[mb][k], less[mb][k]);
+              acc[t][mb][i][k] = __builtin_fmaf(p, sw, acc[t][mb][i][k]);
             }
           }
         }
@@ -252,7 +260,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-          red[wave][((par * MB + mb) * S + i) * 64 + lane] = acc[t][mb][i];
+          reinterpret_cast<fJ*>(room[wave])[((par * MB + mb) * S + i) * 64 + lane] = acc[t][mb][i];
           acc[t][mb][i] = fJ{};
         }
       lds_barrier<true>();
@@ -263,9 +271,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
 #pragma unroll
           for (int i = 0; i < S; ++i) {
             const int at = (((par * MB + mb) * S + i) * 64 + lane) * JJ + jj;
-            float r = reinterpret_cast<const float*>(red[0])[at];
+            float r = reinterpret_cast<const float*>(room[0])[at];
 #pragma unroll
-            for (int w = 1; w < W; ++w) r += reinterpret_cast<const float*>(red[w])[at];
+            for (int w = 1; w < W; ++w) r += reinterpret_cast<const float*>(room[w])[at];
             v[k][t][i] = r;
           }
         }
@@ -288,7 +296,7 @@ template <int OUT, int S, int NG, int W, int D, int MB, int JJ>
 bool launch(const FewArgs& f, hipStream_t st) {
   constexpr auto kern = &k_a8_few<OUT, S, NG, W, D, MB, JJ>;
   constexpr int slots = (OUT == A8_GLU ? 2 : 1) * W * D * DmaSlot<4, S>::kUnits * 16;
-  constexpr int fixed = W * few_buffers<MB, S>(W) * MB * S * 256 * JJ + (JJ == 1 ? 1 : W) * MB * 2048;
+  constexpr int fixed = W * few_red<MB, S, JJ>(W) * 16;
   static_assert(slots + W * NG * 128 * MB + fixed <= kLdsBytes, "LDS of a CU");
   allow_lds<kern>(slots + W * NG * 128 * MB);
   kern<<<f.P, 64 * W, slots + f.a.G * 128 * MB, st>>>(f);

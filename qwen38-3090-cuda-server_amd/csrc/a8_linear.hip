@@ -40,10 +40,9 @@ namespace {
 //    instruction), D groups buffered. Row m holds 16-byte chunk c at c ^ g(m), g = (m % 8) ^
 //    (m / 8 % 2): the 8 rows that 128 bytes of banks serve, and the 16 of 256 bytes, differ.
 //    The scales of the tile's rows lie behind them.
-//  * A block's four MFMAs start from M = 1.5 2^23 as bits, so that the sums, read as
-//    floats, are M + sum: t = fma(f, sx, -M sx) is the scaled sum, rounded once (M sx is
-//    exact for an sx of 22 bits, to which it is cut), and acc = fma(t, sw, acc): two
-//    instructions a sum and group where a conversion, two products and an addition were four.
+//  * A block's four MFMAs start from M (a8_scale): its 16 sums a lane are scaled into the
+//    accumulators by two instructions each where a conversion, two products and an addition
+//    were four.
 //
 // MFMA layout: lane l holds weight row l % 32, inputs of chunks 2 s + l / 32 (s = 0, 1), low
 // nibbles and high nibbles an operand each; of the result column l % 32 (a row of x), rows
@@ -52,7 +51,6 @@ constexpr int kA8Waves = 4;
 constexpr int kTileCols = 32 * kA8Waves;
 constexpr int kPerCu = 2;   // workgroups; in halves, 1
 constexpr int kHalvesMb = 4;   // blocks of a tile in halves at most
-constexpr float kMagic = 12582912.f;
 constexpr int kA8MostK = 1 << 23;   // 256 rows of codes are offsets of 31 bits
 
 template <int MB>
@@ -181,12 +179,12 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
   for (int j = 0; j < 4; ++j) sw[j] = bf16_bits_to_f32(w.s[j]);
   i32x16 start;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) start[i] = 0x4B400000;
+  for (int i = 0; i < 16; ++i) start[i] = kA8Start;
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     i32x16 c = start;
-    const float fx = __uint_as_float(__float_as_uint(sx) & ~3u), less = -kMagic * fx;
+    const float fx = a8_scale(sx), less = -kA8Magic * fx;
 #pragma unroll
     for (int o = 0; o < 4; ++o) {
       c = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[o], __builtin_bit_cast(i32x4, v[o]), c, 0, 0, 0);
