@@ -211,3 +211,28 @@ def test_small_workspaces(hip):
         torch.cuda.synchronize()
         assert torch.equal(y, z) and torch.all(buf[size:] == 7)
     hip.awq_free(w)
+
+
+@pytest.mark.parametrize("T", [33, 34, 47, 48, 49, 50, 63, 64])
+@pytest.mark.parametrize("n,k", [(128, 128), (384, 1024), (4224, 640), (256, 2944), (128, 3200), (1280, 4992), (128, 5120),
+                                 (17408, 640), (256, 5248)])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_three_and_four_blocks_of_rows(hip, T, n, k, act):
+    w, less, s = random_weights(hip, n, k, T)
+    q, scale = random_rows(T + 2, k, n)
+    codes = to_layout(q)
+    a = hip.a8_over(codes, scale)   # of two rows more than the call's
+    up = n // 2 if act == "swiglu" else 0
+    y = torch.full((T + 1, n - up), 9.0, **BF16)
+    f = torch.full((T + 1, n), 9.0, device="cuda")
+    hip.linear_w4a8(y, w, a, T, None, act=getattr(hip, "ACT_" + act.upper()))
+    hip.linear_w4a8_f32(f, w, a, T, None)
+    torch.cuda.synchronize()
+    v, size = product(q[:T], scale[:, :T], less, s)
+    tol = sum_tolerance(size, k // 128)
+    assert torch.all((f[:T].double() - v).abs() <= tol)
+    want, moved = _act(v, act, up)
+    tol = moved(tol)
+    assert torch.all((y[:T].double() - want).abs() <= tol + (2.0 ** -8 + 2.0 ** -23) * want.abs() + 2.0 ** -23 * tol)
+    assert torch.all(y[T:] == 9.0) and torch.all(f[T:] == 9.0)
+    hip.awq_free(w)
