@@ -16,7 +16,7 @@
 // logit from below, and one wave reads the eights whose key reaches it again, some k of them.
 // Where a lane's sixth key reaches it, there may have been a seventh: then the waves go over
 // their blocks once more and keep lists (sorted or constant rows). 1000 x 248320 bf16 logits
-// take 103 us at k = 5, 20 and 32, and 92 without alternatives; with lists kept from the start
+// take 102 us at k = 5, 20 and 32, and 92 without alternatives; with lists kept from the start
 // they took 138 / 207 / 245; with four keys one row of some 500 went over its blocks again at
 // k = 32, and its workgroup alone lengthened the launch to 212 us (five: 149).
 //
@@ -388,28 +388,29 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
   const int blocks = (vecs + 64 * kParts - 1) / (64 * kParts);
   const int b0 = split * kLpWaves + wave, step = kLpWaves * a.S;
   LpWave<TOP> w;
-  // the eight that lane `of` has in block b: its 16-byte parts (past the row's, some other),
-  // its logits, and their indices
+  // the eight that lane `of` has in block b: its 16-byte parts (past the row's, its last) --
+  // there is one --, -Inf for those past the row's in its last block, its logits, their indices
   auto load = [&](u32x4 (&v)[kParts], int b, int of) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      const long long i = ((long long)b * kParts + p) * 64 + of;
-      v[p] = xv[i < vecs ? i : 0];
-    }
+    for (int p = 0; p < kParts; ++p) v[p] = xv[min((b * kParts + p) * 64 + of, vecs - 1)];
   };
-  auto values = [&](float (&x)[8], const u32x4 (&v)[kParts], int b, int of) __attribute__((always_inline)) {
+  auto end = [&](u32x4 (&v)[kParts], int b, int of) __attribute__((always_inline)) {
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      const bool in = ((long long)b * kParts + p) * 64 + of < vecs;
+    for (int p = 0; p < kParts; ++p)
+      if ((b * kParts + p) * 64 + of >= vecs) v[p] = u32x4{kNone, kNone, kNone, kNone};
+  };
+  auto values = [&](float (&x)[8], const u32x4 (&v)[kParts]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         if constexpr (sizeof(T) == 4) {
-          x[p * 4 + c] = in ? __uint_as_float(v[p][c]) : -INFINITY;
+          x[p * 4 + c] = __uint_as_float(v[p][c]);
         } else {
-          x[2 * c] = in ? bf16_bits_to_f32(v[p][c] & 0xffffu) : -INFINITY;
-          x[2 * c + 1] = in ? bf16_bits_to_f32(v[p][c] >> 16) : -INFINITY;
+          x[2 * c] = bf16_bits_to_f32(v[p][c] & 0xffffu);
+          x[2 * c + 1] = bf16_bits_to_f32(v[p][c] >> 16);
         }
-    }
   };
   auto index = [&](int b, int of, int e) { return head + ((b * kParts + e / kVec) * 64 + of) * kVec + e % kVec; };
   // use(x, block, number) for the wave's blocks, kLpAhead of them read at a time
@@ -422,7 +423,8 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
       for (int d = 0; d < kLpAhead; ++d) {
         if (b + d * step >= blocks) break;
         float x[8];
-        values(x, v[d], b + d * step, lane);
+        if (b + d * step == blocks - 1) end(v[d], b + d * step, lane);
+        values(x, v[d]);
         use(x, b + d * step, (uint32_t)(number + d));
       }
     }
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
             count += __popcll(some);
           }
         }
-      if (fits && count <= 64) {
+      if (fits && count > 0 && count <= 64) {
         __builtin_amdgcn_wave_barrier();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         const bool has = lane < count;
@@ -478,13 +480,12 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
         u32x4 v[kParts];
         float x[8];
         load(v, b, of);
-        values(x, v, b, of);
+        end(v, b, of);
+        values(x, v);
         const float least = lp_least(t >> 16);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = has && x[e] >= least ? x[e] : -INFINITY;
         w.choose(x, [&](int e) { return index(b, of, e); }, a.k, lane, least, slots[0]);
-      } else {
-        fits = false;
       }
       if (lane == 0) again = !fits || count > 64;
     }
