@@ -540,7 +540,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LpArgs a) {
 }
 
 // A row's splits joined: wave w takes the splits w, w + 16, ..., then pairs of waves.
-constexpr int kLpJoinWaves = 16, kLpMostSplits = 64;
+constexpr int kLpJoinWaves = 16, kLpMostSplits = 32;
 
 template <class T>
 __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
@@ -589,8 +589,10 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void k_logprobs_join(LpArgs a) {
 }
 
 // Workgroups a row is split over: one from 640 rows on; else some 1024 workgroups, of at least
-// two blocks a wave. 256 / 400 rows of 248320 bf16 logits: 40 / 54 us, with some 512 workgroups
-// 46 / 68, with 2048 42 / 54; 64 rows 22, 22 and 25; 1000 rows 103 whole, 112 in two.
+// two blocks a wave, at most 32 a row. 256 / 400 rows of 248320 bf16 logits: 39 / 54 us, with
+// some 512 workgroups 46 / 68, with 2048 42 / 54; 64 rows 21, 22 and 25; 1000 rows 103 whole, 112
+// in two. One / 16 fp32 rows with 20 alternatives in 32 parts 13.3 / 15.8, in 16 13.9 / 15.3, in
+// 64 14.0 / 17.2.
 int lp_splits(int T, int n) {
   const long long blocks = ((long long)n + kLpBlock - 1) / kLpBlock;
   const long long most = blocks / (2 * kLpWaves);
