@@ -453,7 +453,8 @@ int qw4_combine(uint16_t* out, const uint16_t* y, const qw4_plan* plan, const fl
  * Rows of activations as int8 codes with a scale for each group of 128 inputs, and the
  * products that read them (no reference counterpart: its activations stay bf16). A
  * value is q scale, scale = (largest |value| of the group) / 127, q = its nearest
- * integer in [-127, 127].
+ * integer in [-127, 127], of two as near the even one (of qw4_a8_rmsnorm's fp32 values up
+ * to 2^-23 of the quotient).
  *   q      [max_rows][in_f]; input 8 w + e of a chunk of 32 (w, e = 0..3, 0..7) lies at
  *          byte 4 w + {0, 2, -, -, 1, 3, -, -}[e] or 16 + 4 w + {-, -, 0, 2, -, -, 1, 3}[e]
  *          of the chunk: the order in which the nibbles of a packed weight word meet it

@@ -2,7 +2,11 @@
 //
 // A group of 128 inputs is 16 lanes of 8. A = max |v| over the group (a maximum of the
 // bits, in which NaN is the largest), scale = A / 127, q = RNE(v 127 / A): the product
-// and the rounding are one fma against 1.5 2^23, whose lowest byte is then q.
+// and the rounding are one fma against 1.5 2^23, whose lowest byte is then q. 127 / A is
+// rounded up: v = A / 2, which bf16 rows meet constantly, is 63.5 or as little above it as
+// fp32 tells, and becomes 64, the even one. Of bf16 values no other quotient is so close to
+// the middle of two codes that the rounding of 127 / A moves it across (all pairs of
+// mantissas are tested); of a norm's fp32 values one within 2^-23 of itself may go either way.
 // The codes of a word's 8 inputs are the bytes {0, 4, 1, 5} and {2, 6, 3, 7}, as the low
 // and the high nibbles of a packed weight word hold them: a product reads its operand
 // 16 bytes at a time with no shuffle.
@@ -50,7 +54,8 @@ __device__ __forceinline__ u32x2 a8_codes(const float (&v)[8], int lane, float& 
   const float a = __uint_as_float(top);
   const bool some = a >= kA8Least && top < 0x7f800000u;
   scale = some ? a / 127.f : top >= 0x7f800000u ? __builtin_nanf("") : 0.f;
-  const float r = some ? 127.f / a : 0.f;
+  float r = some ? 127.f / a : 0.f;
+  if (__builtin_fmaf(-r, a, 127.f) > 0.f && some) r = __uint_as_float(__float_as_uint(r) + 1);   // the fma is exact
   uint32_t b[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(__builtin_fmaf(v[e], r, 12582912.f));
