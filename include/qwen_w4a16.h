@@ -490,9 +490,8 @@ int qw4_a8_dequant_rows(uint16_t* dst, const qw4_a8* a, int row0, int nrows, voi
  * within a group (weights are not rounded); fp32 from there to the one rounding. A
  * workspace (may be NULL; 256-byte aligned) of >= 2 x CUs x 256 KiB, as qw4_gemm's, lets
  * tiles be split along in_f when there are too few to fill the GPU; calls that share one
- * must be stream-ordered. Scales of a count to 22 bits, and a group whose largest value
- * is 2^110 or more may make its row's products Inf or NaN. y, bias and residual 16-byte
- * aligned; residual may be y. */
+ * must be stream-ordered. Weight scales of 2^104 or more may make their outputs Inf or
+ * NaN. y, bias and residual 16-byte aligned; residual may be y. */
 int qw4_a8_linear(uint16_t* y, const qw4_weights* w, const qw4_a8* a, int T, const uint16_t* bias,
                   int act, const uint16_t* residual, qw4_workspace* ws, void* stream);
 /* The same without an epilogue, y [T][out_f] in fp32: logits. */

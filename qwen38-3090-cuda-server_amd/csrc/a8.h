@@ -31,11 +31,11 @@ __device__ __forceinline__ uint32_t a8_less(uint32_t nib, uint32_t z) {
 }
 
 // A group's integer sum starts as the bits of M = 1.5 2^23, so that, read as a float, it is M +
-// sum: t = fma(f, sx, -M sx) is the scaled sum, rounded once, for M sx is exact for an sx of 22
-// bits, to which it is cut.
+// sum: t = fma(f, sw, -M sw) is the sum scaled by the weight's scale, rounded once, for M sw is
+// exact for the 8 bits of a bf16 sw (below 2^104, from where it is Inf). The row's scale, of 24
+// bits, comes second.
 constexpr float kA8Magic = 12582912.f;
 constexpr int kA8Start = 0x4B400000;
-__device__ __forceinline__ float a8_scale(float sx) { return __uint_as_float(__float_as_uint(sx) & ~3u); }
 
 // The kernel for few rows (a8_few.h): launches it and returns true, or returns false
 // where it does not apply.

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
   // Scales: of MFMA row m of block b, at 16 b + m.
   for (int i = threadIdx.x; i < a.G * 16 * MB; i += 64 * W) {
     const int g = i / (16 * MB), m = i - g * (16 * MB), row = (m & ~15) + 4 * (m & 3) + ((m & 15) >> 2);
-    sxl[(2 * g) * 16 * MB + m] = row < a.M ? a8_scale(a.scale[(size_t)g * a.max_rows + row]) : 0.f;
+    sxl[(2 * g) * 16 * MB + m] = row < a.M ? a.scale[(size_t)g * a.max_rows + row] : 0.f;
   }
 
   u32x4 x[NG][MB][2];
@@ -195,12 +195,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
         }
       }
       float* const sg = sxl + 2 * (wave + W * gi) * 16 * MB + 4 * q;
-      fJ sx[MB], xs[MB], less[MB];   // scales, minus the sums of the rows' codes, -M sx
+      fJ sx[MB], xs[MB];   // scales, minus the sums of the rows' codes
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         sx[mb] = *reinterpret_cast<const fJ*>(sg + 16 * mb);
-#pragma unroll
-        for (int k = 0; k < JJ; ++k) less[mb][k] = -kA8Magic * sx[mb][k];
         if constexpr (kFirst) {   // the same in all columns
           const i32x4 minus = {-1, -1, -1, -1};
           i32x4 C = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x[gi][mb][0]), minus, i32x4{0, 0, 0, 0}, 0, 0, 0);
@@ -218,6 +216,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
         for (int i = 0; i < S; ++i) {
           const int z = (int)((d[t].z >> (zsh + 4 * i)) & 0xFu);
           const float sw = bf16_bits_to_f32((d[t].s[i >> 1] >> (16 * (S == 1 ? (st0 & 1) : (i & 1)))) & 0xffffu);
+          const float less = -kA8Magic * sw;
           u32x4 lo, hi;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -233,8 +232,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_a8_few(FewArgs f) {
 #pragma unroll
             for (int k = 0; k < JJ; ++k) {
               const int v = __mul24(z, __float_as_int(xs[mb][k])) + C[k];
-              const float p = __builtin_fmaf(__int_as_float(v), sx[mb][k], less[mb][k]);
-              acc[t][mb][i][k] = __builtin_fmaf(p, sw, acc[t][mb][i][k]);
+              const float p = __builtin_fmaf(__int_as_float(v), sw, less);
+              acc[t][mb][i][k] = __builtin_fmaf(p, sx[mb][k], acc[t][mb][i][k]);
             }
           }
         }

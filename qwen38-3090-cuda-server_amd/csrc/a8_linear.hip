@@ -33,20 +33,20 @@ namespace {
 // 77 rows of 5120 x 17408 26 us (29.6 in whole workgroups), 96 of 34816 x 5120 44 (50), 512 of
 // 5120 x 4096 25 (31). Other sizes lose: 256 of 5120 x 17408 50.5 against 49.
 //
-//  * Weights (the MFMA's A operand) come straight into registers, a lane the 32 bytes of
+//  * Weights (the MFMA's B operand) come straight into registers, a lane the 32 bytes of
 //    its row and half of a group: every weight is unpacked once per workgroup, 7 vector
 //    instructions for 8.
-//  * Codes (B) go global -> LDS (buffer_load ... lds, whole 128-byte row segments, 1 KiB an
+//  * Codes (A) go global -> LDS (buffer_load ... lds, whole 128-byte row segments, 1 KiB an
 //    instruction), D groups buffered. Row m holds 16-byte chunk c at c ^ g(m), g = (m % 8) ^
 //    (m / 8 % 2): the 8 rows that 128 bytes of banks serve, and the 16 of 256 bytes, differ.
 //    The scales of the tile's rows lie behind them.
-//  * A block's four MFMAs start from M (a8_scale): its 16 sums a lane are scaled into the
+//  * A block's four MFMAs start from M (kA8Magic): its 16 sums a lane are scaled into the
 //    accumulators by two instructions each where a conversion, two products and an addition
-//    were four.
+//    were four: by the lane's weight scale, then by the rows' scales, taken across lanes.
 //
 // MFMA layout: lane l holds weight row l % 32, inputs of chunks 2 s + l / 32 (s = 0, 1), low
-// nibbles and high nibbles an operand each; of the result column l % 32 (a row of x), rows
-// 8 j + 4 (l / 32) + i.
+// nibbles and high nibbles an operand each; of the result column l % 32 (a weight row), rows
+// (of x) 8 j + 4 (l / 32) + i.
 constexpr int kA8Waves = 4;
 constexpr int kTileCols = 32 * kA8Waves;
 constexpr int kPerCu = 2;   // workgroups; in halves, 1
@@ -57,7 +57,7 @@ template <int MB>
 struct A8Split {
   static constexpr int ACT = 4 * MB / kA8Waves;               // 1 KiB loads of codes a wave and group
   static constexpr int DEPTH = MB <= 2 ? 4 : MB <= 4 ? 3 : 2;   // one or two more: 0 .. 9% slower
-  static constexpr int LOADS = ACT + 1 + 7;        // codes, scales, weights (2 + 4 + 1)
+  static constexpr int LOADS = ACT + 1 + 4;        // codes, scales, weights (2 + 1 + 1)
   static constexpr int CODES = 32 * MB * 8;        // 16-byte units of a buffer's codes
   static constexpr int UNITS = CODES + kA8Waves * 16;   // and of its scales, 64 a wave's load
   static_assert(4 * MB % kA8Waves == 0 && 32 * MB <= 64 * kA8Waves, "whole loads a wave");
@@ -72,7 +72,7 @@ struct A8Tiles {
 
 struct A8Weights {
   u32x4 q[2];                // chunks h, 2 + h of the lane's row
-  uint32_t s[4];             // scale of row 8 j + 4 h + lane % 4
+  uint32_t s;                // its scale
   uint32_t z;                // zero points of rows r & ~3 .. + 3
 };
 struct A8Src {               // of a wave's weight tile: blocks and (scale, zero-point) records
@@ -84,7 +84,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t a8_rsrc(const void* p, uint32_
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
 }
 
-// Part 0: the words and zero points of group g, part 1: the scales. A group of which there
+// Part 0: the words and zero points of group g, part 1: the scale. A group of which there
 // is not `some` is out of its resource's range: no memory, no branch. Tiles of 8 blocks have
 // one resource for all groups and an offset, others one a group: 4096 rows of 34816 x 5120
 // take 0.883 and 0.930 ms in these forms, 1001 of 5120 x 4096 (of fewer blocks) 40.8 and 39.2 us.
@@ -105,9 +105,7 @@ __device__ __forceinline__ void a8_load_weights(A8Weights& w, const A8Src& src, 
       w.q[s] = __builtin_amdgcn_raw_buffer_load_b128(qw, ((2 * s + h) * 64 + pos) * 16, at * 4096, 0);
     w.z = __builtin_amdgcn_raw_buffer_load_b16(rec, 128 + (8 * b + (r >> 2)) * 2, at * kMetaBytes, 0);
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w.s[j] = __builtin_amdgcn_raw_buffer_load_b16(rec, (32 * b + 8 * j + 4 * h + (lane & 3)) * 2, at * kMetaBytes, 0);
+    w.s = __builtin_amdgcn_raw_buffer_load_b16(rec, (32 * b + r) * 2, at * kMetaBytes, 0);
   }
 }
 
@@ -148,10 +146,11 @@ __device__ __forceinline__ void a8_fmac_quad(float& y, float s, float f) {
     asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
 }
 
-// One group: the MFMAs over buf with the weights w, while the loads of group gn go out. Four
-// sums of the block before are scaled behind each MFMA, and the operand that it has taken is
-// read for the block after; the fences keep that order. sw: in each four lanes the scales of
-// four neighbouring rows, for a v_fmac that takes its factor from one of them.
+// One group: the MFMAs over buf with the weights w, while the loads of group gn go out. Behind
+// each MFMA the operand that it has taken is read for the block after; a block's sums are
+// scaled once its four MFMAs are out, and the fences keep the blocks in order. sx: in each four
+// lanes the scales of four neighbouring rows of x, for a v_fmac that takes its factor from one
+// of them.
 template <int MB>
 __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], const A8Weights& w, A8Weights& wn,
                                          const u32x4* buf, u32x4* nbuf, const A8Rows& x, const A8Src& src, bool more,
@@ -165,7 +164,12 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
   auto code = [&](int mb, int o) { return buf[(32 * mb + r) * 8 + ((4 * (o >> 1) + 2 * h + (o & 1)) ^ swz)]; };
 #pragma unroll
   for (int o = 0; o < 4; ++o) v[o] = code(0, o);
-  float sx = scales[r];
+  float sx[4];               // of rows 8 j + 4 h + lane % 4
+  auto row_scales = [&](int mb) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sx[j] = scales[32 * mb + 8 * j + 4 * h + (lane & 3)];
+  };
+  row_scales(0);
   i32x4 op[4];               // chunk s = 0 low, high nibbles, s = 1 low, high
 #pragma unroll
   for (int s = 0; s < 2; ++s)
@@ -174,9 +178,7 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
       op[2 * s][i] = (int)a8_less(w.q[s][i] & 0x0F0F0F0Fu, z);
       op[2 * s + 1][i] = (int)a8_less((w.q[s][i] >> 4) & 0x0F0F0F0Fu, z);
     }
-  float sw[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) sw[j] = bf16_bits_to_f32(w.s[j]);
+  const float sw = bf16_bits_to_f32(w.s), less = -kA8Magic * sw;
   i32x16 start;
 #pragma unroll
   for (int i = 0; i < 16; ++i) start[i] = kA8Start;
@@ -184,13 +186,13 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     i32x16 c = start;
-    const float fx = a8_scale(sx), less = -kA8Magic * fx;
+    const float fx[4] = {sx[0], sx[1], sx[2], sx[3]};
 #pragma unroll
     for (int o = 0; o < 4; ++o) {
-      c = __builtin_amdgcn_mfma_i32_32x32x32_i8(op[o], __builtin_bit_cast(i32x4, v[o]), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, v[o]), op[o], c, 0, 0, 0);
       if (mb + 1 < MB) {
         v[o] = code(mb + 1, o);
-        if (o == 0) sx = scales[32 * (mb + 1) + r];
+        if (o == 0) row_scales(mb + 1);
       }
     }
 #pragma unroll
@@ -205,12 +207,12 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
     for (int o = 0; o < 4; ++o) {
       float f[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = __builtin_fmaf(__int_as_float(c[4 * o + i]), fx, less);
+      for (int i = 0; i < 4; ++i) f[i] = __builtin_fmaf(__int_as_float(c[4 * o + i]), sw, less);
       float* y = acc[mb] + 4 * o;
-      a8_fmac_quad<0>(y[0], sw[o], f[0]);
-      a8_fmac_quad<1>(y[1], sw[o], f[1]);
-      a8_fmac_quad<2>(y[2], sw[o], f[2]);
-      a8_fmac_quad<3>(y[3], sw[o], f[3]);
+      a8_fmac_quad<0>(y[0], fx[o], f[0]);
+      a8_fmac_quad<1>(y[1], fx[o], f[1]);
+      a8_fmac_quad<2>(y[2], fx[o], f[2]);
+      a8_fmac_quad<3>(y[3], fx[o], f[3]);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -329,10 +331,10 @@ __device__ __forceinline__ void a8_store(const A8Args& a, const float (&acc)[MB]
       if (p0 + k >= MB || (KS == 2 && half)) break;
       const float(&v)[16] = acc[p0 + k < MB ? p0 + k : 0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        lds[(32 * k + r) * kChunks + ((8 * wave + 2 * j + h) ^ (r & 15))] =
-            u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-                  __float_as_uint(v[4 * j + 3])};
+      for (int i = 0; i < 16; ++i) {
+        const int row = 8 * (i >> 2) + 4 * h + (i & 3);
+        reinterpret_cast<float*>(lds + (32 * k + row) * kChunks + ((8 * wave + (r >> 2)) ^ (row & 15)))[r & 3] = v[i];
+      }
     }
     __syncthreads();
     const int rows = 32 * (p0 + kPass <= MB ? kPass : MB - p0);
@@ -443,10 +445,26 @@ __global__ __launch_bounds__(64 * kA8Waves * KS, 2) void k_a8_tiles(A8Tiles t) {
   }
 }
 
-// The cut tiles: a wave sums a quarter of a block (wave w, m-block mb, 8 j .. 8 j + 7 of its
-// columns; gated: of gate and up) over its pieces, in order, kAhead of them loaded at a time,
-// and stores it.
+// The cut tiles: a wave sums a quarter of a block (wave w, m-block mb, rows 8 j .. 8 j + 7 of
+// it; gated: of gate and up) over its pieces, in order, kAhead of them loaded at a time, and
+// stores it: a lane has four rows of a column, and takes four columns of a row from its four.
 constexpr int kA8Quarters = 4;
+
+// A 4 x 4 block in four lanes, turned: v[i] of lane j to v[j] of lane i.
+template <int CTRL>
+__device__ __forceinline__ void a8_swap(float& low, float& high, bool second) {
+  const int give = __float_as_int(second ? low : high);
+  const float got = __int_as_float(__builtin_amdgcn_update_dpp(give, give, CTRL, 0xf, 0xf, false));
+  low = second ? got : low;
+  high = second ? high : got;
+}
+__device__ __forceinline__ void a8_turn_quad(float (&v)[4], int lane) {
+  const bool odd = lane & 1, upper = lane & 2;
+  a8_swap<0xB1>(v[0], v[1], odd);     // quad_perm [1, 0, 3, 2]
+  a8_swap<0xB1>(v[2], v[3], odd);
+  a8_swap<0x4E>(v[0], v[2], upper);   // quad_perm [2, 3, 0, 1]
+  a8_swap<0x4E>(v[1], v[3], upper);
+}
 
 template <int MB, int OUT>
 __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
@@ -460,8 +478,8 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
   int tn, tm;
   a8_tile_coords(t, t.full + ts, tn, tm);
   const A8Wave wv = a8_wave<OUT>(a, tn, w);
-  const int lane = threadIdx.x, r = lane & 31, h = lane >> 5, m = tm * 32 * MB + 32 * mb + r;
-  if (!wv.valid || tm * 32 * MB + 32 * mb >= a.M) return;
+  const int lane = threadIdx.x, m0 = tm * 32 * MB + 32 * mb + 8 * j, m = m0 + 4 * (lane >> 5) + (lane & 3);
+  if (!wv.valid || m0 >= a.M) return;
   const __amdgpu_buffer_rsrc_t rs = a8_rsrc(t.slots, 2u * t.P * kA8SlotBytes);
   float acc[NP][4] = {};
   for (int pp = p0; pp <= p1; pp += kAhead) {
@@ -483,8 +501,10 @@ __global__ __launch_bounds__(64) void k_a8_fixup(A8Tiles t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[p][i] += __uint_as_float(v[k][p][i]);
   }
+#pragma unroll
+  for (int p = 0; p < NP; ++p) a8_turn_quad(acc[p], lane);
   if (m >= a.M) return;
-  const int col = wv.col + 8 * j + 4 * h;
+  const int col = wv.col + (lane & 28);
   const size_t at = (size_t)m * a.ld + col;
   if constexpr (OUT == A8_F32) {
     *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = f32x4{acc[0][0], acc[0][1], acc[0][2], acc[0][3]};
