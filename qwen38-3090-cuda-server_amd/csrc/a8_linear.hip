@@ -132,18 +132,17 @@ __device__ __forceinline__ void a8_load_rows(const A8Args& a, const A8Rows& x, u
   }
 }
 
-// y += f times lane I's s of each lane's four. I = 0 waits as a register that a vector
-// instruction has written needs before it is read across lanes.
-template <int I>
-__device__ __forceinline__ void a8_fmac_quad(float& y, float s, float f) {
-  if constexpr (I == 0)
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
-  else if constexpr (I == 1)
-    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
-  else if constexpr (I == 2)
-    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
-  else
-    asm("v_fmac_f32_dpp %0, %1, %2 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf" : "+v"(y) : "v"(s), "v"(f));
+// y[i] += f[i] times lane i's s of each lane's four. One block, whose wait is what a register
+// that a vector instruction has written needs before it is read across lanes: whatever the
+// compiler puts before it, a copy of s included, is far enough.
+__device__ __forceinline__ void a8_fmac_quad(float* y, float s, const float (&f)[4]) {
+  asm("s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %4, %5 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %1, %4, %6 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %2, %4, %7 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %3, %4, %8 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf"
+      : "+&v"(y[0]), "+&v"(y[1]), "+&v"(y[2]), "+&v"(y[3])
+      : "v"(s), "v"(f[0]), "v"(f[1]), "v"(f[2]), "v"(f[3]));
 }
 
 // One group: the MFMAs over buf with the weights w, while the loads of group gn go out. Behind
@@ -208,11 +207,7 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
       float f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = __builtin_fmaf(__int_as_float(c[4 * o + i]), sw, less);
-      float* y = acc[mb] + 4 * o;
-      a8_fmac_quad<0>(y[0], fx[o], f[0]);
-      a8_fmac_quad<1>(y[1], fx[o], f[1]);
-      a8_fmac_quad<2>(y[2], fx[o], f[2]);
-      a8_fmac_quad<3>(y[3], fx[o], f[3]);
+      a8_fmac_quad(acc[mb] + 4 * o, fx[o], f);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
