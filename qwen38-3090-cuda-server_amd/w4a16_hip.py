@@ -771,9 +771,12 @@ def a8_over(q, scale) -> A8Rows:
     int8 (in the order that qw4_a8 describes) and scale [in_f / 128][max_rows] fp32."""
     if _same is None:
         _types()
+    if q.dim() != 2 or q.shape[1] % 128:
+        raise ValueError(f"a8_over q: shape {tuple(q.shape)}, needs rows of whole groups of 128")
     (rows, in_f), dev = q.shape, max(q.get_device(), 0)   # both on one GPU, the current one or not
-    return A8Rows(_buf(q, _i8, 0, dev, "a8_over q"),
-                  _buf(scale, _f32, rows * (in_f // 128) * 4, dev, "a8_over scale"), rows, in_f)
+    if tuple(scale.shape) != (in_f // 128, rows):
+        raise ValueError(f"a8_over scale: shape {tuple(scale.shape)}, needs {(in_f // 128, rows)}")
+    return A8Rows(_buf(q, _i8, 0, dev, "a8_over q"), _buf(scale, _f32, 0, dev, "a8_over scale"), rows, in_f)
 
 
 def a8_free(a: A8Rows) -> None:
