@@ -9,7 +9,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "../../include/qwen_w4a16.h"
 #include "a8.h"
@@ -567,19 +566,6 @@ A8Plan a8_plan(int M, int cols, int G, int ks, int mb, int cus, bool ws_ok) {
   return p;
 }
 
-int device_cus() {
-  static std::once_flag once[64];
-  static int cus[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  std::call_once(once[dev], [dev] {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cus[dev] = n;
-  });
-  return cus[dev];
-}
-
 template <int OUT, int MB>
 void launch_tiles(const A8Tiles& t, int ks, int grid, int nt, hipStream_t s) {
   if (ks == 1) {
@@ -594,11 +580,11 @@ void launch_tiles(const A8Tiles& t, int ks, int grid, int nt, hipStream_t s) {
 
 template <int OUT>
 int run(const A8Args& a, qw4_workspace* ws, hipStream_t s) {
-  if (a8_few(OUT, a, device_cus(), s)) {
+  const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
+  if (a8_few(OUT, a, cus, s)) {
     QW4_LAUNCH_CHECK();
     return QW4_OK;
   }
-  const int cus = device_cus(), cols = OUT == A8_GLU ? 2 * a.ld : a.ld;
   const bool ws_ok = ws && ws->buf && ((uintptr_t)ws->buf & 255) == 0 && cus % 8 == 0 &&
                      ws->bytes >= 2ull * kPerCu * cus * kA8SlotBytes;
   A8Plan p = a8_plan(a.M, cols, a.G, 1, 8, cus, ws_ok);

@@ -12,7 +12,6 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
-#include <mutex>
 
 #include <algorithm>
 #include <cstdlib>
@@ -397,20 +396,6 @@ __global__ __launch_bounds__(64 * NW, 1) void k_gemm(GemmArgs a) {
 
 // Workspace bytes that enable stream-K: two fp32 partial tiles per CU.
 size_t gemm_workspace_need(int cus) { return 2ull * (size_t)cus * kSlotBytes; }
-
-int device_cus() {
-  static std::once_flag once[64];
-  static int cus[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  std::call_once(once[dev], [dev] {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-      n = 256;
-    cus[dev] = n;
-  });
-  return cus[dev];
-}
 
 // Tuning and test override of the prefill schedule (qw4_tune_gemm): -1 the
 // cost model, 0 per tile, 1 stream-K, 2 hybrid, 3 split-K.

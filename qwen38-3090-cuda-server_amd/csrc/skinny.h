@@ -558,26 +558,6 @@ __device__ __forceinline__ void emit_swiglu(const SkinnyArgs& a, int b, int st0,
 }
 
 // ------------------------------------------------------------- host side
-constexpr int kMaxDevices = 64;
-
-inline int current_device() {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
-  return dev;
-}
-// The current device's CUs.
-inline int device_cus() {
-  static std::atomic<int> cus[kMaxDevices];
-  std::atomic<int>& v = cus[current_device()];
-  int n = v.load(std::memory_order_relaxed);
-  if (!n) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, current_device()) != hipSuccess || n <= 0)
-      n = 256;
-    v.store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 // Dynamic LDS above the default limit is allowed per kernel, once per device:
 // qw4_scratch_alloc raises every LDS-DMA kernel to its maximum, so no launch --
 // captured into a graph or not -- has to. A launch that needs more than a

@@ -30,6 +30,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/qwen_w4a16.h"
 
 namespace qw4 {
@@ -164,6 +166,26 @@ void launch_rows_of(int rows, int most, const F& f) {
     f(first, n);
     first += n;
   } while (first < rows);
+}
+
+constexpr int kMaxDevices = 64;
+
+inline int current_device() {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
+  return dev;
+}
+// The current device's CUs.
+inline int device_cus() {
+  static std::atomic<int> cus[kMaxDevices];
+  std::atomic<int>& v = cus[current_device()];
+  int n = v.load(std::memory_order_relaxed);
+  if (!n) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, current_device()) != hipSuccess || n <= 0)
+      n = 256;
+    v.store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 }  // namespace qw4
 #define QW4_LAUNCH_CHECK()                                   \
