@@ -341,7 +341,13 @@ bool launch_few(const FewArgs& f, hipStream_t st) {
     if (M <= 8) return launch16<OUT, S, 2>(f, st);
     if (M <= 16) return launch16<OUT, S, 4>(f, st);
     if (G <= 40) return launch<OUT, S, 5, 8, D, 2, 4>(f, st);
-    return G <= 80 && launch<OUT, S, 10, 8, D, 2, 4>(f, st);
+    // gated, codes of more than 8 groups a wave do not fit beside the sums: 32 rows of 34816 x 8192
+    // 34.2 us, as tiles 39.9, with spills 43.9; of 28672 x 10240 as tiles 36.6, with spills 41.6.
+    // Of few columns tiles in slices are the faster: 4096 x 8192 12.8 and 15.5
+    if constexpr (OUT == A8_GLU)
+      return G <= 64 && launch<OUT, S, 8, 8, D, 2, 4>(f, st);
+    else
+      return G <= 80 && launch<OUT, S, 10, 8, D, 2, 4>(f, st);
   }
   return false;
 }
