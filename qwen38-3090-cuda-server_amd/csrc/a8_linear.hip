@@ -84,27 +84,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t a8_rsrc(const void* p, uint32_
 }
 
 // Part 0: the words and zero points of group g, part 1: the scale. A group of which there
-// is not `some` is out of its resource's range: no memory, no branch. Tiles of 8 blocks have
-// one resource for all groups and an offset, others one a group: 4096 rows of 34816 x 5120
-// take 0.883 and 0.930 ms in these forms, 1001 of 5120 x 4096 (of fewer blocks) 40.8 and 39.2 us.
-template <int MB>
-__device__ __forceinline__ void a8_load_weights(A8Weights& w, const A8Src& src, int b, int g, int G, bool some,
-                                                int lane, int part) {
-  constexpr bool kOne = MB == 8;
+// is not `some` has a resource of no length: no memory, no branch.
+__device__ __forceinline__ void a8_load_weights(A8Weights& w, const A8Src& src, int b, int g, bool some, int lane,
+                                                int part) {
   const int r = lane & 31, h = lane >> 5;
-  const int pos = tile_pos_of_row(32 * b + r);
-  const int at = kOne ? (some ? g : G) : 0;
-  const uint32_t groups = kOne ? (uint32_t)G : some ? 1u : 0u;
-  const size_t base = kOne ? 0 : (size_t)g;
-  const __amdgpu_buffer_rsrc_t rec = a8_rsrc(src.sc + base * kMetaU16, groups * kMetaBytes);
+  const __amdgpu_buffer_rsrc_t rec = a8_rsrc(src.sc + (size_t)g * kMetaU16, some ? (uint32_t)kMetaBytes : 0u);
   if (part == 0) {
-    const __amdgpu_buffer_rsrc_t qw = a8_rsrc(src.qw + base * kWordsPerBlock, groups * 4096u);
+    const __amdgpu_buffer_rsrc_t qw = a8_rsrc(src.qw + (size_t)g * kWordsPerBlock, some ? 4096u : 0u);
+    const int pos = tile_pos_of_row(32 * b + r);
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-      w.q[s] = __builtin_amdgcn_raw_buffer_load_b128(qw, ((2 * s + h) * 64 + pos) * 16, at * 4096, 0);
-    w.z = __builtin_amdgcn_raw_buffer_load_b16(rec, 128 + (8 * b + (r >> 2)) * 2, at * kMetaBytes, 0);
+    for (int s = 0; s < 2; ++s) w.q[s] = __builtin_amdgcn_raw_buffer_load_b128(qw, ((2 * s + h) * 64 + pos) * 16, 0, 0);
+    w.z = __builtin_amdgcn_raw_buffer_load_b16(rec, 128 + (8 * b + (r >> 2)) * 2, 0, 0);
   } else {
-    w.s = __builtin_amdgcn_raw_buffer_load_b16(rec, (32 * b + r) * 2, at * kMetaBytes, 0);
+    w.s = __builtin_amdgcn_raw_buffer_load_b16(rec, (32 * b + r) * 2, 0, 0);
   }
 }
 
@@ -197,7 +189,7 @@ __device__ __forceinline__ void a8_group(const A8Args& a, float (&acc)[MB][16], 
     for (int p = 0; p < Sp::ACT + 3; ++p)
       if (p * MB / 2 / (Sp::ACT + 3) == mb) {
         if (p < 2)
-          a8_load_weights<MB>(wn, src, b, gn, a.G, more, lane, p);
+          a8_load_weights(wn, src, b, gn, more, lane, p);
         else
           a8_load_rows<MB>(a, x, voff, nbuf, gn, more, wave, lane, p - 2);
       }
@@ -239,7 +231,7 @@ __device__ __forceinline__ void a8_segment(const A8Args& a, float (&acc)[MB][16]
 #pragma unroll
     for (int p = 0; p <= Sp::ACT; ++p) a8_load_rows<MB>(a, x, voff, lds + d * Sp::UNITS, g0 + d, in, wave, lane, p);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) a8_load_weights<MB>(w[d], src, b, g0 + d, a.G, in, lane, p);
+    for (int p = 0; p < 2; ++p) a8_load_weights(w[d], src, b, g0 + d, in, lane, p);
   }
   for (int gb = g0; gb < end; gb += D) {
 #pragma unroll
