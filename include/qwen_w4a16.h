@@ -505,7 +505,8 @@ int qw4_a8_linear_f32(float* y, const qw4_weights* w, const qw4_a8* a, int T, qw
  *   entropy [T]         -sum p log p, p = exp(x - L); may be NULL
  *   top_ids, top_lp [T][top_k]   the top_k (0..32) largest, largest first, the lower index
  *                       among equals, and x - L of each; both NULL with top_k = 0
- * asked >= 0 targets a row (lp and targets NULL with 0). In fp32. -Inf is a masked token:
+ * asked >= 0 targets a row (lp and targets NULL with 0). In fp32, the sums too (off by some
+ * 1e-7 of themselves). -Inf is a masked token:
  * never chosen (id -1, -Inf, also behind the last that there is), lp -Inf; a row of
  * nothing else has entropy 0. NaN or +Inf in a row make its numbers NaN (ids still go by
  * the other logits; NaN is never chosen). The reference has only argmax over rows

@@ -1,7 +1,7 @@
 // Products of few rows in 8 bits (1 to 16, for shorter K up to 64, in one reading of the
 // weights): qw4_a8_linear's decode, verify and small batches. HBM-bound: one / 9 / 16 / 32
-// rows of 34816 x 5120 gated 18.2 / 20.0 / 20.3 / 24.8 us (93 MB: 5.1 TB/s of one row), 9 of
-// 248320 x 5120 in fp32 105.5 (6.4 TB/s), 48 159; of small weights the launch and the first loads:
+// rows of 34816 x 5120 gated 17.9 / 19.6 / 20.3 / 24.8 us (93 MB: 5.2 TB/s of one row), 9 of
+// 248320 x 5120 in fp32 105.8 (6.3 TB/s), 48 156; of small weights the launch and the first loads:
 // one row of 5120 x 4096 5.1 us.
 //
 // Workgroup p owns whole units (S row quads of a tile, 16 or 32 weight rows, over all of
@@ -324,14 +324,14 @@ bool launch16(const FewArgs& f, hipStream_t st) {
 }
 
 // More than 32 rows in gated units of 16 rows each: those of 32 have twice the sums, which do
-// not fit the registers beside the codes (48 rows of 34816 x 5120 30.9 and 44.8 us).
+// not fit the registers beside the codes (48 rows of 34816 x 5120 30.3 and 44.8 us).
 template <int OUT, int S>
 bool launch_few(const FewArgs& f, hipStream_t st) {
   constexpr int D = OUT == A8_GLU ? 2 : 3;
   const int G = f.a.G, M = f.a.M;
   if constexpr (OUT != A8_GLU || S == 1) {
-    // 48 rows of 7168 x 5120 12.6 us, as tiles 16.5, of 5120 x 4096 10.3 and 13.3, of 34816 x 5120
-    // gated 30.9 and 37.5; 64 of 5120 x 2048 9.2 and 10.2, but of 5120 x 4096 14.7 and 13.4, and
+    // 48 rows of 7168 x 5120 12.8 us, as tiles 15.7, of 5120 x 4096 10.3 and 12.4, of 34816 x 5120
+    // gated 30.3 and 36.7; 64 of 5120 x 2048 9.1 and 10.0, but of 5120 x 4096 14.7 and 12.7, and
     // with more units than workgroups, of 34816 x 2048 gated, 21.6 and 19.0
     if (M > 48) return G <= 24 && f.P >= f.U && launch<OUT, S, 3, 8, D, 4, 4>(f, st);
     if (M > 32) return G <= 40 && launch<OUT, S, 5, 8, D, 3, 4>(f, st);

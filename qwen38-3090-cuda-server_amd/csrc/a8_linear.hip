@@ -24,13 +24,13 @@ namespace {
 // k_a8_tiles: 128 columns (rows of W) x 32 MB rows of x a workgroup of 4 waves; a wave owns
 // 32 columns against all the tile's rows, in MB blocks of 32 x 32. Two workgroups fit a CU, so
 // that one's vector instructions run beside the other's MFMAs: 4096 rows of 34816 x 5120 take
-// 0.88 ms (1.66 POP/s: vector instructions 65% and MFMAs 41% of the cycles), in a first form with one
+// 0.88 ms (1.66 POP/s: vector instructions 65% and MFMAs 42% of the cycles), in a first form with one
 // workgroup of 8 waves and 256 columns a CU 1.04.
 //
 // In halves (KS = 2, tiles of up to 4 blocks) a workgroup has 8 waves, the second four take the
 // second half of the groups, and the sums meet in LDS: half as many slices for as many waves.
-// 77 rows of 5120 x 17408 26 us (29.6 in whole workgroups), 96 of 34816 x 5120 44 (50), 512 of
-// 5120 x 4096 25 (31). Other sizes lose: 256 of 5120 x 17408 50.5 against 49.
+// 77 rows of 5120 x 17408 25 us (28 in whole workgroups), 96 of 34816 x 5120 44 (48), 512 of
+// 5120 x 4096 24 (30). Other sizes lose: 256 of 5120 x 17408 47.6 against 46.8.
 //
 //  * Weights (the MFMA's B operand) come straight into registers, a lane the 32 bytes of
 //    its row and half of a group: every weight is unpacked once per workgroup, 7 vector
@@ -522,7 +522,7 @@ struct A8Plan {
 
 // The best cut of tiles of mb rows. The estimate's figures are fitted to 2100 timed calls on
 // MI355X (15 projections from 2048x2048 to 248320x5120, 24 to 4096 rows, every ks, mb,
-// schedule and S): over its 110 sizes the pick is 1.2% (geometric mean) from the fastest of
+// schedule and S, with steps some 4% longer than now): over its 110 sizes the pick is 1.2% (geometric mean) from the fastest of
 // all, 11% at worst (64 rows and fewer of 2048x2048). A (tile, group) step takes `one` us with
 // one workgroup on a CU and `two` with two, or with one in halves; then come storing a tile, the
 // second kernel that joins slices, and their partial tiles' traffic. All units over all

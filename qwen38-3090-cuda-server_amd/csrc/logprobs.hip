@@ -9,6 +9,9 @@
 // With total = 1 + s:  L = m + log1p(s),  H = log1p(s) - u / (1 + s). Without the
 // largest element s keeps its relative precision when that token is all but certain,
 // where 1 + s would lose it and both results are about s.
+// All of it in fp32: a lane sums n / (256 S) terms, S the splits of the row, the joins some 16,
+// so that s is off by (n / 256 + 80) 2^-24 of itself at most, by some 1e-7 in fact; sums in 64 bits
+// come 1.5 to 4 times as near, which logits of 8 or 24 bits have no use for.
 //
 // Alternatives: a lane keeps the six largest maxima of its eights as keys (the upper 16
 // bits of the value, ordered, over the block's number): 2 vector instructions a logit,
