@@ -62,8 +62,8 @@ def test_sizes_and_types(hip):
         hip.a8_dequant_rows(x, a, 0, 5, stream=0)
     with pytest.raises(ValueError, match="linear_w4a8 y: type torch.float32, needs torch.bfloat16"):
         hip.linear_w4a8(torch.zeros(4, 256), w, a, 4, stream=0)
-    with pytest.raises(ValueError, match="linear_w4a8_f32 y: buffer holds 3072 bytes, needs 4096"):
-        hip.linear_w4a8_f32(torch.zeros(3, 256), w, a, 4, stream=0)
+    with pytest.raises(ValueError, match="linear_w4a8_f32 y: buffer holds 2048 bytes, needs 4096"):
+        hip.linear_w4a8_f32(torch.zeros(2, 256), w, a, 4, stream=0)
     with pytest.raises(ValueError, match="logprobs logits: needs 4 rows of 100"):
         hip.logprobs(torch.zeros(4), torch.zeros(4, 99), torch.zeros(4, dtype=torch.int32), 4, 100, stream=0)
     for targets in (0x3000, torch.zeros(4, 1, 1, dtype=torch.int32), torch.zeros((), dtype=torch.int32)):
